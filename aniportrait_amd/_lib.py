@@ -10,7 +10,7 @@ import os
 HERE = os.path.dirname(os.path.abspath(__file__))
 # ANIP_LIB: an experiment build of the same ABI (aniportrait_amd/build.py --out=...); the product is the default path
 LIB_PATH = os.environ.get("ANIP_LIB") or os.path.join(HERE, "lib", "libaniportrait_hip.so")
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 c_void_p, c_int, c_int64, c_float = C.c_void_p, C.c_int, C.c_int64, C.c_float
 
@@ -35,6 +35,37 @@ class GemmParams(C.Structure):
         ("trans_out", c_int),
         ("workspace", c_void_p), ("workspace_bytes", c_int64),
         ("head_dim", c_int),
+    ]
+
+
+class QkNormParams(C.Structure):
+    """mirror of `struct anip_qk_norm_params`"""
+    _fields_ = [
+        ("dtype", c_int), ("B", c_int), ("T", c_int), ("Hq", c_int), ("Hkv", c_int), ("d", c_int), ("rot", c_int), ("interleaved", c_int),
+        ("eps", c_float), ("q_alpha", c_float),
+        ("q", c_void_p), ("q_stride", c_int64 * 3), ("k", c_void_p), ("k_stride", c_int64 * 3),
+        ("q_weight", c_void_p), ("k_weight", c_void_p),
+        ("rope", c_void_p), ("rope_rows", c_int), ("positions", c_void_p),
+        ("q_out", c_void_p), ("q_out_stride", c_int64 * 3), ("k_out", c_void_p), ("k_out_stride", c_int64 * 3),
+        ("dq_out", c_void_p), ("dq_out_stride", c_int64 * 3), ("dk_out", c_void_p), ("dk_out_stride", c_int64 * 3),
+        ("dq_weight", c_void_p), ("dk_weight", c_void_p),
+        ("ws", c_void_p), ("ws_floats", c_int64),
+    ]
+
+
+class AttnParams(C.Structure):
+    """mirror of `struct anip_attn_params`"""
+    _fields_ = [
+        ("dtype", c_int), ("B", c_int), ("Tq", c_int), ("Tk", c_int), ("H", c_int), ("Hkv", c_int), ("d", c_int), ("causal", c_int),
+        ("scale", c_float),
+        ("q", c_void_p), ("q_stride", c_int64 * 3), ("k", c_void_p), ("k_stride", c_int64 * 3), ("v", c_void_p), ("v_stride", c_int64 * 3),
+        ("kv_lens", c_void_p), ("q_start", c_void_p),
+        ("table", c_void_p), ("buckets", c_void_p), ("n_buckets", c_int), ("max_distance", c_int),
+        ("lam", c_void_p),
+        ("out", c_void_p), ("out2", c_void_p), ("lse", c_void_p),
+        ("dout", c_void_p), ("dout_stride", c_int64 * 3),
+        ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p), ("dtable", c_void_p), ("dlam", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
     ]
 
 
@@ -78,6 +109,15 @@ SIGNATURES = {
     "anip_temporal_qkv_attention_supported": (c_int, [c_int, c_int, c_int, c_int]),
     "anip_temporal_qkv_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                             c_int, c_float, c_float, c_void_p]),
+    "anip_qk_norm_rope": (c_int, [C.POINTER(QkNormParams), c_void_p]),
+    "anip_qk_norm_rope_backward_ws_floats": (c_int64, [c_int64, c_int, c_int]),
+    "anip_qk_norm_rope_backward": (c_int, [C.POINTER(QkNormParams), c_void_p]),
+    "anip_relative_attention_ws_bytes": (c_int64, [C.POINTER(AttnParams), c_int]),
+    "anip_relative_attention": (c_int, [C.POINTER(AttnParams), c_void_p]),
+    "anip_relative_attention_backward": (c_int, [C.POINTER(AttnParams), c_void_p]),
+    "anip_differential_attention_ws_bytes": (c_int64, [C.POINTER(AttnParams), c_int]),
+    "anip_differential_attention": (c_int, [C.POINTER(AttnParams), c_void_p]),
+    "anip_differential_attention_backward": (c_int, [C.POINTER(AttnParams), c_void_p]),
     "anip_softmax_rows": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "anip_linear_small": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "anip_add": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
@@ -96,7 +136,7 @@ SIGNATURES = {
                                              C.POINTER(c_int), C.POINTER(c_float), C.POINTER(c_int64)]),
     "anip_profile_kernel_name": (C.c_char_p, [c_int]),
 }
-N_KERNEL_IDS = 12  # ANIP_K_COUNT
+N_KERNEL_IDS = 15  # ANIP_K_COUNT
 
 _lib = None
 

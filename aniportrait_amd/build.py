@@ -12,7 +12,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libaniportrait_hip.so")
-SOURCES = ["gemm.hip", "gemm2.hip", "ffn.hip", "tblock.hip", "norm.hip", "convbn.hip", "attention.hip", "attn_dma.hip", "elementwise.hip", "api.cpp"]
+SOURCES = ["gemm.hip", "gemm2.hip", "ffn.hip", "tblock.hip", "norm.hip", "convbn.hip", "attention.hip", "attn_dma.hip", "elementwise.hip",
+           "headnorm.hip", "mapattn_fwd.hip", "mapattn_bwd.hip", "mapattn.cpp", "api.cpp"]
 ARCH = "gfx950"
 # no packed fp32 instructions (v_pk_fma_f32 and the like): some of their forms have given wrong results now and then on this
 # hardware.  The scalar forms round the same.  (hipcc's host pass does not know the feature and says so.)

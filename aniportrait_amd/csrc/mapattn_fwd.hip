@@ -1,0 +1,546 @@
+// Forward of the attention of mapattn.h: 128 queries of one head per workgroup (4 waves x 32), tiles of KT keys in two LDS
+// stages, one pass over the keys with running maxima and sums (base 2).  S^T = K Q^T per 32 keys, so that a lane owns one query:
+// its maximum and sum are 16 register operations and one exchange between the half-waves, and P^T is the B operand of
+// O^T += V^T P^T as it lies.  Differential attention gives each of its two
+// maps a wave of its own (two accumulators of 2 d channels would not fit one wave's registers from d = 64 on); both read the same
+// V tile, and the second hands its share to the first at the end.
+#include "mapattn.h"
+
+using namespace mapattn;
+
+namespace {
+
+constexpr float THR = 8.0f;  // the running maximum is raised when a score exceeds it by more: P <= 2^8
+
+// one map's running softmax over the 32 scores-per-lane-pair of a sub-tile: scores s (x = mul s + add in base 2) -> P fragments
+template <typename T, int NT>
+__device__ __forceinline__ void soft_step(f32x16& s, float mul, float add, float& m, float& l, f32x16 (&o)[NT], u32x4 (&p)[2]) {
+  float mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
+#pragma unroll
+  for (int r = 3; r < 15; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
+  mx = xor32_max(fmaxf(mx, s[15]));
+  mx = fmaf(mx, mul, add);
+  if (__any(mx - m > THR)) {  // always on the first seen key (m = -inf); never while both are -inf (NaN > THR is false)
+    const float mn = fmaxf(m, mx);
+    const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[nt][r] *= alpha;
+  }
+  const float c = add - (m == -INFINITY ? 0.f : m);
+  float t = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, c));
+    t += s[r];
+  }
+  l += t;
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[kb][i] = Num<T>::pack(s[8 * kb + 2 * i], s[8 * kb + 2 * i + 1]);
+}
+
+}  // namespace
+
+template <typename T, int MAPS, int KS, int NT, int KT>
+__global__ __launch_bounds__(256 * MAPS, 2) void mapattn_fwd_kernel(const MapAttnArgs a) {
+  constexpr bool BIAS = MAPS == 1;
+  constexpr int NW = 4 * MAPS, BQ = 128;
+  constexpr int KCH = 4 * ((KS + 1) / 2), VCH = 4 * NT;
+  constexpr int K_BYTES = KT * KCH * 16, V_BYTES = KT * VCH * 16, STAGE = MAPS * K_BYTES + V_BYTES;
+  constexpr int E = BQ + KT;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  float* near = (float*)(smem + 2 * STAGE);
+
+  const int tid = threadIdx.x, lane = tid & 63, ql = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = wave / MAPS, m = wave % MAPS;  // 32 queries, and the map that this wave computes for them
+  const int nqb = (a.Tq + BQ - 1) / BQ;
+  int slot, bh;
+  if (!place(blockIdx.x, nqb * a.splits, a.B * a.H, slot, bh)) return;
+  const int split = slot % a.splits, qb = nqb - 1 - slot / a.splits;  // causal: the longest rows first
+  const int b = bh / a.H, head = bh - b * a.H, kvh = head / a.G;
+  const int len = seq_len(a, b), start = seq_start(a, b);
+  const int qi = qb * BQ + grp * 32 + ql;      // this lane's query
+  const int pw = start + qb * BQ + grp * 32;   // position of the wave's first query
+  const int lim = a.causal ? min(len - 1, start + qi) : len - 1;  // last key this lane sees
+
+  // ---- the keys this workgroup walks over -------------------------------------------------------------------------------
+  int kend = len;
+  if (a.causal) kend = min(kend, start + min(qb * BQ + BQ, a.Tq));
+  const int nt_all = kend > 0 ? (kend + KT - 1) / KT : 0;
+  const int t0 = (int)((int64_t)nt_all * split / a.splits), t1 = (int)((int64_t)nt_all * (split + 1) / a.splits);
+
+  u32x4 qf[KS];
+  load_row<KS>(qf, (const char*)a.q + 2 * (b * a.q_sb + (int64_t)qi * a.q_st + (int64_t)(head * MAPS + m) * a.q_sh), qi < a.Tq, h, a.d);
+
+  const char* kb[MAPS];
+#pragma unroll
+  for (int i = 0; i < MAPS; ++i) kb[i] = (const char*)a.k + 2 * (b * a.k_sb + (int64_t)(kvh * MAPS + i) * a.k_sh);
+  const char* vb = (const char*)a.v + 2 * (b * a.v_sb + (int64_t)kvh * a.v_sh);
+  TileDma<KCH, KT, NW> kd;
+  TileDma<VCH, KT, NW> vd;
+  kd.init(wave, lane, a.k_st, a.d);
+  vd.init(wave, lane, a.v_st, a.dv);
+  auto issue = [&](int t) {
+    char* st = smem + (t & 1) * STAGE;
+    const int64_t row = (int64_t)t * KT;
+    const int valid = len - t * KT;
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i) kd.issue(kb[i] + row * a.k_st * 2, valid, st + i * K_BYTES, wave);
+    vd.issue(vb + row * a.v_st * 2, valid, st + MAPS * K_BYTES, wave);
+  };
+  RowRead<KCH, KS> kr;
+  TrRead<VCH, NT> vr;
+  kr.init(lane);
+  vr.init(lane);
+
+  f32x16 o[NT];
+  float mrun = -INFINITY, lrun = 0.f;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) o[nt] = zero16();
+  float far_lo = 0.f, far_hi = 0.f;
+  if (BIAS) {
+    fill_near<T>(a, head, E, near, tid, 64 * NW);
+    far_lo = bias_at<T>(a, head, -a.R);
+    far_hi = bias_at<T>(a, head, a.R);
+  }
+
+  if (t0 < t1) issue(t0);
+  for (int t = t0; t < t1; ++t) {
+    MAPATTN_WAIT_DMA();
+    __syncthreads();  // tile t is there for all waves; nobody reads the other stage any more
+    if (t + 1 < t1) issue(t + 1);
+    const char* st = smem + (t & 1) * STAGE;
+    const int kt0 = t * KT;
+    if (a.causal && kt0 > pw + 31) continue;  // nothing of this tile is seen by this wave
+#pragma unroll
+    for (int sub = 0; sub < KT / 32; ++sub) {
+      const int k0 = kt0 + 32 * sub;
+      f32x16 s = zero16();
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk) s = Num<T>::mfma(kr.get(st + m * K_BYTES, sub, kk), qf[kk], s);
+      float mul = a.scale_log2, add = 0.f;
+      if (BIAS) {
+        if (k0 + 31 - pw <= -a.R) add = far_lo;
+        else if (k0 - (pw + 31) >= a.R) add = far_hi;
+        else {
+          const float* nb = near + (k0 + 4 * h - (pw + ql) + a.R + E);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mul, nb[acc_row(r)]);
+          mul = 1.f;
+        }
+      }
+      if (k0 + 31 >= len || (a.causal && k0 + 31 > pw)) {
+        const int dl = lim - k0 - 4 * h;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = acc_row(r) > dl ? -INFINITY : s[r];
+      }
+      u32x4 p[2];
+      soft_step<T, NT>(s, mul, add, mrun, lrun, o, p);
+#pragma unroll
+      for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) o[nt] = Num<T>::mfma(vr.get(st + MAPS * K_BYTES, 2 * sub + kb2, nt), p[kb2], o[nt]);
+    }
+  }
+
+  // ---- epilogue ---------------------------------------------------------------------------------------------------------
+  const float l = xor32_sum(lrun);
+  const bool none = mrun == -INFINITY;  // no key seen: the row is zeros
+  const float inv = none ? 0.f : 1.0f / l;
+  const float lse2 = none ? -INFINITY : mrun + __builtin_amdgcn_logf(l);
+  if (MAPS == 2 && a.splits == 1) {
+    // the second map's wave hands lam o2 to the first one's, lane for lane
+    float* x = (float*)smem + grp * (NT * 16 * 64) + lane;
+    __syncthreads();  // all tiles read
+    if (m == 1) {
+      const float f = inv * a.lam[head];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[(nt * 16 + r) * 64] = o[nt][r] * f;
+    }
+    __syncthreads();
+    if (m == 0) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[nt][r] = o[nt][r] * inv - x[(nt * 16 + r) * 64];
+    }
+  }
+  if (qi >= a.Tq) return;
+  const int64_t row = ((int64_t)b * a.Tq + qi) * a.H + head;
+  if (a.splits > 1) {
+    const int64_t at = ((int64_t)split * a.B * a.Tq * a.H + row) * MAPS + m;
+    float* op = a.part_o + at * a.dv;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const int c0 = nt * 32 + rq * 8 + h * 4;
+        if (c0 < a.dv) *(f32x4*)(op + c0) = f32x4{o[nt][4 * rq] * inv, o[nt][4 * rq + 1] * inv, o[nt][4 * rq + 2] * inv, o[nt][4 * rq + 3] * inv};
+      }
+    if (h == 0) a.part_l[at] = lse2;
+    return;
+  }
+  if (a.lse && h == 0) a.lse[((int64_t)bh * MAPS + m) * a.Tq + qi] = lse2 * LN2;
+  char* op = (char*)(m == 0 ? a.out : a.out2);
+  if (op == nullptr) return;
+  op += row * a.dv * 2;
+  const float f = (MAPS == 2 && m == 0) ? 1.0f : inv;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) {
+      const int c0 = nt * 32 + rq * 8 + h * 4;
+      if (c0 < a.dv)
+        *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(o[nt][4 * rq] * f, o[nt][4 * rq + 1] * f), Num<T>::pack(o[nt][4 * rq + 2] * f, o[nt][4 * rq + 3] * f)};
+    }
+}
+
+// ---- single tokens: few queries against many keys -----------------------------------------------------------------------
+// The Tq x G queries that share a key head are at most 32 columns of one tile.  Bound by reading the keys and values once, so a
+// team of MAPS waves (one for each map, sharing the V tile) walks its own 32-key tiles with its own two LDS stages; the kw = NTEAM
+// teams of a workgroup share a problem (tiles t, t + kw, ..) and join their results in LDS, or each team has its own problem
+// (kw = 1: many short sequences).  A team of one wave waits for its own DMA alone and needs no barrier.
+template <typename T, int MAPS, int KS, int NT, int NTEAM>
+__global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(const MapAttnArgs a) {
+  constexpr bool BIAS = MAPS == 1;
+  constexpr int KT = 32;
+  constexpr int KCH = 4 * ((KS + 1) / 2), VCH = 4 * NT;
+  constexpr int K_BYTES = KT * KCH * 16, V_BYTES = KT * VCH * 16, STAGE = MAPS * K_BYTES + V_BYTES;
+  constexpr int OW = NT * 16 * 64;  // floats of a wave's result
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+
+  const int tid = threadIdx.x, lane = tid & 63, ql = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int team = wave / MAPS, m = wave % MAPS;
+  const int ppb = NTEAM / a.kw, kwi = team % a.kw;
+  const int problems = a.B * a.Hkv * a.splits;
+  const int prob = blockIdx.x * ppb + team / a.kw;
+  const bool live = prob < problems;  // (kw = NTEAM: the same for all waves)
+  const int split = prob % a.splits, bk = live ? prob / a.splits : 0;
+  const int b = bk / a.Hkv, kvh = bk - b * a.Hkv;
+  const int len = live ? seq_len(a, b) : 0, start = seq_start(a, b);
+  const int nrow = a.Tq * a.G;
+  const int qi = ql / a.G, head = kvh * a.G + (ql - qi * a.G);
+  const bool mine = live && ql < nrow;
+  const int lim = mine ? (a.causal ? min(len - 1, start + qi) : len - 1) : -1;
+
+  int kend = len;
+  if (a.causal) kend = min(kend, start + a.Tq);
+  const int nt_all = kend > 0 ? (kend + KT - 1) / KT : 0;
+  const int t0 = (int)((int64_t)nt_all * split / a.splits), t1 = (int)((int64_t)nt_all * (split + 1) / a.splits);
+  // turns of the loop: with barriers inside, the same for all teams of the workgroup
+  const int turns = MAPS == 1 ? (t1 - t0 - kwi + a.kw - 1) / a.kw : (a.kw == 1 ? (a.Tk + KT - 1) / KT : (t1 - t0 + a.kw - 1) / a.kw);
+
+  u32x4 qf[KS];
+  load_row<KS>(qf, (const char*)a.q + 2 * (b * a.q_sb + (int64_t)qi * a.q_st + (int64_t)(head * MAPS + m) * a.q_sh), mine, h, a.d);
+
+  const char* kb[MAPS];
+#pragma unroll
+  for (int i = 0; i < MAPS; ++i) kb[i] = (const char*)a.k + 2 * (b * a.k_sb + (int64_t)(kvh * MAPS + i) * a.k_sh);
+  const char* vb = (const char*)a.v + 2 * (b * a.v_sb + (int64_t)kvh * a.v_sh);
+  TileDma<KCH, KT, MAPS> kd;
+  TileDma<VCH, KT, MAPS> vd;
+  kd.init(m, lane, a.k_st, a.d);
+  vd.init(m, lane, a.v_st, a.dv);
+  char* mem = smem + team * 2 * STAGE;
+  auto issue = [&](int t, int st) {
+    char* p = mem + st * STAGE;
+    const int64_t row = (int64_t)t * KT;
+    const int valid = len - t * KT;
+#pragma unroll
+    for (int i = 0; i < MAPS; ++i) kd.issue(kb[i] + row * a.k_st * 2, valid, p + i * K_BYTES, m);
+    vd.issue(vb + row * a.v_st * 2, valid, p + MAPS * K_BYTES, m);
+  };
+  constexpr int PIECES = TileDma<KCH, KT, 1>::P + TileDma<VCH, KT, 1>::P;  // (MAPS = 1)
+  RowRead<KCH, KS> kr;
+  TrRead<VCH, NT> vr;
+  kr.init(lane);
+  vr.init(lane);
+
+  f32x16 o[NT];
+  float mrun = -INFINITY, lrun = 0.f;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) o[nt] = zero16();
+  const float far_lo = BIAS && mine ? bias_at<T>(a, head, -a.R) : 0.f, far_hi = BIAS && mine ? bias_at<T>(a, head, a.R) : 0.f;
+
+  if (t0 + kwi < t1) issue(t0 + kwi, 0);
+  for (int it = 0; it < turns; ++it) {
+    const int t = t0 + kwi + it * a.kw;
+    const int k0 = t * KT;
+    // the bias is fetched before the next tile's DMA is issued, so that waiting for it does not wait for that
+    f32x16 bias;
+    float mul = a.scale_log2, add = 0.f;
+    bool close = false;
+    if (BIAS) {
+      if (k0 + 31 - start <= -a.R) add = far_lo;
+      else if (k0 - (start + a.Tq - 1) >= a.R) add = far_hi;
+      else {
+        close = true;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bias[r] = mine ? bias_at<T>(a, head, k0 + acc_row(r) + 4 * h - (start + qi)) : 0.f;
+      }
+    }
+    if (MAPS == 1) {
+      if (t + a.kw < t1) {
+        issue(t + a.kw, (it + 1) & 1);
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
+      } else {
+        MAPATTN_WAIT_DMA();
+      }
+    } else {
+      MAPATTN_WAIT_DMA();
+      __syncthreads();
+      if (t + a.kw < t1) issue(t + a.kw, (it + 1) & 1);
+      if (t >= t1) continue;
+    }
+    const char* tile = mem + (it & 1) * STAGE;
+    f32x16 s = zero16();
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) s = Num<T>::mfma(kr.get(tile + m * K_BYTES, 0, kk), qf[kk], s);
+    if (BIAS && close) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mul, bias[r]);
+      mul = 1.f;
+    }
+    if (k0 + 31 >= len || (a.causal && k0 + 31 > start)) {
+      const int dl = lim - k0 - 4 * h;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = acc_row(r) > dl ? -INFINITY : s[r];
+    }
+    u32x4 p[2];
+    soft_step<T, NT>(s, mul, add, mrun, lrun, o, p);
+#pragma unroll
+    for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) o[nt] = Num<T>::mfma(vr.get(tile + MAPS * K_BYTES, kb2, nt), p[kb2], o[nt]);
+    // (MAPS = 1) the stage just read is written by the DMA issued in the next turn: its reads have returned before that
+    if (MAPS == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  }
+  lrun = xor32_sum(lrun);
+
+  // ---- join the teams of a problem: team 0 adds the others' results scaled to the common maximum ---------------------------
+  if (a.kw > 1) {
+    float* jo = (float*)smem;
+    float* jm = jo + (NTEAM - 1) * MAPS * OW;
+    __syncthreads();  // all tiles read
+    if (kwi > 0) {
+      const int w = (kwi - 1) * MAPS + m;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) jo[w * OW + (nt * 16 + r) * 64 + lane] = o[nt][r];
+      jm[w * 128 + lane] = mrun;
+      jm[w * 128 + 64 + lane] = lrun;
+    }
+    __syncthreads();
+    if (kwi == 0) {
+      float mw[NTEAM], all = mrun;
+#pragma unroll
+      for (int i = 0; i < NTEAM - 1; ++i) {
+        mw[i] = jm[(i * MAPS + m) * 128 + lane];
+        all = fmaxf(all, mw[i]);
+      }
+      const float base = all == -INFINITY ? 0.f : all;
+      float f = __builtin_amdgcn_exp2f(mrun - base);
+      lrun *= f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[nt][r] *= f;
+#pragma unroll
+      for (int i = 0; i < NTEAM - 1; ++i) {
+        const int w = i * MAPS + m;
+        f = __builtin_amdgcn_exp2f(mw[i] - base);
+        lrun += f * jm[w * 128 + 64 + lane];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[nt][r] += f * jo[w * OW + (nt * 16 + r) * 64 + lane];
+      }
+      mrun = all;
+    }
+  }
+  const bool none = mrun == -INFINITY;
+  const float inv = none ? 0.f : 1.0f / lrun;
+  const float lse2 = none ? -INFINITY : mrun + __builtin_amdgcn_logf(lrun);
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) o[nt][r] *= inv;
+  const int64_t row = ((int64_t)b * a.Tq + qi) * a.H + head;
+  if (MAPS == 2 && a.splits == 1) {
+    float* x = (float*)smem + team * OW + lane;
+    __syncthreads();  // tiles and joined results read
+    if (m == 1 && mine) {
+      const float lam = a.lam[head];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[(nt * 16 + r) * 64] = o[nt][r] * lam;
+    }
+    __syncthreads();
+    if (m == 0)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[nt][r] -= x[(nt * 16 + r) * 64];
+  }
+  if (!mine || kwi > 0) return;
+  if (a.splits > 1) {
+    const int64_t at = ((int64_t)split * a.B * a.Tq * a.H + row) * MAPS + m;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const int c0 = nt * 32 + rq * 8 + h * 4;
+        if (c0 < a.dv) *(f32x4*)(a.part_o + at * a.dv + c0) = f32x4{o[nt][4 * rq], o[nt][4 * rq + 1], o[nt][4 * rq + 2], o[nt][4 * rq + 3]};
+      }
+    if (h == 0) a.part_l[at] = lse2;
+    return;
+  }
+  if (a.lse && h == 0) a.lse[((int64_t)(b * a.H + head) * MAPS + m) * a.Tq + qi] = lse2 * LN2;
+  char* op = (char*)(m == 0 ? a.out : a.out2);
+  if (op == nullptr) return;
+  op += row * a.dv * 2;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) {
+      const int c0 = nt * 32 + rq * 8 + h * 4;
+      if (c0 < a.dv) *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(o[nt][4 * rq], o[nt][4 * rq + 1]), Num<T>::pack(o[nt][4 * rq + 2], o[nt][4 * rq + 3])};
+    }
+}
+
+// ---- joins the parts of a split forward: o = sum_s 2^(l_s - l) o_s, l = log2 sum_s 2^l_s; one thread per 4 channels -----------
+template <typename T, int MAPS>
+__global__ __launch_bounds__(256) void mapattn_combine_kernel(const MapAttnArgs a) {
+  const int64_t rows = (int64_t)a.B * a.Tq * a.H;
+  const int qn = a.dv / 4;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * qn) return;
+  const int64_t row = i / qn;
+  const int c0 = (int)(i - row * qn) * 4;
+  float x[MAPS][4], lse2[MAPS];
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    float mx = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, a.part_l[((int64_t)s * rows + row) * MAPS + m]);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    float sum = 0.f;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < a.splits; ++s) {
+      const int64_t at = ((int64_t)s * rows + row) * MAPS + m;
+      const float w = __builtin_amdgcn_exp2f(a.part_l[at] - base);
+      sum += w;
+      const f32x4 v = *(const f32x4*)(a.part_o + at * a.dv + c0);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+    }
+    const bool none = mx == -INFINITY;
+    const float inv = none ? 0.f : 1.0f / sum;
+    lse2[m] = none ? -INFINITY : base + __builtin_amdgcn_logf(sum);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[m][e] = acc[e] * inv;
+  }
+  const int head = (int)(row % a.H);
+  const int64_t bt = row / a.H;
+  if (MAPS == 2) {
+    if (a.out2) *(u32x2*)((char*)a.out2 + (row * a.dv + c0) * 2) = u32x2{Num<T>::pack(x[MAPS - 1][0], x[MAPS - 1][1]), Num<T>::pack(x[MAPS - 1][2], x[MAPS - 1][3])};
+    const float lam = a.lam[head];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[0][e] -= lam * x[MAPS - 1][e];
+  }
+  *(u32x2*)((char*)a.out + (row * a.dv + c0) * 2) = u32x2{Num<T>::pack(x[0][0], x[0][1]), Num<T>::pack(x[0][2], x[0][3])};
+  if (a.lse && c0 == 0) {
+    const int64_t b = bt / a.Tq, qi = bt - b * a.Tq;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) a.lse[((b * a.H + head) * MAPS + m) * a.Tq + qi] = lse2[m] * LN2;
+  }
+}
+
+// ---- dispatch -----------------------------------------------------------------------------------------------------------
+namespace {
+
+template <typename T, int MAPS, int KS, int NT>
+int run_fwd(const MapAttnArgs& a, hipStream_t s) {
+  constexpr int KT = 64;
+  constexpr int KCH = 4 * ((KS + 1) / 2), VCH = 4 * NT;
+  constexpr int tiles = 2 * KT * 16 * (MAPS * KCH + VCH), hand = MAPS == 2 ? 4 * NT * 16 * 64 * 4 : 0;
+  const int lds = (tiles > hand ? tiles : hand) + (MAPS == 1 ? (2 * (a.R + 128 + KT) + 1) * 4 : 0);
+  const void* f = (const void*)mapattn_fwd_kernel<T, MAPS, KS, NT, KT>;
+  if (anip_raise_lds_limit(f, lds) != 0) {
+    anip_set_error("mapattn forward: cannot raise the dynamic LDS limit to %d bytes", lds);
+    return -2;
+  }
+  const int nqb = (a.Tq + 127) / 128;
+  hipLaunchKernelGGL((mapattn_fwd_kernel<T, MAPS, KS, NT, KT>), dim3((unsigned)(nqb * a.splits * a.B * a.H)), dim3(256 * MAPS), lds, s, a);
+  ANIP_LAUNCH_CHECK("mapattn_fwd_kernel");
+  return 0;
+}
+
+// bytes of a team's two stages of 32 keys; as many teams to a workgroup, up to four, as fit the CU's LDS
+constexpr int token_team_lds(int maps, int ks, int nt) { return 2 * 32 * 16 * (maps * 4 * ((ks + 1) / 2) + 4 * nt); }
+constexpr int token_teams(int maps, int ks, int nt) { return 4 * token_team_lds(maps, ks, nt) <= 160 * 1024 ? 4 : 2; }
+
+template <typename T, int MAPS, int KS, int NT>
+int run_token(const MapAttnArgs& a0, hipStream_t s) {
+  constexpr int NTEAM = token_teams(MAPS, KS, NT), OW = NT * 16 * 64 * 4;
+  constexpr int tiles = NTEAM * token_team_lds(MAPS, KS, NT), join = (NTEAM - 1) * MAPS * (OW + 512), hand = MAPS == 2 ? NTEAM * OW : 0;
+  constexpr int lds = tiles > join ? (tiles > hand ? tiles : hand) : (join > hand ? join : hand);
+  static_assert(lds <= 160 * 1024, "LDS of a CU");
+  MapAttnArgs a = a0;
+  if (a.kw > 1) a.kw = NTEAM;
+  const void* f = (const void*)mapattn_token_kernel<T, MAPS, KS, NT, NTEAM>;
+  if (anip_raise_lds_limit(f, lds) != 0) {
+    anip_set_error("mapattn token: cannot raise the dynamic LDS limit to %d bytes", lds);
+    return -2;
+  }
+  const int ppb = NTEAM / a.kw;
+  hipLaunchKernelGGL((mapattn_token_kernel<T, MAPS, KS, NT, NTEAM>), dim3((unsigned)((a.B * a.Hkv * a.splits + ppb - 1) / ppb)), dim3(64 * NTEAM * MAPS), lds, s, a);
+  ANIP_LAUNCH_CHECK("mapattn_token_kernel");
+  return 0;
+}
+
+template <typename T, int MAPS>
+int run_combine(const MapAttnArgs& a, hipStream_t s) {
+  const int64_t n = (int64_t)a.B * a.Tq * a.H * (a.dv / 4);
+  hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS>), dim3((unsigned)cdiv64(n, 256)), dim3(256), 0, s, a);
+  ANIP_LAUNCH_CHECK("mapattn_combine_kernel");
+  return 0;
+}
+
+#define TRY1(KS, NT) if (ks <= KS) return run<T, 1, KS, NT>(a, s);
+#define TRY2(KS, NT) if (ks <= KS) return run<T, 2, KS, NT>(a, s);
+template <typename T>
+int fwd_t(const MapAttnArgs& a, int maps, hipStream_t s) {
+  const int ks = (a.d + 15) / 16;
+#define run run_fwd
+  if (maps == 1) { MAPATTN_GEOS_1(TRY1) } else { MAPATTN_GEOS_2(TRY2) }
+#undef run
+  return -1;
+}
+template <typename T>
+int token_t(const MapAttnArgs& a, int maps, hipStream_t s) {
+  const int ks = (a.d + 15) / 16;
+#define run run_token
+  if (maps == 1) { MAPATTN_GEOS_1(TRY1) } else { MAPATTN_GEOS_2(TRY2) }
+#undef run
+  return -1;
+}
+
+}  // namespace
+
+int mapattn_forward(const MapAttnArgs& a, int maps, int bf16, hipStream_t s) { return bf16 ? fwd_t<bf16_t>(a, maps, s) : fwd_t<f16>(a, maps, s); }
+int mapattn_token(const MapAttnArgs& a, int maps, int bf16, hipStream_t s) { return bf16 ? token_t<bf16_t>(a, maps, s) : token_t<f16>(a, maps, s); }
+int mapattn_combine(const MapAttnArgs& a, int maps, int bf16, hipStream_t s) {
+  if (maps == 1) return bf16 ? run_combine<bf16_t, 1>(a, s) : run_combine<f16, 1>(a, s);
+  return bf16 ? run_combine<bf16_t, 2>(a, s) : run_combine<f16, 2>(a, s);
+}

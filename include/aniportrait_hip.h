@@ -25,7 +25,7 @@
 extern "C" {
 #endif
 
-#define ANIP_ABI_VERSION 15   /* 15 (round 6): anip_gemm act = 2 (quick-GELU); anip_conv_small removed */
+#define ANIP_ABI_VERSION 16   /* 16: anip_qk_norm_rope, anip_relative_attention, anip_differential_attention and their gradients */
 
 int anip_version(void);
 const char* anip_last_error(void);
@@ -219,6 +219,74 @@ int anip_temporal_qkv_attention_supported(int F, int T, int C, int heads);
 int anip_temporal_qkv_attention(const void* x, const float* gamma, const float* beta_pe, const void* w_packed, void* out,
                                 int B, int F, int T, int C, int heads, float eps, float scale, void* stream);
 
+/* ---- attention with learned positions and maps: norm and rotation of heads, relative bias, differential attention ------------
+ * Beyond the reference: its attention knows positions only through the added sinusoids of src/models/motion_module.py:262-277
+ * (32 frames at most).  These entry points take tensors (batch, token, head, channel) with strides in elements {batch, token,
+ * head} and contiguous channels; dtype 0 = fp16, 1 = bf16.  Pointers are 16-byte aligned, strides multiples of 8 elements.
+ *
+ * anip_qk_norm_rope — y = R(pos) (x (mean x^2 + eps)^-1/2 w) for all Hq query and Hkv key heads (Hkv = 0: queries alone), the
+ *   queries also times q_alpha (e.g. scale * log2 e for ANIP_ATTN_Q_LOG2_SCALED).  R turns channel pairs of the first `rot`
+ *   channels (a multiple of 8, 0: no rotation): pair i = (i, i + rot / 2), interleaved != 0: (2 i, 2 i + 1), by the angle whose
+ *   (cos, sin) is rope[pos][i] (fp32 [rope_rows][rot / 2][2]); pos = positions[b][t], or t where positions is NULL; positions
+ *   outside the table are clamped to it.  An output may be its input (in place), else they must not overlap.
+ * anip_qk_norm_rope_backward — q_out / k_out receive dq / dk from dq_out / dk_out and the forward's inputs; dq_weight / dk_weight
+ *   (fp32 [d]) are written.  ws: anip_qk_norm_rope_backward_ws_floats(B * T, Hq + Hkv, d) floats. */
+typedef struct anip_qk_norm_params {
+  int dtype;
+  int B, T, Hq, Hkv, d, rot, interleaved;
+  float eps, q_alpha;
+  const void* q; int64_t q_stride[3];
+  const void* k; int64_t k_stride[3];
+  const float* q_weight; const float* k_weight;          /* [d] */
+  const float* rope; int rope_rows; const int* positions; /* [B][T] or NULL */
+  void* q_out; int64_t q_out_stride[3];
+  void* k_out; int64_t k_out_stride[3];
+  const void* dq_out; int64_t dq_out_stride[3];           /* backward only, from here on */
+  const void* dk_out; int64_t dk_out_stride[3];
+  float* dq_weight; float* dk_weight;
+  float* ws; int64_t ws_floats;
+} anip_qk_norm_params;
+int anip_qk_norm_rope(const anip_qk_norm_params* p, void* stream);
+int64_t anip_qk_norm_rope_backward_ws_floats(int64_t M, int heads, int d);
+int anip_qk_norm_rope_backward(const anip_qk_norm_params* p, void* stream);
+
+/* anip_relative_attention — o_i = softmax_j(scale q_i.k_j + table[h][buckets[clamp(j - p_i, +-max_distance) + max_distance]]) v_j
+ *   q (B, Tq, H, d), k, v (B, Tk, Hkv, d), H a multiple of Hkv (query head h reads key head h / (H / Hkv)), d a multiple of 8 up
+ *   to 160; table [H][n_buckets] in the inputs' type, buckets int32 [2 max_distance + 1] (max_distance <= 4096; entries outside
+ *   [0, n_buckets) are clamped).
+ * anip_differential_attention — o_i = (softmax_j(scale q1_i.k1_j) - lam[h] softmax_j(scale q2_i.k2_j)) v_j
+ *   q (B, Tq, 2 H, d), k (B, Tk, 2 Hkv, d): heads 2 h and 2 h + 1 are the two maps of head h; v (B, Tk, Hkv, 2 d), lam fp32 [H],
+ *   d a multiple of 8 up to 128; out (B, Tq, H, 2 d).
+ * Both: p_i = q_start[b] + i is the position of query i (int32 [B]; NULL: Tk - Tq + i).  Query i sees key j if j < kv_lens[b]
+ *   (int32 [B], clamped to [0, Tk]; NULL: Tk) and, when causal, j <= p_i; a query that sees no key gets zeros.  Keys and values
+ *   behind kv_lens[b] are never used, whatever they hold.  out, dq, dk, dv are contiguous.  lse (fp32 [B][H * maps][Tq], natural
+ *   logarithm, -inf for rows without keys) and, for two maps, out2 (the second map's own output, as out) may be NULL where no
+ *   backward follows.
+ * Backward: dq, dk, dv, dtable [H][n_buckets] (inputs' type) or dlam fp32 [H] from dout and the forward's out, out2, lse.  Keys
+ *   behind kv_lens get zero gradients.  No atomics: equal inputs give equal gradients.
+ * workspace: anip_*_ws_bytes(p, backward) bytes (0: none; < 0: error), 16-byte aligned. */
+typedef struct anip_attn_params {
+  int dtype;
+  int B, Tq, Tk, H, Hkv, d, causal;
+  float scale;
+  const void* q; int64_t q_stride[3];
+  const void* k; int64_t k_stride[3];
+  const void* v; int64_t v_stride[3];
+  const int* kv_lens; const int* q_start;
+  const void* table; const int* buckets; int n_buckets, max_distance;
+  const float* lam;
+  void* out; void* out2; float* lse;
+  const void* dout; int64_t dout_stride[3];               /* backward only, to dlam */
+  void* dq; void* dk; void* dv; void* dtable; float* dlam;
+  void* workspace; int64_t workspace_bytes;
+} anip_attn_params;
+int64_t anip_relative_attention_ws_bytes(const anip_attn_params* p, int backward);
+int anip_relative_attention(const anip_attn_params* p, void* stream);
+int anip_relative_attention_backward(const anip_attn_params* p, void* stream);
+int64_t anip_differential_attention_ws_bytes(const anip_attn_params* p, int backward);
+int anip_differential_attention(const anip_attn_params* p, void* stream);
+int anip_differential_attention_backward(const anip_attn_params* p, void* stream);
+
 /* ---- row softmax fp32 -> fp16 (VAE mid-block attention, diffusers Attention upcast_softmax) ---- */
 int anip_softmax_rows(const float* s, void* p, int64_t rows, int cols, void* stream);
 
@@ -276,7 +344,10 @@ enum {
   ANIP_K_LINEAR_SMALL = 9,
   ANIP_K_ELEMENTWISE = 10, /* add / window accumulate / cfg+ddim / layout conversions */
   ANIP_K_BATCHNORM = 11,  /* bn_stats + bn_finalize + bn_apply (PoseGuider) */
-  ANIP_K_COUNT = 12
+  ANIP_K_QK_NORM = 12,    /* anip_qk_norm_rope and its backward */
+  ANIP_K_REL_ATTN = 13,   /* anip_relative_attention and its backward */
+  ANIP_K_DIFF_ATTN = 14,  /* anip_differential_attention and its backward */
+  ANIP_K_COUNT = 15
 };
 int anip_profile_enable(int on);
 int anip_profile_collect(int max_ids, int64_t* launches, double* total_ms);
