@@ -30,8 +30,7 @@ struct HeadNormArgs {
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const char* row, int a, int b) {
-  const u32x2 u = *(const u32x2*)(row + 2 * a), v = *(const u32x2*)(row + 2 * b);
+__device__ __forceinline__ void widen(float (&x)[8], u32x2 u, u32x2 v) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     x[2 * i] = Num<T>::lo(u[i]);
@@ -39,6 +38,10 @@ __device__ __forceinline__ void load8(float (&x)[8], const char* row, int a, int
     x[4 + 2 * i] = Num<T>::lo(v[i]);
     x[5 + 2 * i] = Num<T>::hi(v[i]);
   }
+}
+template <typename T>
+__device__ __forceinline__ void load8(float (&x)[8], const char* row, int a, int b) {
+  widen<T>(x, *(const u32x2*)(row + 2 * a), *(const u32x2*)(row + 2 * b));
 }
 template <typename T>
 __device__ __forceinline__ void store8(char* row, int a, int b, const float (&x)[8]) {
@@ -164,34 +167,51 @@ __global__ __launch_bounds__(256) void head_norm_bwd_kernel(const HeadNormArgs p
     const int t = (int)(m - b * p.T);
     float cs[8];
     load_cs(cs, p, ln, m, t, j);
-    for (int hh = h0; hh < h1; ++hh) {
-      const int w = hh >= p.H[0], h = w ? hh - p.H[0] : hh;
-      float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, u[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (ln.on) {
-        load8<T>(x, (const char*)p.x[w] + 2 * (b * p.x_sb[w] + t * p.x_st[w] + h * p.x_sh[w]), ln.a, ln.b);
-        load8<T>(u, (const char*)p.dy[w] + 2 * (b * p.dy_sb[w] + t * p.dy_st[w] + h * p.dy_sh[w]), ln.a, ln.b);
-      }
-      if (ln.rot) turn(u, cs, p.inter, -1.f);
-      float ss = 0.f, dot = 0.f;
-      const float al = w ? 1.f : p.alpha;
+    constexpr int U = 4;  // heads whose loads are in flight together
+    for (int h2 = h0; h2 < h1; h2 += U) {
+      u32x2 xa[U], xb[U], ga[U], gb[U];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ss = fmaf(x[i], x[i], ss);
-        u[i] *= al;
-        dot = fmaf(u[i] * (w ? wt[1][i] : wt[0][i]), x[i], dot);
+      for (int k = 0; k < U; ++k) {
+        const int hh = h2 + k, w = hh >= p.H[0], h = w ? hh - p.H[0] : hh;
+        xa[k] = xb[k] = ga[k] = gb[k] = u32x2{0u, 0u};
+        if (ln.on && hh < h1) {
+          const char* xr = (const char*)p.x[w] + 2 * (b * p.x_sb[w] + t * p.x_st[w] + h * p.x_sh[w]);
+          const char* gr = (const char*)p.dy[w] + 2 * (b * p.dy_sb[w] + t * p.dy_st[w] + h * p.dy_sh[w]);
+          xa[k] = *(const u32x2*)(xr + 2 * ln.a);
+          xb[k] = *(const u32x2*)(xr + 2 * ln.b);
+          ga[k] = *(const u32x2*)(gr + 2 * ln.a);
+          gb[k] = *(const u32x2*)(gr + 2 * ln.b);
+        }
       }
-      ss = group_sum<L>(ss);
-      dot = group_sum<L>(dot);
-      const float rstd = __builtin_amdgcn_rsqf(fmaf(ss, p.inv_d, p.eps));
-      const float c = dot * p.inv_d * rstd * rstd;  // mean(u w x^) rstd
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float g = u[i] * x[i] * rstd;
-        dw[0][i] += w ? 0.f : g;
-        dw[1][i] += w ? g : 0.f;
-        x[i] = rstd * fmaf(u[i], w ? wt[1][i] : wt[0][i], -(x[i] * c));
+      for (int k = 0; k < U; ++k) {
+        const int hh = h2 + k, w = hh >= p.H[0], h = w ? hh - p.H[0] : hh;
+        float x[8], u[8];
+        widen<T>(x, xa[k], xb[k]);
+        widen<T>(u, ga[k], gb[k]);
+        if (ln.rot) turn(u, cs, p.inter, -1.f);
+        float ss = 0.f, dot = 0.f;
+        const float al = w ? 1.f : p.alpha;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ss = fmaf(x[i], x[i], ss);
+          u[i] *= al;
+          dot = fmaf(u[i] * (w ? wt[1][i] : wt[0][i]), x[i], dot);
+        }
+        ss = group_sum<L>(ss);
+        dot = group_sum<L>(dot);
+        const float rstd = __builtin_amdgcn_rsqf(fmaf(ss, p.inv_d, p.eps));
+        const float c = dot * p.inv_d * rstd * rstd;  // mean(u w x^) rstd
+        const float f0 = w ? 0.f : rstd, f1 = w ? rstd : 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float g = u[i] * x[i];
+          dw[0][i] = fmaf(g, f0, dw[0][i]);
+          dw[1][i] = fmaf(g, f1, dw[1][i]);
+          x[i] = rstd * fmaf(u[i], w ? wt[1][i] : wt[0][i], -(x[i] * c));
+        }
+        if (ln.on && hh < h1) store8<T>((char*)p.y[w] + 2 * (b * p.y_sb[w] + t * p.y_st[w] + h * p.y_sh[w]), ln.a, ln.b, x);
       }
-      if (ln.on) store8<T>((char*)p.y[w] + 2 * (b * p.y_sb[w] + t * p.y_st[w] + h * p.y_sh[w]), ln.a, ln.b, x);
     }
   }
   // ---- the workgroup's part of dw: groups added in their order --------------------------------------------------------------

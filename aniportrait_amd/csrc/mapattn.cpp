@@ -63,9 +63,8 @@ int splits_of(const anip_attn_params* p) {
   const bool few = few_rows(p);
   const int64_t blocks = few ? (int64_t)p->B * p->Hkv : (int64_t)((p->Tq + 127) / 128) * p->B * p->H;
   const int64_t tiles = few ? (p->Tk + 127) / 128 : (p->Tk + 63) / 64;
-  const int64_t want = few ? 512 : 512;
-  if (blocks * 2 > want) return 1;
-  int64_t s = want / blocks;
+  if (blocks * 2 > 512) return 1;
+  int64_t s = 512 / blocks;
   const int64_t most = tiles / 4;
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
@@ -104,9 +103,20 @@ int forward(const char* what, const anip_attn_params* p, int maps, int kid, void
 // one wave per workgroup on short sequences, which would leave three of four idle
 int waves_for(int T) { return T <= 64 ? 1 : 4; }
 
+// the keys' kernel walks over the queries of all heads that share a key head; where the keys alone make fewer workgroups than the
+// chip holds at once (one of 4 wave groups per CU), the walk is split towards two rounds of them, each with 8 tiles at the least
+int dkv_splits(const anip_attn_params* p, int nwk) {
+  const int64_t blocks = (int64_t)((p->Tk + 32 * nwk - 1) / (32 * nwk)) * p->B * p->Hkv * nwk / 4 + 1;
+  const int64_t tiles = (int64_t)((p->Tq + 63) / 64) * (p->H / p->Hkv);
+  if (blocks * 2 > 512) return 1;
+  int64_t s = 512 / blocks;
+  s = s < tiles / 8 ? s : tiles / 8;
+  return (int)(s < 1 ? 1 : (s > 16 ? 16 : s));
+}
+
 struct BwdLayout {
-  int nwq, nwk, Tp, QW, ND, parts;
-  int64_t rows, diag, dlam, part, total;  // floats
+  int nwq, nwk, Tp, QW, ND, parts, splits;
+  int64_t rows, diag, dlam, part, dkv, total;  // floats
 };
 BwdLayout layout(const anip_attn_params* p, int maps) {
   BwdLayout l{};
@@ -118,13 +128,15 @@ BwdLayout layout(const anip_attn_params* p, int maps) {
   if (maps == 1) {
     l.ND = 2 * p->max_distance + 128;
     const int64_t groups = (int64_t)p->B * l.QW;
-    l.parts = (int)(groups < 64 ? groups : 64);
+    l.parts = (int)(groups < 32 ? groups : 32);
     l.diag = (int64_t)p->H * groups * (l.ND + 2);
     l.part = (int64_t)p->H * l.parts * (l.ND + 2);
   } else {
     l.dlam = (int64_t)p->H * p->B * l.QW;
   }
-  l.total = 2 * l.rows + l.diag + l.part + l.dlam;
+  l.splits = dkv_splits(p, l.nwk);
+  if (l.splits > 1) l.dkv = (int64_t)l.splits * p->B * p->Tk * p->Hkv * 2 * maps * p->d;
+  l.total = l.dkv + 2 * l.rows + l.diag + l.part + l.dlam;
   return l;
 }
 
@@ -133,13 +145,14 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   if (rc) return rc;
   const BwdLayout l = layout(p, maps);
   ANIP_REQUIRE(p->workspace != nullptr && ((uintptr_t)p->workspace & 15) == 0 && p->workspace_bytes >= l.total * 4, "%s: a workspace of %lld bytes is wanted, 16-byte aligned", what, (long long)l.total * 4);
-  ANIP_REQUIRE((int64_t)(l.Tp / 32) * p->B * p->H < (1ll << 31) && (int64_t)((p->Tk + 31) / 32) * p->B * p->Hkv < (1ll << 31), "%s: too many rows for one launch", what);
+  ANIP_REQUIRE((int64_t)(l.Tp / 32) * p->B * p->H < (1ll << 31) && (int64_t)((p->Tk + 31) / 32) * p->B * p->Hkv < (1ll << 31) && (int64_t)p->B * p->Tk * p->Hkv * maps * p->d / 512 < (1ll << 31), "%s: too many rows for one launch", what);
   ANIP_REQUIRE((int64_t)((p->Tq + 31) / 32) * (p->H / p->Hkv) < (1ll << 31), "%s: too many query tiles", what);
   MapAttnArgs a = args(p, maps);
   a.dout = p->dout, a.do_sb = p->dout_stride[0], a.do_st = p->dout_stride[1], a.do_sh = p->dout_stride[2];
   a.dq = p->dq, a.dk = p->dk, a.dvo = p->dv, a.dtable = p->dtable, a.dlam = p->dlam;
   a.Tp = l.Tp, a.QW = l.QW, a.ND = l.ND, a.parts = l.parts;
-  a.rows_lse = (float*)p->workspace;
+  a.part_o = (float*)p->workspace;
+  a.rows_lse = a.part_o + l.dkv;
   a.rows_d = a.rows_lse + l.rows;
   a.diag = a.rows_d + l.rows;
   a.diag_part = a.diag + l.diag;
@@ -147,6 +160,7 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   hipStream_t s = (hipStream_t)stream;
   AnipProfScope prof_(kid, stream);
   int r = mapattn_dq(a, maps, p->dtype, l.nwq, s);
+  a.splits = l.splits;
   if (!r) r = mapattn_dkv(a, maps, p->dtype, l.nwk, s);
   if (!r) r = mapattn_reduce(a, maps, p->dtype, s);
   return r;

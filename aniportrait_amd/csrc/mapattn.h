@@ -105,30 +105,37 @@ __device__ __forceinline__ u32x2 lds_tr(const char* p) {
 }
 __device__ __forceinline__ u32x4 join(u32x2 a, u32x2 b) { return u32x4{a[0], a[1], b[0], b[1]}; }
 
-// row-major reads: lane (l & 31, h) takes row l & 31, chunk 2 kk + h
-template <int CH, int KS>
+// Both reads keep one offset per lane and derive the others: a chunk 32 or 64 bytes on is an exclusive or where the swizzle
+// reaches those bits (CH a multiple of 8), an immediate otherwise.  The compiler holds the derived offsets in registers across
+// the tiles; opaque() makes it derive them anew, where the accumulators need the registers.
+__device__ __forceinline__ void opaque(int& x) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  asm volatile("" : "+v"(x));
+#endif
+}
+// row-major reads: lane (l & 31, h) takes row l & 31, chunk 2 (STEP kk + m) + h (STEP = 2: a pair of waves, m = 0, 1, shares the row)
+template <int CH, int STEP = 1>
 struct RowRead {
-  int off[KS];
-  __device__ __forceinline__ void init(int lane) {
-    const int row = lane & 31, h = lane >> 5;
-#pragma unroll
-    for (int kk = 0; kk < KS; ++kk) off[kk] = chunk_at<CH>(row, 2 * kk + h);
+  int base;
+  __device__ __forceinline__ void init(int lane, int m = 0) { base = chunk_at<CH>(lane & 31, 2 * m + (lane >> 5)); }
+  __device__ __forceinline__ u32x4 get(const char* tile, int sub, int kk) const {
+    // where the swizzle stays below chunk bit 2 an odd step flips bit 1 and the rest adds
+    const int off = CH % 8 == 0 ? base ^ (32 * STEP * kk) : STEP == 2 ? base + 64 * kk : (kk & 1 ? base ^ 32 : base) + 64 * (kk >> 1);
+    return lds16(tile + off + sub * (32 * CH * 16));
   }
-  __device__ __forceinline__ u32x4 get(const char* tile, int sub, int kk) const { return lds16(tile + off[kk] + sub * (32 * CH * 16)); }
 };
-// transposed reads: the A operand with rows = channels 32 nt .. + 31 and contraction over tile rows 16 kb .. + 15
-template <int CH, int NT>
+// transposed reads: the A operand with rows = channels 32 (nt0 + nt) .. + 31 and contraction over tile rows 16 kb .. + 15
+template <int CH>
 struct TrRead {
-  int off[NT];
-  __device__ __forceinline__ void init(int lane) {
+  int base;
+  __device__ __forceinline__ void init(int lane, int nt0 = 0) {
     const int j = lane & 15, g = (lane >> 4) & 1, h = lane >> 5;
-    const int row = 4 * h + (j >> 2);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) off[nt] = chunk_at<CH>(row, 4 * nt + 2 * g + ((j & 3) >> 1)) + (j & 1) * 8;
+    base = chunk_at<CH>(4 * h + (j >> 2), 4 * nt0 + 2 * g + ((j & 3) >> 1)) + (j & 1) * 8;
   }
   __device__ __forceinline__ u32x4 get(const char* tile, int kb, int nt) const {
+    const int off = CH % 8 == 0 ? base ^ (64 * nt) : base + 64 * nt;
     const char* p = tile + kb * (16 * CH * 16);
-    return join(lds_tr(p + off[nt]), lds_tr(p + (off[nt] ^ 32) + 8 * CH * 16));  // rows 8 on: chunk bit 1 flips
+    return join(lds_tr(p + off), lds_tr(p + (off ^ 32) + 8 * CH * 16));  // rows 8 on: chunk bit 1 flips
   }
 };
 
@@ -170,12 +177,12 @@ struct TileDma {
   }
 };
 
-// B operand fragments of a row held in registers: chunk 2 kk + h of the row, zeros where it does not exist
-template <int KS>
-__device__ __forceinline__ void load_row(u32x4 (&f)[KS], const void* row, bool exists, int h, int d) {
+// B operand fragments of a row held in registers: chunk 2 (STEP kk + m) + h of the row, zeros where it does not exist
+template <int KS, int STEP = 1>
+__device__ __forceinline__ void load_row(u32x4 (&f)[KS], const void* row, bool exists, int h, int d, int m = 0) {
 #pragma unroll
   for (int kk = 0; kk < KS; ++kk) {
-    const int c = 2 * kk + h;
+    const int c = 2 * (STEP * kk + m) + h;
     f[kk] = u32x4{0u, 0u, 0u, 0u};
     if (exists && c * 8 < d) f[kk] = *(const u32x4*)((const char*)row + c * 16);
   }

@@ -10,26 +10,49 @@
 
 using namespace mapattn;
 
-// ---- dQ: 32 queries per wave, tiles of KT keys ----------------------------------------------------------------------------
-template <typename T, int MAPS, int KS, int NT, int KT, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void mapattn_dq_kernel(const MapAttnArgs a) {
+// Differential attention gives each map a wave of its own (both maps' accumulators would take all registers of one from d = 64
+// on).  The pair shares W: each wave sums it over half of the channels and they exchange the halves through LDS; for dV they
+// exchange P as well and each takes half of the channels' tiles.  Both values cross in 32 bits, with one barrier per tile of 32.
+
+__device__ __forceinline__ void put16(float* x, const f32x16& v) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) *(f32x4*)(x + i * 256) = f32x4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+}
+__device__ __forceinline__ f32x16 get16(const float* x) {
+  f32x16 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 t = *(const f32x4*)(x + i * 256);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[4 * i + e] = t[e];
+  }
+  return v;
+}
+
+// ---- dQ: 32 queries per wave (pair), tiles of KT keys -----------------------------------------------------------------------
+template <typename T, int MAPS, int KS, int NT, int KT, int NG>
+__global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) void mapattn_dq_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
-  constexpr int BQ = 32 * NW, DT = (KS + 1) / 2, KSV = MAPS == 1 ? KS : 2 * NT;
+  constexpr int NW = NG * MAPS, BQ = 32 * NG, DT = (KS + 1) / 2, KSV = MAPS == 1 ? KS : NT;  // KSV: steps over this wave's share of dv
   constexpr int KCH = 4 * DT, VCH = 4 * NT;
   constexpr int K_BYTES = KT * KCH * 16, V_BYTES = KT * VCH * 16, STAGE = MAPS * K_BYTES + V_BYTES;
   constexpr int E = BQ + KT;
+  static_assert(MAPS == 1 || KT == 32, "the pair's exchange has one slot per tile");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  float* near = (float*)(smem + 2 * STAGE);
+  float* near = (float*)(smem + 2 * STAGE);  // (one map)
 
   const int tid = threadIdx.x, lane = tid & 63, ql = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = wave / MAPS, m = wave % MAPS;
+  float* mine = (float*)(smem + 2 * STAGE) + wave * 1024 + lane * 4;         // (two maps) 16 values of each lane
+  float* theirs = (float*)(smem + 2 * STAGE) + (wave ^ 1) * 1024 + lane * 4;
   const int nqb = a.Tp / BQ;
   int qb, bh;
   if (!place(blockIdx.x, nqb, a.B * a.H, qb, bh)) return;
   qb = nqb - 1 - qb;
   const int b = bh / a.H, head = bh - b * a.H, kvh = head / a.G;
   const int len = seq_len(a, b), start = seq_start(a, b);
-  const int q0 = qb * BQ + wave * 32, qi = q0 + ql, pw = start + q0;
+  const int q0 = qb * BQ + grp * 32, qi = q0 + ql, pw = start + q0;
   const bool valid = qi < a.Tq;
   const int lim = a.causal ? min(len - 1, start + qi) : len - 1;
   int kend = len;
@@ -38,42 +61,41 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dq_kernel(const MapAttnArg
   const int nt_all = kend > 0 ? (kend + KT - 1) / KT : 0;
 
   const float lam = MAPS == 2 ? a.lam[head] : 0.f;
-  u32x4 qf[MAPS][KS], df[KSV];
-#pragma unroll
-  for (int m = 0; m < MAPS; ++m)
-    load_row<KS>(qf[m], (const char*)a.q + 2 * (b * a.q_sb + (int64_t)qi * a.q_st + (int64_t)(head * MAPS + m) * a.q_sh), valid, h, a.d);
-  load_row<KSV>(df, (const char*)a.dout + 2 * (b * a.do_sb + (int64_t)qi * a.do_st + (int64_t)head * a.do_sh), valid, h, a.dv);
+  u32x4 qf[KS], df[KSV];
+  const char* drow = (const char*)a.dout + 2 * (b * a.do_sb + (int64_t)qi * a.do_st + (int64_t)head * a.do_sh);
+  load_row<KS>(qf, (const char*)a.q + 2 * (b * a.q_sb + (int64_t)qi * a.q_st + (int64_t)(head * MAPS + m) * a.q_sh), valid, h, a.d);
+  load_row<KSV, MAPS>(df, drow, valid, h, a.dv, m);
 
   // ---- row statistics: D_m = dO . o_m (o_1 = o + lam o_2), -lse in base 2 -------------------------------------------------
-  float nl[MAPS], D[MAPS];
+  float nl, D;
   {
     const int64_t orow = (((int64_t)b * a.Tq + qi) * a.H + head) * a.dv * 2;
-    float dot[MAPS];
-#pragma unroll
-    for (int m = 0; m < MAPS; ++m) {
-      u32x4 of[KSV];
-      load_row<KSV>(of, (const char*)(m == 0 ? a.out : a.out2) + orow, valid, h, a.dv);
+    auto dot = [&](const void* o) {
       float t = 0.f;
+#pragma unroll 4
+      for (int c = h; c < a.dv / 8; c += 2) {
+        u32x4 x = {0u, 0u, 0u, 0u}, y = x;
+        if (valid) {
+          x = *(const u32x4*)(drow + c * 16);
+          y = *(const u32x4*)((const char*)o + orow + c * 16);
+        }
 #pragma unroll
-      for (int kk = 0; kk < KSV; ++kk)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) t = fmaf(Num<T>::lo(df[kk][i]), Num<T>::lo(of[kk][i]), fmaf(Num<T>::hi(df[kk][i]), Num<T>::hi(of[kk][i]), t));
-      dot[m] = xor32_sum(t);
-    }
-    D[0] = dot[0];
-    if (MAPS == 2) {
-      D[MAPS - 1] = dot[MAPS - 1];
-      D[0] = fmaf(lam, D[MAPS - 1], dot[0]);
-    }
-#pragma unroll
-    for (int m = 0; m < MAPS; ++m) {
-      const float l = valid ? a.lse[((int64_t)bh * MAPS + m) * a.Tq + qi] * LOG2E : -INFINITY;
-      nl[m] = l == -INFINITY ? -INFINITY : -l;  // rows without keys: P = 2^-inf = 0
-      if (h == 0) {
-        const int64_t at = ((int64_t)bh * MAPS + m) * a.Tp + qi;
-        a.rows_lse[at] = nl[m] + Num<T>::PSH;
-        a.rows_d[at] = D[m] * (1.0f / (1 << Num<T>::PSH));
+        for (int i = 0; i < 4; ++i) t = fmaf(Num<T>::lo(x[i]), Num<T>::lo(y[i]), fmaf(Num<T>::hi(x[i]), Num<T>::hi(y[i]), t));
       }
+      return xor32_sum(t);
+    };
+    if (MAPS == 1) {
+      D = dot(a.out);
+    } else {
+      D = dot(a.out2);
+      if (m == 0) D = fmaf(lam, D, dot(a.out));
+    }
+    const float l = valid ? a.lse[((int64_t)bh * MAPS + m) * a.Tq + qi] * LOG2E : -INFINITY;
+    nl = l == -INFINITY ? -INFINITY : -l;  // rows without keys: P = 2^-inf = 0
+    if (h == 0) {
+      const int64_t at = ((int64_t)bh * MAPS + m) * a.Tp + qi;
+      a.rows_lse[at] = nl + Num<T>::PSH;
+      a.rows_d[at] = D * (1.0f / (1 << Num<T>::PSH));
     }
   }
 
@@ -86,7 +108,7 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dq_kernel(const MapAttnArg
 
   const char* kb[MAPS];
 #pragma unroll
-  for (int m = 0; m < MAPS; ++m) kb[m] = (const char*)a.k + 2 * (b * a.k_sb + (int64_t)(kvh * MAPS + m) * a.k_sh);
+  for (int i = 0; i < MAPS; ++i) kb[i] = (const char*)a.k + 2 * (b * a.k_sb + (int64_t)(kvh * MAPS + i) * a.k_sh);
   const char* vb = (const char*)a.v + 2 * (b * a.v_sb + (int64_t)kvh * a.v_sh);
   TileDma<KCH, KT, NW> kd;
   TileDma<VCH, KT, NW> vd;
@@ -97,21 +119,19 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dq_kernel(const MapAttnArg
     const int64_t row = (int64_t)t * KT;
     const int n = len - t * KT;
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m) kd.issue(kb[m] + row * a.k_st * 2, n, st + m * K_BYTES, wave);
+    for (int i = 0; i < MAPS; ++i) kd.issue(kb[i] + row * a.k_st * 2, n, st + i * K_BYTES, wave);
     vd.issue(vb + row * a.v_st * 2, n, st + MAPS * K_BYTES, wave);
   };
-  RowRead<KCH, KS> kr;
-  RowRead<VCH, KSV> vr;
-  TrRead<KCH, DT> kt;
+  RowRead<KCH> kr;
+  RowRead<VCH, MAPS> vr;
+  TrRead<KCH> kt;
   kr.init(lane);
-  vr.init(lane);
+  vr.init(lane, MAPS == 2 ? m : 0);
   kt.init(lane);
 
-  f32x16 dq[MAPS][DT];
+  f32x16 dq[DT];
 #pragma unroll
-  for (int m = 0; m < MAPS; ++m)
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt) dq[m][dt] = zero16();
+  for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();
   float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f, dl_sum = 0.f;
   float dpos = 0.f, dneg = 0.f;  // diagonals rel = base + ql and base - 32 + ql of the current 32 keys, base = k0 - pw
   int next_base = 0;
@@ -121,6 +141,8 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dq_kernel(const MapAttnArg
     far_lo = bias_at<T>(a, head, -a.R);
     far_hi = bias_at<T>(a, head, a.R);
   }
+  // dS = wf P W + wd P
+  const float wf = m == 0 ? 1.f : -lam, wd = m == 0 ? -D : lam * D;
 
   if (nt_all > 0) issue(0);
   for (int t = 0; t < nt_all; ++t) {
@@ -129,20 +151,19 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dq_kernel(const MapAttnArg
     if (t + 1 < nt_all) issue(t + 1);
     const char* st = smem + (t & 1) * STAGE;
     const int kt0 = t * KT;
-    if (a.causal && kt0 > pw + 31) continue;
+    const bool skip = a.causal && kt0 > pw + 31;
+    if (MAPS == 1 && skip) continue;
 #pragma unroll
     for (int sub = 0; sub < KT / 32; ++sub) {
       const int k0 = kt0 + 32 * sub;
-      f32x16 s[MAPS], w = zero16();
+      f32x16 s = zero16(), w = zero16();
+      if (MAPS == 1 || !skip) {
 #pragma unroll
-      for (int m = 0; m < MAPS; ++m) {
-        s[m] = zero16();
+        for (int kk = 0; kk < KSV; ++kk) w = Num<T>::mfma(vr.get(st + MAPS * K_BYTES, sub, kk), df[kk], w);
+        if (MAPS == 2) put16(mine, w);
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) s[m] = Num<T>::mfma(kr.get(st + m * K_BYTES, sub, kk), qf[m][kk], s[m]);
+        for (int kk = 0; kk < KS; ++kk) s = Num<T>::mfma(kr.get(st + m * K_BYTES, sub, kk), qf[kk], s);
       }
-#pragma unroll
-      for (int kk = 0; kk < KSV; ++kk) w = Num<T>::mfma(vr.get(st + MAPS * K_BYTES, sub, kk), df[kk], w);
-
       float mul = a.scale_log2, add = 0.f;
       int zone = 0;  // -1, 1: the whole of these 32 x 32 pairs beyond the bias's reach
       if (BIAS) {
@@ -151,33 +172,35 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dq_kernel(const MapAttnArg
         else {
           const float* nb = near + (k0 + 4 * h - (pw + ql) + a.R + E);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[0][r] = fmaf(s[0][r], mul, nb[acc_row(r)]);
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mul, nb[acc_row(r)]);
           mul = 1.f;
         }
       }
       if (k0 + 31 >= len || (a.causal && k0 + 31 > pw)) {
         const int dl = lim - k0 - 4 * h;
 #pragma unroll
-        for (int m = 0; m < MAPS; ++m)
+        for (int r = 0; r < 16; ++r) s[r] = acc_row(r) > dl ? -INFINITY : s[r];
+      }
+      const float c = add + nl;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[m][r] = acc_row(r) > dl ? -INFINITY : s[m][r];
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, c));
+      if (MAPS == 2) {
+        __syncthreads();  // the other half of W is there (the next tile's comes behind its own first barrier)
+        if (skip) continue;
+        const f32x16 w2 = get16(theirs);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) w[r] += w2[r];
+        if (m == 1)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) dl_sum = fmaf(s[r], w[r], dl_sum);
       }
 #pragma unroll
-      for (int m = 0; m < MAPS; ++m) {
-        const float c = add + nl[m];
-        const float wf = m == 0 ? 1.f : -lam, wd = m == 0 ? -D[0] : lam * D[MAPS - 1];
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const float p = __builtin_amdgcn_exp2f(fmaf(s[m][r], mul, c));
-          if (MAPS == 2 && m == 1) dl_sum = fmaf(p, w[r], dl_sum);
-          s[m][r] = p * (m == 0 ? w[r] + wd : fmaf(w[r], wf, wd));
-        }
-      }
+      for (int r = 0; r < 16; ++r) s[r] *= MAPS == 1 ? w[r] - D : fmaf(w[r], wf, wd);
       if (BIAS) {
         if (zone != 0) {
           float t16 = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) t16 += s[0][r];
+          for (int r = 0; r < 16; ++r) t16 += s[r];
           if (zone < 0) sum_lo += t16;
           else sum_hi += t16;
         } else {
@@ -187,7 +210,7 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dq_kernel(const MapAttnArg
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int ko = acc_row(r) + 4 * h;
-            const float v = __uint_as_float(__builtin_amdgcn_ds_bpermute((((ko - ql) & 31) | (lane & 32)) << 2, __float_as_uint(s[0][r])));
+            const float v = __uint_as_float(__builtin_amdgcn_ds_bpermute((((ko - ql) & 31) | (lane & 32)) << 2, __float_as_uint(s[r])));
             dpos += ql <= ko ? v : 0.f;
             dneg += ql <= ko ? 0.f : v;
           }
@@ -198,15 +221,12 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dq_kernel(const MapAttnArg
         }
       }
 #pragma unroll
-      for (int m = 0; m < MAPS; ++m) {
-        u32x4 p[2];
+      for (int kb2 = 0; kb2 < 2; ++kb2) {
+        u32x4 p;
 #pragma unroll
-        for (int kb2 = 0; kb2 < 2; ++kb2) {
+        for (int i = 0; i < 4; ++i) p[i] = Num<T>::pack(s[8 * kb2 + 2 * i], s[8 * kb2 + 2 * i + 1]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) p[kb2][i] = Num<T>::pack(s[m][8 * kb2 + 2 * i], s[m][8 * kb2 + 2 * i + 1]);
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) dq[m][dt] = Num<T>::mfma(kt.get(st + m * K_BYTES, 2 * sub + kb2, dt), p[kb2], dq[m][dt]);
-        }
+        for (int dt = 0; dt < DT; ++dt) dq[dt] = Num<T>::mfma(kt.get(st + m * K_BYTES, 2 * sub + kb2, dt), p, dq[dt]);
       }
     }
   }
@@ -220,53 +240,56 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dq_kernel(const MapAttnArg
       diag[a.ND + 1] = hi;
     }
   }
-  if (MAPS == 2 && q0 < a.Tq) {
+  if (MAPS == 2 && m == 1 && q0 < a.Tq) {
     const float t = wave_sum(dl_sum);
     if (lane == 0) a.dlam_part[((int64_t)head * a.B + b) * a.QW + q0 / 32] = -t;
   }
   if (!valid) return;
+  char* op = (char*)a.dq + ((((int64_t)b * a.Tq + qi) * a.H + head) * MAPS + m) * a.d * 2;
 #pragma unroll
-  for (int m = 0; m < MAPS; ++m) {
-    char* op = (char*)a.dq + ((((int64_t)b * a.Tq + qi) * a.H + head) * MAPS + m) * a.d * 2;
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int rq = 0; rq < 4; ++rq) {
-        const int c0 = dt * 32 + rq * 8 + h * 4;
-        const f32x16& x = dq[m][dt];
-        if (c0 < a.d)
-          *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale), Num<T>::pack(x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale)};
-      }
-  }
+    for (int rq = 0; rq < 4; ++rq) {
+      const int c0 = dt * 32 + rq * 8 + h * 4;
+      const f32x16& x = dq[dt];
+      if (c0 < a.d)
+        *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale), Num<T>::pack(x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale)};
+    }
 }
 
-// ---- dK, dV: 32 keys per wave (K and V rows in registers), tiles of QT queries of every head that shares them ------------------
-template <typename T, int MAPS, int KS, int NT, int QT, int NW>
-__global__ __launch_bounds__(64 * NW, 1) void mapattn_dkv_kernel(const MapAttnArgs a) {
+// ---- dK, dV: 32 keys per wave (pair; K and V rows in registers), tiles of QT queries of every head that shares them ------------
+template <typename T, int MAPS, int KS, int NT, int QT, int NG>
+__global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) void mapattn_dkv_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
-  constexpr int BK = 32 * NW, DT = (KS + 1) / 2, KSV = MAPS == 1 ? KS : 2 * NT;
+  constexpr int NW = NG * MAPS, BK = 32 * NG, DT = (KS + 1) / 2;
+  constexpr int KSV = MAPS == 1 ? KS : NT;               // steps over this wave's share of dv in W
+  constexpr int VT = MAPS == 1 ? NT : (NT + 1) / 2;      // 32-channel tiles of this wave's share of dV
   constexpr int QCH = 4 * DT, OCH = 4 * NT;
   constexpr int Q_BYTES = QT * QCH * 16, O_BYTES = QT * OCH * 16, R_BYTES = 256;
   constexpr int STAGE = MAPS * Q_BYTES + O_BYTES + 2 * MAPS * R_BYTES;
   constexpr int E = BK + QT;
+  static_assert(MAPS == 1 || QT == 32, "the pair's exchange has one slot per tile");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  float* near = (float*)(smem + 2 * STAGE);
+  float* near = (float*)(smem + 2 * STAGE);  // (one map)
 
   const int tid = threadIdx.x, lane = tid & 63, kl = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int grp = wave / MAPS, m = wave % MAPS;
+  float* mine = (float*)(smem + 2 * STAGE) + wave * 2048 + lane * 4;         // (two maps) 16 values of W, 16 of P of each lane
+  float* theirs = (float*)(smem + 2 * STAGE) + (wave ^ 1) * 2048 + lane * 4;
   const int nkb = (a.Tk + BK - 1) / BK;
   int kblk, bk;
-  if (!place(blockIdx.x, nkb, a.B * a.Hkv, kblk, bk)) return;  // causal: the first keys meet the most queries
+  if (!place(blockIdx.x, nkb * a.splits, a.B * a.Hkv, kblk, bk)) return;  // causal: the first keys meet the most queries
+  const int split = kblk % a.splits;
+  kblk /= a.splits;
   const int b = bk / a.Hkv, kvh = bk - b * a.Hkv;
   const int len = seq_len(a, b), start = seq_start(a, b);
-  const int kw0 = kblk * BK + wave * 32, key = kw0 + kl;
+  const int kw0 = kblk * BK + grp * 32, key = kw0 + kl;
   const bool valid = key < len;
 
-  u32x4 kf[MAPS][KS], vf[KSV];
-#pragma unroll
-  for (int m = 0; m < MAPS; ++m)
-    load_row<KS>(kf[m], (const char*)a.k + 2 * (b * a.k_sb + (int64_t)key * a.k_st + (int64_t)(kvh * MAPS + m) * a.k_sh), valid, h, a.d);
-  load_row<KSV>(vf, (const char*)a.v + 2 * (b * a.v_sb + (int64_t)key * a.v_st + (int64_t)kvh * a.v_sh), valid, h, a.dv);
+  u32x4 kf[KS], vf[KSV];
+  load_row<KS>(kf, (const char*)a.k + 2 * (b * a.k_sb + (int64_t)key * a.k_st + (int64_t)(kvh * MAPS + m) * a.k_sh), valid, h, a.d);
+  load_row<KSV, MAPS>(vf, (const char*)a.v + 2 * (b * a.v_sb + (int64_t)key * a.v_st + (int64_t)kvh * a.v_sh), valid, h, a.dv, m);
 
   // ---- query tiles that meet these keys -----------------------------------------------------------------------------------
   const int nqt = (a.Tq + QT - 1) / QT;
@@ -275,7 +298,8 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dkv_kernel(const MapAttnAr
     const int first = kblk * BK - start;  // first query that sees the workgroup's first key
     tq0 = first <= 0 ? 0 : min(first / QT, nqt);
   }
-  const int per = kblk * BK < len ? nqt - tq0 : 0, total = per * a.G;
+  const int per = kblk * BK < len ? nqt - tq0 : 0, all = per * a.G;
+  const int it0 = (int)((int64_t)all * split / a.splits), total = (int)((int64_t)all * (split + 1) / a.splits);
 
   TileDma<QCH, QT, NW> qd;
   TileDma<OCH, QT, NW> od;
@@ -287,8 +311,8 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dkv_kernel(const MapAttnAr
     const int64_t row = (int64_t)t * QT;
     const int n = a.Tq - t * QT;
 #pragma unroll
-    for (int m = 0; m < MAPS; ++m)
-      qd.issue((const char*)a.q + 2 * (b * a.q_sb + row * a.q_st + (int64_t)(head * MAPS + m) * a.q_sh), n, st + m * Q_BYTES, wave);
+    for (int i = 0; i < MAPS; ++i)
+      qd.issue((const char*)a.q + 2 * (b * a.q_sb + row * a.q_st + (int64_t)(head * MAPS + i) * a.q_sh), n, st + i * Q_BYTES, wave);
     od.issue((const char*)a.dout + 2 * (b * a.do_sb + row * a.do_st + (int64_t)head * a.do_sh), n, st + MAPS * Q_BYTES, wave);
     char* rt = st + MAPS * Q_BYTES + O_BYTES;
 #pragma unroll
@@ -298,32 +322,30 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dkv_kernel(const MapAttnAr
         dma4(src, QT * 4, rt + i * R_BYTES, lane * 4);
       }
   };
-  RowRead<QCH, KS> qr;
-  RowRead<OCH, KSV> orr;
-  TrRead<QCH, DT> qt;
-  TrRead<OCH, NT> ot;
+  RowRead<QCH> qr;
+  RowRead<OCH, MAPS> orr;
+  TrRead<QCH> qt;
+  TrRead<OCH> ot;
   qr.init(lane);
-  orr.init(lane);
+  orr.init(lane, MAPS == 2 ? m : 0);
   qt.init(lane);
-  ot.init(lane);
+  ot.init(lane, m * VT);
 
-  f32x16 dk[MAPS][DT], dv[NT];
+  f32x16 dk[DT], dv[VT];
 #pragma unroll
-  for (int m = 0; m < MAPS; ++m)
+  for (int dt = 0; dt < DT; ++dt) dk[dt] = zero16();
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) dk[m][dt] = zero16();
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) dv[nt] = zero16();
+  for (int nt = 0; nt < VT; ++nt) dv[nt] = zero16();
   float far_lo = 0.f, far_hi = 0.f, lam = 0.f;
   constexpr float PF = 1.0f / (1 << Num<T>::PSH);
 
-  if (total > 0) issue(0);
-  for (int it = 0; it < total; ++it) {
+  if (it0 < total) issue(it0);
+  for (int it = it0; it < total; ++it) {
     const int g = it / per, t = tq0 + it - g * per;
-    if (it - g * per == 0) {  // the next head: its bias, its lam
+    if (it == it0 || it - g * per == 0) {  // the next head: its bias, its lam
       const int head = kvh * a.G + g;
       if (BIAS) {
-        if (g > 0) __syncthreads();  // the head before is read to the end
+        if (it > it0) __syncthreads();  // the head before is read to the end
         fill_near<T>(a, head, E, near, tid, 64 * NW);
         far_lo = bias_at<T>(a, head, -a.R);
         far_hi = bias_at<T>(a, head, a.R);
@@ -334,22 +356,28 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dkv_kernel(const MapAttnAr
     MAPATTN_WAIT_DMA();
     __syncthreads();
     if (it + 1 < total) issue(it + 1);
+    if (MAPS * NT >= 16) {
+      opaque(qr.base);
+      opaque(orr.base);
+      opaque(qt.base);
+      opaque(ot.base);
+    }
     const char* st = smem + (it & 1) * STAGE;
     const char* rt = st + MAPS * Q_BYTES + O_BYTES;
     const int pt = start + t * QT;
-    if (a.causal && pt + QT - 1 < kw0) continue;  // no query of the tile sees this wave's keys
+    const bool skip = a.causal && pt + QT - 1 < kw0;  // no query of the tile sees this wave's keys
+    if (MAPS == 1 && skip) continue;
 #pragma unroll
     for (int sub = 0; sub < QT / 32; ++sub) {
       const int pq = pt + 32 * sub;
-      f32x16 s[MAPS], w = zero16();
+      f32x16 s = zero16(), w = zero16();
+      if (MAPS == 1 || !skip) {
 #pragma unroll
-      for (int m = 0; m < MAPS; ++m) {
-        s[m] = zero16();
+        for (int kk = 0; kk < KSV; ++kk) w = Num<T>::mfma(orr.get(st + MAPS * Q_BYTES, sub, kk), vf[kk], w);
+        if (MAPS == 2) put16(mine, w);
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) s[m] = Num<T>::mfma(qr.get(st + m * Q_BYTES, sub, kk), kf[m][kk], s[m]);
+        for (int kk = 0; kk < KS; ++kk) s = Num<T>::mfma(qr.get(st + m * Q_BYTES, sub, kk), kf[kk], s);
       }
-#pragma unroll
-      for (int kk = 0; kk < KSV; ++kk) w = Num<T>::mfma(orr.get(st + MAPS * Q_BYTES, sub, kk), vf[kk], w);
       float mul = a.scale_log2, add = 0.f;
       if (BIAS) {
         if (kw0 + 31 - pq <= -a.R) add = far_lo;
@@ -357,82 +385,129 @@ __global__ __launch_bounds__(64 * NW, 1) void mapattn_dkv_kernel(const MapAttnAr
         else {
           const float* nb = near + (key - pq - 4 * h + a.R + E);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[0][r] = fmaf(s[0][r], mul, nb[-acc_row(r)]);
+          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mul, nb[-acc_row(r)]);
           mul = 1.f;
         }
       }
       if (kw0 + 31 >= len || (a.causal && kw0 + 31 > pq)) {
         const int dl = !valid ? 64 : (a.causal ? key - pq - 4 * h : -64);  // rows before dl do not see this lane's key
 #pragma unroll
-        for (int m = 0; m < MAPS; ++m)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[m][r] = acc_row(r) < dl ? -INFINITY : s[m][r];
+        for (int r = 0; r < 16; ++r) s[r] = acc_row(r) < dl ? -INFINITY : s[r];
       }
       // P' = 2^PSH P; rows_lse and rows_d carry 2^PSH and 2^-PSH
-      f32x16 ds[MAPS];
 #pragma unroll
       for (int rq = 0; rq < 4; ++rq) {
-        f32x4 nl[MAPS], D[MAPS];
+        const f32x4 nl = *(const f32x4*)(rt + m * R_BYTES + (32 * sub + 8 * rq + 4 * h) * 4);
 #pragma unroll
-        for (int m = 0; m < MAPS; ++m) {
-          nl[m] = *(const f32x4*)(rt + m * R_BYTES + (32 * sub + 8 * rq + 4 * h) * 4);
-          D[m] = *(const f32x4*)(rt + (MAPS + m) * R_BYTES + (32 * sub + 8 * rq + 4 * h) * 4);
+        for (int e = 0; e < 4; ++e) s[4 * rq + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * rq + e], mul, nl[e] + add));
+      }
+      u32x4 pv[2];  // what meets dO in dV
+      if (MAPS == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) pv[i >> 2][i & 3] = Num<T>::pack(s[2 * i], s[2 * i + 1]);
+      } else {
+        if (!skip) put16(mine + 1024, s);
+        __syncthreads();
+        if (skip) continue;
+        const float f1 = m == 0 ? 1.f : -lam, f2 = m == 0 ? -lam : 1.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const f32x4 w2 = *(const f32x4*)(theirs + i * 256), p2 = *(const f32x4*)(theirs + 1024 + i * 256);
+          float pc[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            w[4 * i + e] += w2[e];
+            pc[e] = fmaf(f1, s[4 * i + e], f2 * p2[e]);
+          }
+          pv[i >> 1][2 * (i & 1)] = Num<T>::pack(pc[0], pc[1]);
+          pv[i >> 1][2 * (i & 1) + 1] = Num<T>::pack(pc[2], pc[3]);
         }
+      }
+#pragma unroll
+      for (int kb2 = 0; kb2 < 2; ++kb2)
+#pragma unroll
+        for (int nt = 0; nt < VT; ++nt)
+          if (MAPS == 1 || NT % 2 == 0 || m * VT + nt < NT) dv[nt] = Num<T>::mfma(ot.get(st + MAPS * Q_BYTES, 2 * sub + kb2, nt), pv[kb2], dv[nt]);
+      const float wf = m == 0 ? PF : -lam * PF, wd = m == 0 ? -1.f : lam;
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const f32x4 D = *(const f32x4*)(rt + (MAPS + m) * R_BYTES + (32 * sub + 8 * rq + 4 * h) * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * rq + e;
-#pragma unroll
-          for (int m = 0; m < MAPS; ++m) s[m][r] = __builtin_amdgcn_exp2f(fmaf(s[m][r], mul, nl[m][e] + add));
-          ds[0][r] = s[0][r] * fmaf(w[r], PF, -D[0][e]);
-          if (MAPS == 2) {
-            ds[MAPS - 1][r] = -lam * (s[MAPS - 1][r] * fmaf(w[r], PF, -D[MAPS - 1][e]));
-            s[0][r] = fmaf(-lam, s[MAPS - 1][r], s[0][r]);
-          }
+          s[r] *= MAPS == 1 ? fmaf(w[r], PF, -D[e]) : fmaf(w[r], wf, wd * D[e]);
         }
       }
 #pragma unroll
       for (int kb2 = 0; kb2 < 2; ++kb2) {
         u32x4 p;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = Num<T>::pack(s[0][8 * kb2 + 2 * i], s[0][8 * kb2 + 2 * i + 1]);
+        for (int i = 0; i < 4; ++i) p[i] = Num<T>::pack(s[8 * kb2 + 2 * i], s[8 * kb2 + 2 * i + 1]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) dv[nt] = Num<T>::mfma(ot.get(st + MAPS * Q_BYTES, 2 * sub + kb2, nt), p, dv[nt]);
-#pragma unroll
-        for (int m = 0; m < MAPS; ++m) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) p[i] = Num<T>::pack(ds[m][8 * kb2 + 2 * i], ds[m][8 * kb2 + 2 * i + 1]);
-#pragma unroll
-          for (int dt = 0; dt < DT; ++dt) dk[m][dt] = Num<T>::mfma(qt.get(st + m * Q_BYTES, 2 * sub + kb2, dt), p, dk[m][dt]);
-        }
+        for (int dt = 0; dt < DT; ++dt) dk[dt] = Num<T>::mfma(qt.get(st + m * Q_BYTES, 2 * sub + kb2, dt), p, dk[dt]);
       }
     }
   }
 
   if (key >= a.Tk) return;  // keys behind len get zeros
   const int64_t row = ((int64_t)b * a.Tk + key) * a.Hkv + kvh;
-#pragma unroll
-  for (int m = 0; m < MAPS; ++m) {
-    char* op = (char*)a.dk + (row * MAPS + m) * a.d * 2;
+  if (a.splits > 1) {  // 32-bit parts, (dk of each map, dv) of a key together
+    float* pp = a.part_o + ((int64_t)split * a.B * a.Tk * a.Hkv + row) * (2 * a.dv);
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int rq = 0; rq < 4; ++rq) {
         const int c0 = dt * 32 + rq * 8 + h * 4;
-        const f32x16& x = dk[m][dt];
-        if (c0 < a.d)
-          *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale), Num<T>::pack(x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale)};
+        const f32x16& x = dk[dt];
+        if (c0 < a.d) *(f32x4*)(pp + m * a.d + c0) = f32x4{x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale, x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale};
       }
-  }
-  char* op = (char*)a.dvo + row * a.dv * 2;
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < VT; ++nt)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const int c0 = (m * VT + nt) * 32 + rq * 8 + h * 4;
+        const f32x16& x = dv[nt];
+        if (c0 < a.dv) *(f32x4*)(pp + a.dv + c0) = f32x4{x[4 * rq] * PF, x[4 * rq + 1] * PF, x[4 * rq + 2] * PF, x[4 * rq + 3] * PF};
+      }
+    return;
+  }
+  char* op = (char*)a.dk + (row * MAPS + m) * a.d * 2;
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
     for (int rq = 0; rq < 4; ++rq) {
-      const int c0 = nt * 32 + rq * 8 + h * 4;
+      const int c0 = dt * 32 + rq * 8 + h * 4;
+      const f32x16& x = dk[dt];
+      if (c0 < a.d)
+        *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale), Num<T>::pack(x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale)};
+    }
+  op = (char*)a.dvo + row * a.dv * 2;
+#pragma unroll
+  for (int nt = 0; nt < VT; ++nt)
+#pragma unroll
+    for (int rq = 0; rq < 4; ++rq) {
+      const int c0 = (m * VT + nt) * 32 + rq * 8 + h * 4;
       const f32x16& x = dv[nt];
       if (c0 < a.dv)
         *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * PF, x[4 * rq + 1] * PF), Num<T>::pack(x[4 * rq + 2] * PF, x[4 * rq + 3] * PF)};
     }
+}
+
+// dK, dV from the parts of a split walk: one thread per 4 channels, the parts in their order
+template <typename T>
+__global__ __launch_bounds__(256) void mapattn_dkv_join_kernel(const MapAttnArgs a) {
+  const int64_t rows = (int64_t)a.B * a.Tk * a.Hkv;
+  const int qn = a.dv / 2;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= rows * qn) return;
+  const int64_t row = i / qn;
+  const int c0 = (int)(i - row * qn) * 4;
+  const float* p = a.part_o + row * (2 * a.dv) + c0;
+  f32x4 t = *(const f32x4*)p;
+#pragma unroll 4
+  for (int s = 1; s < a.splits; ++s) t += *(const f32x4*)(p + (int64_t)s * rows * (2 * a.dv));
+  char* op = c0 < a.dv ? (char*)a.dk + (row * a.dv + c0) * 2 : (char*)a.dvo + (row * a.dv + c0 - a.dv) * 2;
+  *(u32x2*)op = u32x2{Num<T>::pack(t[0], t[1]), Num<T>::pack(t[2], t[3])};
 }
 
 // ---- sums of the query groups' parts, in a fixed order --------------------------------------------------------------------
@@ -443,36 +518,32 @@ __global__ __launch_bounds__(256) void mapattn_diag_kernel(const MapAttnArgs a) 
   const int64_t rows = (int64_t)a.B * a.QW, r0 = rows * part / a.parts, r1 = rows * (part + 1) / a.parts;
   const float* p = a.diag + ((int64_t)head * rows) * (a.ND + 2) + slot;
   float t = 0.f;
+#pragma unroll 8
   for (int64_t r = r0; r < r1; ++r) t += p[r * (a.ND + 2)];
   a.diag_part[((int64_t)head * a.parts + part) * (a.ND + 2) + slot] = t;
 }
+// a head's bucket sums: the parts added per slot, then a wave per bucket adds the slots that belong to it
 template <typename T>
-__global__ __launch_bounds__(256) void mapattn_dtable_kernel(const MapAttnArgs a) {
+__global__ __launch_bounds__(1024) void mapattn_dtable_kernel(const MapAttnArgs a) {
   extern __shared__ float sums[];
-  const int head = blockIdx.x, n = a.ND + 2;
-  for (int x = threadIdx.x; x < n; x += 256) {
+  const int head = blockIdx.x, n = a.ND + 2, lane = threadIdx.x & 63;
+  for (int x = threadIdx.x; x < n; x += 1024) {
     float t = 0.f;
+#pragma unroll 8
     for (int p = 0; p < a.parts; ++p) t += a.diag_part[((int64_t)head * a.parts + p) * n + x];
     sums[x] = t;
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < a.NB; c += 256) {
+  for (int c = threadIdx.x >> 6; c < a.NB; c += 16) {
     float t = 0.f;
-    for (int x = 0; x <= 2 * a.R; ++x) {
-      int bx = a.buckets[x];
+    for (int x = lane; x < a.ND; x += 64) {  // slot x: relative position x - R - 64, beyond +-R as +-R
+      const int r = x < 64 ? 0 : (x > 2 * a.R + 64 ? 2 * a.R : x - 64);
+      int bx = a.buckets[r];
       bx = bx < 0 ? 0 : (bx >= a.NB ? a.NB - 1 : bx);
-      if (bx != c) continue;
-      t += sums[x + 64];
-      if (x == 0) {
-        t += sums[a.ND];
-        for (int i = 0; i < 64; ++i) t += sums[i];
-      }
-      if (x == 2 * a.R) {
-        t += sums[a.ND + 1];
-        for (int i = 2 * a.R + 65; i < a.ND; ++i) t += sums[i];
-      }
+      if (bx == c) t += sums[x] + (x == 64 ? sums[a.ND] : 0.f) + (x == 2 * a.R + 64 ? sums[a.ND + 1] : 0.f);
     }
-    ((T*)a.dtable)[(int64_t)head * a.NB + c] = (T)t;
+    t = wave_sum(t);
+    if (lane == 0) ((T*)a.dtable)[(int64_t)head * a.NB + c] = (T)t;
   }
 }
 __global__ __launch_bounds__(256) void mapattn_dlam_kernel(const MapAttnArgs a) {
@@ -490,31 +561,31 @@ __global__ __launch_bounds__(256) void mapattn_dlam_kernel(const MapAttnArgs a) 
 // ---- dispatch -----------------------------------------------------------------------------------------------------------
 namespace {
 
-template <typename T, int MAPS, int KS, int NT, int NW>
+template <typename T, int MAPS, int KS, int NT, int NG>
 int run_dq(const MapAttnArgs& a, hipStream_t s) {
   constexpr int ROW = 16 * (MAPS * 4 * ((KS + 1) / 2) + 4 * NT);
-  constexpr int KT = (NW == 1 || 2 * 64 * ROW > 64 * 1024) ? 32 : 64;
-  const int lds = 2 * KT * ROW + (MAPS == 1 ? (2 * (a.R + 32 * NW + KT) + 1) * 4 : 0);
-  const void* f = (const void*)mapattn_dq_kernel<T, MAPS, KS, NT, KT, NW>;
+  constexpr int KT = (MAPS == 2 || NG == 1 || 2 * 64 * ROW > 64 * 1024) ? 32 : 64;
+  const int lds = 2 * KT * ROW + (MAPS == 1 ? (2 * (a.R + 32 * NG + KT) + 1) * 4 : 2 * NG * 4096);
+  const void* f = (const void*)mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG>;
   if (anip_raise_lds_limit(f, lds) != 0) {
     anip_set_error("mapattn dq: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
-  hipLaunchKernelGGL((mapattn_dq_kernel<T, MAPS, KS, NT, KT, NW>), dim3((unsigned)(a.Tp / (32 * NW) * a.B * a.H)), dim3(64 * NW), lds, s, a);
+  hipLaunchKernelGGL((mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG>), dim3((unsigned)(a.Tp / (32 * NG) * a.B * a.H)), dim3(64 * NG * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dq_kernel");
   return 0;
 }
-template <typename T, int MAPS, int KS, int NT, int NW>
+template <typename T, int MAPS, int KS, int NT, int NG>
 int run_dkv(const MapAttnArgs& a, hipStream_t s) {
   constexpr int ROW = 16 * (MAPS * 4 * ((KS + 1) / 2) + 4 * NT);
-  constexpr int QT = (NW == 1 || 2 * 64 * ROW > 64 * 1024) ? 32 : 64;
-  const int lds = 2 * (QT * ROW + 2 * MAPS * 256) + (MAPS == 1 ? (2 * (a.R + 32 * NW + QT) + 1) * 4 : 0);
-  const void* f = (const void*)mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NW>;
+  constexpr int QT = (MAPS == 2 || NG == 1 || 2 * 64 * ROW > 64 * 1024) ? 32 : 64;
+  const int lds = 2 * (QT * ROW + 2 * MAPS * 256) + (MAPS == 1 ? (2 * (a.R + 32 * NG + QT) + 1) * 4 : 2 * NG * 8192);
+  const void* f = (const void*)mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG>;
   if (anip_raise_lds_limit(f, lds) != 0) {
     anip_set_error("mapattn dkv: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
-  hipLaunchKernelGGL((mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NW>), dim3((unsigned)((a.Tk + 32 * NW - 1) / (32 * NW) * a.B * a.Hkv)), dim3(64 * NW), lds, s, a);
+  hipLaunchKernelGGL((mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG>), dim3((unsigned)((a.Tk + 32 * NG - 1) / (32 * NG) * a.splits * a.B * a.Hkv)), dim3(64 * NG * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dkv_kernel");
   return 0;
 }
@@ -541,7 +612,15 @@ int dkv_t(const MapAttnArgs& a, int maps, int nw, hipStream_t s) {
 }  // namespace
 
 int mapattn_dq(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) { return bf16 ? dq_t<bf16_t>(a, maps, nw, s) : dq_t<f16>(a, maps, nw, s); }
-int mapattn_dkv(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) { return bf16 ? dkv_t<bf16_t>(a, maps, nw, s) : dkv_t<f16>(a, maps, nw, s); }
+int mapattn_dkv(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) {
+  const int r = bf16 ? dkv_t<bf16_t>(a, maps, nw, s) : dkv_t<f16>(a, maps, nw, s);
+  if (r || a.splits == 1) return r;
+  const dim3 grid((unsigned)cdiv64((int64_t)a.B * a.Tk * a.Hkv * (a.dv / 2), 256));
+  if (bf16) hipLaunchKernelGGL((mapattn_dkv_join_kernel<bf16_t>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((mapattn_dkv_join_kernel<f16>), grid, dim3(256), 0, s, a);
+  ANIP_LAUNCH_CHECK("mapattn_dkv_join_kernel");
+  return 0;
+}
 int mapattn_reduce(const MapAttnArgs& a, int maps, int bf16, hipStream_t s) {
   if (maps == 2) {
     hipLaunchKernelGGL(mapattn_dlam_kernel, dim3((unsigned)a.H), dim3(256), 0, s, a);
@@ -551,8 +630,8 @@ int mapattn_reduce(const MapAttnArgs& a, int maps, int bf16, hipStream_t s) {
   hipLaunchKernelGGL(mapattn_diag_kernel, dim3((unsigned)((a.ND + 2 + 255) / 256), (unsigned)a.parts, (unsigned)a.H), dim3(256), 0, s, a);
   ANIP_LAUNCH_CHECK("mapattn_diag_kernel");
   const int lds = (a.ND + 2) * 4;
-  if (bf16) hipLaunchKernelGGL((mapattn_dtable_kernel<bf16_t>), dim3((unsigned)a.H), dim3(256), lds, s, a);
-  else hipLaunchKernelGGL((mapattn_dtable_kernel<f16>), dim3((unsigned)a.H), dim3(256), lds, s, a);
+  if (bf16) hipLaunchKernelGGL((mapattn_dtable_kernel<bf16_t>), dim3((unsigned)a.H), dim3(1024), lds, s, a);
+  else hipLaunchKernelGGL((mapattn_dtable_kernel<f16>), dim3((unsigned)a.H), dim3(1024), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dtable_kernel");
   return 0;
 }

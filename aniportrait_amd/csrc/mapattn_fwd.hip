@@ -94,8 +94,8 @@ __global__ __launch_bounds__(256 * MAPS, 2) void mapattn_fwd_kernel(const MapAtt
     for (int i = 0; i < MAPS; ++i) kd.issue(kb[i] + row * a.k_st * 2, valid, st + i * K_BYTES, wave);
     vd.issue(vb + row * a.v_st * 2, valid, st + MAPS * K_BYTES, wave);
   };
-  RowRead<KCH, KS> kr;
-  TrRead<VCH, NT> vr;
+  RowRead<KCH> kr;
+  TrRead<VCH> vr;
   kr.init(lane);
   vr.init(lane);
 
@@ -115,6 +115,10 @@ __global__ __launch_bounds__(256 * MAPS, 2) void mapattn_fwd_kernel(const MapAtt
     MAPATTN_WAIT_DMA();
     __syncthreads();  // tile t is there for all waves; nobody reads the other stage any more
     if (t + 1 < t1) issue(t + 1);
+    if (MAPS * NT >= 16) {
+      opaque(kr.base);
+      opaque(vr.base);
+    }
     const char* st = smem + (t & 1) * STAGE;
     const int kt0 = t * KT;
     if (a.causal && kt0 > pw + 31) continue;  // nothing of this tile is seen by this wave
@@ -260,8 +264,8 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
     vd.issue(vb + row * a.v_st * 2, valid, p + MAPS * K_BYTES, m);
   };
   constexpr int PIECES = TileDma<KCH, KT, 1>::P + TileDma<VCH, KT, 1>::P;  // (MAPS = 1)
-  RowRead<KCH, KS> kr;
-  TrRead<VCH, NT> vr;
+  RowRead<KCH> kr;
+  TrRead<VCH> vr;
   kr.init(lane);
   vr.init(lane);
 
@@ -419,39 +423,68 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
     }
 }
 
-// ---- joins the parts of a split forward: o = sum_s 2^(l_s - l) o_s, l = log2 sum_s 2^l_s; one thread per 4 channels -----------
-template <typename T, int MAPS>
+// ---- joins the parts of a split forward: o = sum_s 2^(l_s - l) o_s, l = log2 sum_s 2^l_s -----------------------------------------
+// One wave per row: lane s holds the weight of parts s, s + 64, ..; 64 / LR parts are added at once by LR lanes of 4 channels each.
+template <typename T, int MAPS, int LR>
 __global__ __launch_bounds__(256) void mapattn_combine_kernel(const MapAttnArgs a) {
+  constexpr int PG = 64 / LR, MW = 4;  // parts at once; weights of a lane (256 parts at most)
   const int64_t rows = (int64_t)a.B * a.Tq * a.H;
-  const int qn = a.dv / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * qn) return;
-  const int64_t row = i / qn;
-  const int c0 = (int)(i - row * qn) * 4;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 63, c0 = (lane % LR) * 4, sg = lane / LR;
   float x[MAPS][4], lse2[MAPS];
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    float mx = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, a.part_l[((int64_t)s * rows + row) * MAPS + m]);
+    float lw[MW], mx = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < MW; ++i) {
+      const int s = lane + 64 * i;
+      lw[i] = s < a.splits ? a.part_l[((int64_t)s * rows + row) * MAPS + m] : -INFINITY;
+      mx = fmaxf(mx, lw[i]);
+    }
+    mx = wave_max(mx);
     const float base = mx == -INFINITY ? 0.f : mx;
     float sum = 0.f;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < a.splits; ++s) {
-      const int64_t at = ((int64_t)s * rows + row) * MAPS + m;
-      const float w = __builtin_amdgcn_exp2f(a.part_l[at] - base);
-      sum += w;
-      const f32x4 v = *(const f32x4*)(a.part_o + at * a.dv + c0);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+    for (int i = 0; i < MW; ++i) {
+      lw[i] = __builtin_amdgcn_exp2f(lw[i] - base);
+      sum += lw[i];
     }
+    sum = wave_sum(sum);
     const bool none = mx == -INFINITY;
     const float inv = none ? 0.f : 1.0f / sum;
     lse2[m] = none ? -INFINITY : base + __builtin_amdgcn_logf(sum);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[m][e] = acc[e] * inv;
+    for (int i = 0; i < MW; ++i) {
+      if (64 * i >= a.splits) break;
+      const int n = min(64, a.splits - 64 * i);
+#pragma unroll 4
+      for (int s0 = 0; s0 < n; s0 += PG) {
+        const int s = s0 + sg;  // (a part behind the last weighs nothing)
+        const float w = __shfl(lw[i], s & 63, 64);
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (s < n && c0 < a.dv) v = *(const f32x4*)(a.part_o + (((int64_t)(s + 64 * i) * rows + row) * MAPS + m) * a.dv + c0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float t = acc[e];
+#pragma unroll
+      for (int o = LR; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
+      x[m][e] = t * inv;
+    }
   }
   const int head = (int)(row % a.H);
   const int64_t bt = row / a.H;
+  if (a.lse && lane == 0) {
+    const int64_t b = bt / a.Tq, qi = bt - b * a.Tq;
+#pragma unroll
+    for (int m = 0; m < MAPS; ++m) a.lse[((b * a.H + head) * MAPS + m) * a.Tq + qi] = lse2[m] * LN2;
+  }
+  if (sg != 0 || c0 >= a.dv) return;
   if (MAPS == 2) {
     if (a.out2) *(u32x2*)((char*)a.out2 + (row * a.dv + c0) * 2) = u32x2{Num<T>::pack(x[MAPS - 1][0], x[MAPS - 1][1]), Num<T>::pack(x[MAPS - 1][2], x[MAPS - 1][3])};
     const float lam = a.lam[head];
@@ -459,11 +492,6 @@ __global__ __launch_bounds__(256) void mapattn_combine_kernel(const MapAttnArgs 
     for (int e = 0; e < 4; ++e) x[0][e] -= lam * x[MAPS - 1][e];
   }
   *(u32x2*)((char*)a.out + (row * a.dv + c0) * 2) = u32x2{Num<T>::pack(x[0][0], x[0][1]), Num<T>::pack(x[0][2], x[0][3])};
-  if (a.lse && c0 == 0) {
-    const int64_t b = bt / a.Tq, qi = bt - b * a.Tq;
-#pragma unroll
-    for (int m = 0; m < MAPS; ++m) a.lse[((b * a.H + head) * MAPS + m) * a.Tq + qi] = lse2[m] * LN2;
-  }
 }
 
 // ---- dispatch -----------------------------------------------------------------------------------------------------------
@@ -511,8 +539,10 @@ int run_token(const MapAttnArgs& a0, hipStream_t s) {
 
 template <typename T, int MAPS>
 int run_combine(const MapAttnArgs& a, hipStream_t s) {
-  const int64_t n = (int64_t)a.B * a.Tq * a.H * (a.dv / 4);
-  hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS>), dim3((unsigned)cdiv64(n, 256)), dim3(256), 0, s, a);
+  const dim3 grid((unsigned)cdiv64((int64_t)a.B * a.Tq * a.H, 4));
+  if (a.dv <= 64) hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, 16>), grid, dim3(256), 0, s, a);
+  else if (a.dv <= 128) hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, 32>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, 64>), grid, dim3(256), 0, s, a);
   ANIP_LAUNCH_CHECK("mapattn_combine_kernel");
   return 0;
 }
