@@ -110,7 +110,7 @@ SIGNATURES = {
     "anip_temporal_qkv_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                             c_int, c_float, c_float, c_void_p]),
     "anip_qk_norm_rope": (c_int, [C.POINTER(QkNormParams), c_void_p]),
-    "anip_qk_norm_rope_backward_ws_floats": (c_int64, [c_int64, c_int, c_int]),
+    "anip_qk_norm_rope_backward_ws_floats": (c_int64, [c_int64, c_int, c_int, c_int]),
     "anip_qk_norm_rope_backward": (c_int, [C.POINTER(QkNormParams), c_void_p]),
     "anip_relative_attention_ws_bytes": (c_int64, [C.POINTER(AttnParams), c_int]),
     "anip_relative_attention": (c_int, [C.POINTER(AttnParams), c_void_p]),

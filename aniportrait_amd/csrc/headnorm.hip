@@ -21,7 +21,7 @@ struct HeadNormArgs {
   const float* w[2];
   const float* rope;
   const int* positions;
-  int64_t M;
+  int64_t M, items;
   int T, H[2], d, rot, hc, rope_rows, inter;
   float eps, inv_d, alpha;
   float* part;  // [block][2][d]
@@ -40,34 +40,38 @@ __device__ __forceinline__ void widen(float (&x)[8], u32x2 u, u32x2 v) {
   }
 }
 template <typename T>
-__device__ __forceinline__ void load8(float (&x)[8], const char* row, int a, int b) {
-  widen<T>(x, *(const u32x2*)(row + 2 * a), *(const u32x2*)(row + 2 * b));
-}
-template <typename T>
 __device__ __forceinline__ void store8(char* row, int a, int b, const float (&x)[8]) {
   *(u32x2*)(row + 2 * a) = u32x2{Num<T>::pack(x[0], x[1]), Num<T>::pack(x[2], x[3])};
   *(u32x2*)(row + 2 * b) = u32x2{Num<T>::pack(x[4], x[5]), Num<T>::pack(x[6], x[7])};
 }
+// sum over groups of L lanes, in the vector ALU: quads, then mirrored halves and rows of 16, then the row 16 lanes on
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  v = dpp_add<0xB1>(v);                // quad_perm [1, 0, 3, 2]
+  v = dpp_add<0x4E>(v);                // quad_perm [2, 3, 0, 1]
+  if (L >= 8) v = dpp_add<0x141>(v);   // row_half_mirror
+  if (L >= 16) v = dpp_add<0x140>(v);  // row_mirror
+  if (L == 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
   return v;
 }
 // the lane's four pairs turned by the angles of cs = (cos, sin) x 4; sgn = -1 turns back
-__device__ __forceinline__ void turn(float (&x)[8], const float (&cs)[8], bool inter, float sgn) {
+template <bool INTER>
+__device__ __forceinline__ void turn(float (&x)[8], const float (&cs)[8], float sgn) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float c = cs[2 * i], s = sgn * cs[2 * i + 1];
-    const float a = inter ? x[2 * i] : x[i], b = inter ? x[2 * i + 1] : x[4 + i];
+    float& a = x[INTER ? 2 * i : i];
+    float& b = x[INTER ? 2 * i + 1 : 4 + i];
     const float p = fmaf(a, c, -(b * s)), q = fmaf(a, s, b * c);
-    if (inter) {
-      x[2 * i] = p;
-      x[2 * i + 1] = q;
-    } else {
-      x[i] = p;
-      x[4 + i] = q;
-    }
+    a = p;
+    b = q;
   }
 }
 
@@ -75,10 +79,10 @@ __device__ __forceinline__ void turn(float (&x)[8], const float (&cs)[8], bool i
 struct Lane {
   int a, b;
   bool on, rot;
-  __device__ __forceinline__ Lane(const HeadNormArgs& p, int j) {
+  __device__ __forceinline__ Lane(const HeadNormArgs& p, int j, bool inter) {
     on = 8 * j < p.d;
     rot = 8 * j < p.rot;
-    const bool half = rot && !p.inter;
+    const bool half = rot && !inter;
     a = half ? 4 * j : 8 * j;
     b = half ? p.rot / 2 + 4 * j : 8 * j + 4;
   }
@@ -100,122 +104,150 @@ __device__ __forceinline__ void load_cs(float (&cs)[8], const HeadNormArgs& p, c
 
 }  // namespace
 
-template <typename T, int L>
+// a group of lanes' share of the work: up to hc heads of one token, all of them query heads (w = 0) or key heads (w = 1)
+struct Item {
+  int64_t m;
+  int w, h0, n;
+  __device__ __forceinline__ Item(const HeadNormArgs& p, int64_t item) {
+    const int cq = (p.H[0] + p.hc - 1) / p.hc, ck = (p.H[1] + p.hc - 1) / p.hc;
+    m = item / (cq + ck);
+    int c = (int)(item - m * (cq + ck));
+    w = c >= cq;
+    if (w) c -= cq;
+    h0 = c * p.hc;
+    n = min(p.hc, (w ? p.H[1] : p.H[0]) - h0);
+  }
+};
+
+template <typename T, int L, bool INTER>
 __global__ __launch_bounds__(256) void head_norm_kernel(const HeadNormArgs p) {
-  const int j = threadIdx.x % L;
-  const int heads = p.H[0] + p.H[1], chunks = (heads + p.hc - 1) / p.hc;
-  const int64_t item = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-  if (item >= p.M * chunks) return;
-  const int64_t m = item / chunks;
-  const int h0 = (int)(item - m * chunks) * p.hc, h1 = min(h0 + p.hc, heads);
-  const int64_t b = m / p.T;
-  const int t = (int)(m - b * p.T);
-  const Lane ln(p, j);
-  float cs[8];
-  load_cs(cs, p, ln, m, t, j);
   constexpr int U = 4;  // heads whose loads are in flight together
-  for (int h2 = h0; h2 < h1; h2 += U) {
-    float x[U][8];
+  const int j = threadIdx.x % L;
+  const int64_t item = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+  if (item >= p.items) return;
+  const Item it(p, item);
+  const int w = it.w;
+  const int64_t b = it.m / p.T;
+  const int t = (int)(it.m - b * p.T);
+  const Lane ln(p, j, INTER);
+  const char* src = (const char*)p.x[w] + 2 * (b * p.x_sb[w] + t * p.x_st[w] + it.h0 * p.x_sh[w]);
+  char* dst = (char*)p.y[w] + 2 * (b * p.y_sb[w] + t * p.y_st[w] + it.h0 * p.y_sh[w]);
+  const int64_t sh = p.x_sh[w] * 2, dh = p.y_sh[w] * 2;
+  u32x2 xa[U], xb[U];
+  auto load = [&](int h) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int hh = h2 + u, w = hh >= p.H[0], h = w ? hh - p.H[0] : hh;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
-      if (ln.on && hh < h1) load8<T>(x[u], (const char*)p.x[w] + 2 * (b * p.x_sb[w] + t * p.x_st[w] + h * p.x_sh[w]), ln.a, ln.b);
+      xa[u] = xb[u] = u32x2{0u, 0u};
+      if (ln.on && h + u < it.n) {
+        xa[u] = *(const u32x2*)(src + (h + u) * sh + 2 * ln.a);
+        xb[u] = *(const u32x2*)(src + (h + u) * sh + 2 * ln.b);
+      }
     }
+  };
+  load(0);
+  float cs[8], wt[8];
+  load_cs(cs, p, ln, it.m, t, j);
+  const float f0 = w ? 1.f : p.alpha;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) wt[i] = ln.on ? f0 * p.w[w][(i < 4 ? ln.a : ln.b) + (i & 3)] : 0.f;
+  for (int h = 0;;) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int hh = h2 + u, w = hh >= p.H[0], h = w ? hh - p.H[0] : hh;
+      float x[8];
+      widen<T>(x, xa[u], xb[u]);
       float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) ss = fmaf(x[u][i], x[u][i], ss);
-      ss = group_sum<L>(ss);
-      if (!ln.on || hh >= h1) continue;
-      const float rstd = __builtin_amdgcn_rsqf(fmaf(ss, p.inv_d, p.eps));
-      const f32x4 wa = *(const f32x4*)(p.w[w] + ln.a), wb = *(const f32x4*)(p.w[w] + ln.b);
-      const float f = w ? rstd : rstd * p.alpha;
+      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+      const float rstd = __builtin_amdgcn_rsqf(fmaf(group_sum<L>(ss), p.inv_d, p.eps));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[u][i] *= f * wa[i];
-        x[u][4 + i] *= f * wb[i];
-      }
-      if (ln.rot) turn(x[u], cs, p.inter, 1.f);
-      store8<T>((char*)p.y[w] + 2 * (b * p.y_sb[w] + t * p.y_st[w] + h * p.y_sh[w]), ln.a, ln.b, x[u]);
+      for (int i = 0; i < 8; ++i) x[i] = x[i] * rstd * wt[i];
+      if (ln.rot) turn<INTER>(x, cs, 1.f);
+      if (ln.on && h + u < it.n) store8<T>(dst + (h + u) * dh, ln.a, ln.b, x);
     }
+    h += U;
+    if (h >= it.n) break;
+    load(h);
   }
 }
 
-template <typename T, int L>
+template <typename T, int L, bool INTER>
 __global__ __launch_bounds__(256) void head_norm_bwd_kernel(const HeadNormArgs p) {
+  constexpr int U = 2;  // (4: 162 registers, three waves per SIMD, 87 us against 70 at 524 672 heads of 80)
   __shared__ float red[2][256 * 8];
   const int j = threadIdx.x % L, grp = threadIdx.x / L;
-  const int heads = p.H[0] + p.H[1], chunks = (heads + p.hc - 1) / p.hc;
-  const int64_t items = p.M * chunks;
-  const Lane ln(p, j);
-  float dw[2][8], wt[2][8];
+  const Lane ln(p, j, INTER);
+  float dw[2][8];
 #pragma unroll
   for (int w = 0; w < 2; ++w)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      dw[w][i] = 0.f;
-      wt[w][i] = ln.on && p.w[w] ? p.w[w][(i < 4 ? ln.a : ln.b) + (i & 3)] : 0.f;
-    }
-  for (int64_t item = (int64_t)blockIdx.x * (256 / L) + grp; item < items; item += (int64_t)gridDim.x * (256 / L)) {
-    const int64_t m = item / chunks;
-    const int h0 = (int)(item - m * chunks) * p.hc, h1 = min(h0 + p.hc, heads);
-    const int64_t b = m / p.T;
-    const int t = (int)(m - b * p.T);
-    float cs[8];
-    load_cs(cs, p, ln, m, t, j);
-    constexpr int U = 4;  // heads whose loads are in flight together
-    for (int h2 = h0; h2 < h1; h2 += U) {
-      u32x2 xa[U], xb[U], ga[U], gb[U];
+    for (int i = 0; i < 8; ++i) dw[w][i] = 0.f;
+  for (int64_t item = (int64_t)blockIdx.x * (256 / L) + grp; item < p.items; item += (int64_t)gridDim.x * (256 / L)) {
+    const Item it(p, item);
+    const int w = it.w;
+    const int64_t b = it.m / p.T;
+    const int t = (int)(it.m - b * p.T);
+    const char* xr = (const char*)p.x[w] + 2 * (b * p.x_sb[w] + t * p.x_st[w] + it.h0 * p.x_sh[w]);
+    const char* gr = (const char*)p.dy[w] + 2 * (b * p.dy_sb[w] + t * p.dy_st[w] + it.h0 * p.dy_sh[w]);
+    char* yr = (char*)p.y[w] + 2 * (b * p.y_sb[w] + t * p.y_st[w] + it.h0 * p.y_sh[w]);
+    const int64_t xh = p.x_sh[w] * 2, gh = p.dy_sh[w] * 2, yh = p.y_sh[w] * 2;
+    u32x2 xa[U], xb[U], ga[U], gb[U];
+    auto load = [&](int h) {
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int hh = h2 + k, w = hh >= p.H[0], h = w ? hh - p.H[0] : hh;
-        xa[k] = xb[k] = ga[k] = gb[k] = u32x2{0u, 0u};
-        if (ln.on && hh < h1) {
-          const char* xr = (const char*)p.x[w] + 2 * (b * p.x_sb[w] + t * p.x_st[w] + h * p.x_sh[w]);
-          const char* gr = (const char*)p.dy[w] + 2 * (b * p.dy_sb[w] + t * p.dy_st[w] + h * p.dy_sh[w]);
-          xa[k] = *(const u32x2*)(xr + 2 * ln.a);
-          xb[k] = *(const u32x2*)(xr + 2 * ln.b);
-          ga[k] = *(const u32x2*)(gr + 2 * ln.a);
-          gb[k] = *(const u32x2*)(gr + 2 * ln.b);
+      for (int u = 0; u < U; ++u) {
+        xa[u] = xb[u] = ga[u] = gb[u] = u32x2{0u, 0u};
+        if (ln.on && h + u < it.n) {
+          xa[u] = *(const u32x2*)(xr + (h + u) * xh + 2 * ln.a);
+          xb[u] = *(const u32x2*)(xr + (h + u) * xh + 2 * ln.b);
+          ga[u] = *(const u32x2*)(gr + (h + u) * gh + 2 * ln.a);
+          gb[u] = *(const u32x2*)(gr + (h + u) * gh + 2 * ln.b);
         }
       }
+    };
+    load(0);
+    float cs[8], wt[8], acc[8];
+    load_cs(cs, p, ln, it.m, t, j);
+    const float al = w ? 1.f : p.alpha;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      wt[i] = ln.on ? al * p.w[w][(i < 4 ? ln.a : ln.b) + (i & 3)] : 0.f;
+      acc[i] = 0.f;
+    }
+    for (int h = 0;;) {
 #pragma unroll
       for (int k = 0; k < U; ++k) {
-        const int hh = h2 + k, w = hh >= p.H[0], h = w ? hh - p.H[0] : hh;
         float x[8], u[8];
         widen<T>(x, xa[k], xb[k]);
         widen<T>(u, ga[k], gb[k]);
-        if (ln.rot) turn(u, cs, p.inter, -1.f);
-        float ss = 0.f, dot = 0.f;
-        const float al = w ? 1.f : p.alpha;
+        if (ln.rot) turn<INTER>(u, cs, -1.f);
+        float ss = 0.f, dot = 0.f, g[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           ss = fmaf(x[i], x[i], ss);
-          u[i] *= al;
-          dot = fmaf(u[i] * (w ? wt[1][i] : wt[0][i]), x[i], dot);
+          g[i] = u[i] * x[i];
+          dot = fmaf(g[i], wt[i], dot);
         }
-        ss = group_sum<L>(ss);
-        dot = group_sum<L>(dot);
-        const float rstd = __builtin_amdgcn_rsqf(fmaf(ss, p.inv_d, p.eps));
-        const float c = dot * p.inv_d * rstd * rstd;  // mean(u w x^) rstd
-        const float f0 = w ? 0.f : rstd, f1 = w ? rstd : 0.f;
+        // (a head behind the last is zeros: it adds nothing, also with eps = 0)
+        const float rstd = h + k < it.n ? __builtin_amdgcn_rsqf(fmaf(group_sum<L>(ss), p.inv_d, p.eps)) : 0.f;
+        const float c = -group_sum<L>(dot) * p.inv_d * rstd * rstd * rstd;  // -mean(u w x^) rstd^2: meets x
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float g = u[i] * x[i];
-          dw[0][i] = fmaf(g, f0, dw[0][i]);
-          dw[1][i] = fmaf(g, f1, dw[1][i]);
-          x[i] = rstd * fmaf(u[i], w ? wt[1][i] : wt[0][i], -(x[i] * c));
+          acc[i] = fmaf(g[i], rstd, acc[i]);
+          x[i] = fmaf(u[i] * wt[i], rstd, x[i] * c);
         }
-        if (ln.on && hh < h1) store8<T>((char*)p.y[w] + 2 * (b * p.y_sb[w] + t * p.y_st[w] + h * p.y_sh[w]), ln.a, ln.b, x);
+        if (ln.on && h + k < it.n) store8<T>(yr + (h + k) * yh, ln.a, ln.b, x);
       }
+      h += U;
+      if (h >= it.n) break;
+      load(h);
+    }
+    const float aq = w ? 0.f : al, ak = w ? 1.f : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      dw[0][i] = fmaf(acc[i], aq, dw[0][i]);
+      dw[1][i] = fmaf(acc[i], ak, dw[1][i]);
     }
   }
   // ---- the workgroup's part of dw: groups added in their order --------------------------------------------------------------
-  if (p.part == nullptr) return;
 #pragma unroll
   for (int w = 0; w < 2; ++w)
 #pragma unroll
@@ -261,6 +293,7 @@ int fill(const char* what, const anip_qk_norm_params* p, bool backward, HeadNorm
   ANIP_REQUIRE(p->dtype == 0 || p->dtype == 1, "%s: dtype must be 0 (fp16) or 1 (bf16)", what);
   ANIP_REQUIRE(p->B >= 1 && p->T >= 1 && p->Hq >= 1 && p->Hkv >= 0, "%s: B, T, Hq >= 1 and Hkv >= 0 are wanted", what);
   ANIP_REQUIRE(p->d >= 8 && p->d <= 256 && p->d % 8 == 0, "%s: head width %d: a multiple of 8 up to 256 is wanted", what, p->d);
+  ANIP_REQUIRE(p->eps >= 0.f && p->eps < 1e30f, "%s: eps must not be negative", what);
   ANIP_REQUIRE(p->rot >= 0 && p->rot <= p->d && p->rot % 8 == 0, "%s: rot %d: a multiple of 8 up to the head width is wanted", what, p->rot);
   ANIP_REQUIRE(p->rot == 0 || (p->rope != nullptr && p->rope_rows >= 1 && ((uintptr_t)p->rope & 15) == 0), "%s: the rotation needs its table, 16-byte aligned", what);
   ANIP_REQUIRE(p->rot == 0 || p->positions != nullptr || p->rope_rows >= p->T, "%s: the rotation table has %d rows for %d tokens", what, p->rope_rows, p->T);
@@ -301,44 +334,43 @@ int fill(const char* what, const anip_qk_norm_params* p, bool backward, HeadNorm
 }
 
 int lanes_of(int d) { return d <= 32 ? 4 : d <= 64 ? 8 : d <= 128 ? 16 : 32; }
-// heads per group of lanes: as many as leave 4 waves for every SIMD, 8 at most
-int heads_per_group(int64_t M, int heads, int L) {
+int64_t items_of(int64_t M, int Hq, int Hkv, int hc) { return M * ((Hq + hc - 1) / hc + (Hkv + hc - 1) / hc); }
+// heads per group of lanes: as many, up to 8, as leave 4 waves for every SIMD
+int heads_per_group(int64_t M, int Hq, int Hkv, int L) {
   for (int hc = 8; hc > 1; hc /= 2)
-    if (M * ((heads + hc - 1) / hc) * L / 64 >= 4096) return hc;
+    if (items_of(M, Hq, Hkv, hc) * L / 64 >= 4096) return hc;
   return 1;
 }
+int bwd_blocks(int64_t items, int L) {
+  const int64_t want = cdiv64(items, 256 / L);
+  return (int)(want < 1024 ? want : 1024);
+}
 
-template <typename T>
+template <typename T, bool INTER>
 int run_fwd(const HeadNormArgs& a, int L, hipStream_t s) {
-  const int64_t items = a.M * ((a.H[0] + a.H[1] + a.hc - 1) / a.hc);
-  const dim3 grid((unsigned)cdiv64(items, 256 / L));
+  const dim3 grid((unsigned)cdiv64(a.items, 256 / L));
   switch (L) {
-    case 4: hipLaunchKernelGGL((head_norm_kernel<T, 4>), grid, dim3(256), 0, s, a); break;
-    case 8: hipLaunchKernelGGL((head_norm_kernel<T, 8>), grid, dim3(256), 0, s, a); break;
-    case 16: hipLaunchKernelGGL((head_norm_kernel<T, 16>), grid, dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL((head_norm_kernel<T, 32>), grid, dim3(256), 0, s, a);
+    case 4: hipLaunchKernelGGL((head_norm_kernel<T, 4, INTER>), grid, dim3(256), 0, s, a); break;
+    case 8: hipLaunchKernelGGL((head_norm_kernel<T, 8, INTER>), grid, dim3(256), 0, s, a); break;
+    case 16: hipLaunchKernelGGL((head_norm_kernel<T, 16, INTER>), grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL((head_norm_kernel<T, 32, INTER>), grid, dim3(256), 0, s, a);
   }
   ANIP_LAUNCH_CHECK("head_norm_kernel");
   return 0;
 }
-template <typename T>
+template <typename T, bool INTER>
 int run_bwd(const HeadNormArgs& a, int L, hipStream_t s) {
   const dim3 grid((unsigned)a.nblk);
   switch (L) {
-    case 4: hipLaunchKernelGGL((head_norm_bwd_kernel<T, 4>), grid, dim3(256), 0, s, a); break;
-    case 8: hipLaunchKernelGGL((head_norm_bwd_kernel<T, 8>), grid, dim3(256), 0, s, a); break;
-    case 16: hipLaunchKernelGGL((head_norm_bwd_kernel<T, 16>), grid, dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL((head_norm_bwd_kernel<T, 32>), grid, dim3(256), 0, s, a);
+    case 4: hipLaunchKernelGGL((head_norm_bwd_kernel<T, 4, INTER>), grid, dim3(256), 0, s, a); break;
+    case 8: hipLaunchKernelGGL((head_norm_bwd_kernel<T, 8, INTER>), grid, dim3(256), 0, s, a); break;
+    case 16: hipLaunchKernelGGL((head_norm_bwd_kernel<T, 16, INTER>), grid, dim3(256), 0, s, a); break;
+    default: hipLaunchKernelGGL((head_norm_bwd_kernel<T, 32, INTER>), grid, dim3(256), 0, s, a);
   }
   ANIP_LAUNCH_CHECK("head_norm_bwd_kernel");
   hipLaunchKernelGGL(head_norm_dw_kernel, dim3((unsigned)((2 * a.d + 63) / 64)), dim3(1024), 0, s, a);
   ANIP_LAUNCH_CHECK("head_norm_dw_kernel");
   return 0;
-}
-
-int bwd_blocks(int64_t M, int heads, int hc, int L) {
-  const int64_t want = cdiv64(M * ((heads + hc - 1) / hc), 256 / L);
-  return (int)(want < 1024 ? want : 1024);
 }
 
 }  // namespace
@@ -348,15 +380,18 @@ extern "C" int anip_qk_norm_rope(const anip_qk_norm_params* p, void* stream) {
   const int rc = fill("anip_qk_norm_rope", p, false, a);
   if (rc) return rc;
   const int L = lanes_of(a.d);
-  a.hc = heads_per_group(a.M, a.H[0] + a.H[1], L);
+  a.hc = heads_per_group(a.M, a.H[0], a.H[1], L);
+  a.items = items_of(a.M, a.H[0], a.H[1], a.hc);
+  hipStream_t s = (hipStream_t)stream;
   AnipProfScope prof_(ANIP_K_QK_NORM, stream);
-  return p->dtype ? run_fwd<bf16_t>(a, L, (hipStream_t)stream) : run_fwd<f16>(a, L, (hipStream_t)stream);
+  if (p->dtype) return a.inter ? run_fwd<bf16_t, true>(a, L, s) : run_fwd<bf16_t, false>(a, L, s);
+  return a.inter ? run_fwd<f16, true>(a, L, s) : run_fwd<f16, false>(a, L, s);
 }
 
-extern "C" int64_t anip_qk_norm_rope_backward_ws_floats(int64_t M, int heads, int d) {
-  if (M < 1 || heads < 1 || d < 8 || d > 256) return 0;
+extern "C" int64_t anip_qk_norm_rope_backward_ws_floats(int64_t M, int Hq, int Hkv, int d) {
+  if (M < 1 || Hq < 1 || Hkv < 0 || d < 8 || d > 256) return 0;
   const int L = lanes_of(d);
-  return (int64_t)bwd_blocks(M, heads, heads_per_group(M, heads, L), L) * 2 * d;
+  return (int64_t)bwd_blocks(items_of(M, Hq, Hkv, heads_per_group(M, Hq, Hkv, L)), L) * 2 * d;
 }
 
 extern "C" int anip_qk_norm_rope_backward(const anip_qk_norm_params* p, void* stream) {
@@ -364,13 +399,16 @@ extern "C" int anip_qk_norm_rope_backward(const anip_qk_norm_params* p, void* st
   const int rc = fill("anip_qk_norm_rope_backward", p, true, a);
   if (rc) return rc;
   ANIP_REQUIRE(p->ws != nullptr && p->dq_weight != nullptr && (p->Hkv == 0 || p->dk_weight != nullptr), "anip_qk_norm_rope_backward: ws and the weights' gradients are wanted");
-  const int L = lanes_of(a.d), heads = a.H[0] + a.H[1];
-  a.hc = heads_per_group(a.M, heads, L);
-  a.nblk = bwd_blocks(a.M, heads, a.hc, L);
+  const int L = lanes_of(a.d);
+  a.hc = heads_per_group(a.M, a.H[0], a.H[1], L);
+  a.items = items_of(a.M, a.H[0], a.H[1], a.hc);
+  a.nblk = bwd_blocks(a.items, L);
   ANIP_REQUIRE(p->ws_floats >= (int64_t)a.nblk * 2 * a.d, "anip_qk_norm_rope_backward: ws holds %lld floats, %lld are wanted", (long long)p->ws_floats, (long long)a.nblk * 2 * a.d);
   a.part = p->ws;
   a.dw[0] = p->dq_weight;
   a.dw[1] = p->Hkv ? p->dk_weight : nullptr;
+  hipStream_t s = (hipStream_t)stream;
   AnipProfScope prof_(ANIP_K_QK_NORM, stream);
-  return p->dtype ? run_bwd<bf16_t>(a, L, (hipStream_t)stream) : run_bwd<f16>(a, L, (hipStream_t)stream);
+  if (p->dtype) return a.inter ? run_bwd<bf16_t, true>(a, L, s) : run_bwd<bf16_t, false>(a, L, s);
+  return a.inter ? run_bwd<f16, true>(a, L, s) : run_bwd<f16, false>(a, L, s);
 }

@@ -106,10 +106,11 @@ int waves_for(int T) { return T <= 64 ? 1 : 4; }
 // the keys' kernel walks over the queries of all heads that share a key head; where the keys alone make fewer workgroups than the
 // chip holds at once (one of 4 wave groups per CU), the walk is split towards two rounds of them, each with 8 tiles at the least
 int dkv_splits(const anip_attn_params* p, int nwk) {
-  const int64_t blocks = (int64_t)((p->Tk + 32 * nwk - 1) / (32 * nwk)) * p->B * p->Hkv * nwk / 4 + 1;
+  const int64_t blocks = (int64_t)((p->Tk + 32 * nwk - 1) / (32 * nwk)) * p->B * p->Hkv * nwk / 4;
   const int64_t tiles = (int64_t)((p->Tq + 63) / 64) * (p->H / p->Hkv);
-  if (blocks * 2 > 512) return 1;
-  int64_t s = 512 / blocks;
+  if (blocks < 1) return 1;
+  if (blocks > 192) return 1;
+  int64_t s = (512 + blocks - 1) / blocks;
   s = s < tiles / 8 ? s : tiles / 8;
   return (int)(s < 1 ? 1 : (s > 16 ? 16 : s));
 }

@@ -12,14 +12,21 @@ namespace {
 
 constexpr float THR = 8.0f;  // the running maximum is raised when a score exceeds it by more: P <= 2^8
 
-// one map's running softmax over the 32 scores-per-lane-pair of a sub-tile: scores s (x = mul s + add in base 2) -> P fragments
-template <typename T, int NT>
-__device__ __forceinline__ void soft_step(f32x16& s, float mul, float add, float& m, float& l, f32x16 (&o)[NT], u32x4 (&p)[2]) {
-  float mx = fmaxf(fmaxf(s[0], s[1]), s[2]);
+// a running softmax over NS x 32 keys: scores s (x = mul s + add in base 2) -> P fragments
+template <typename T, int NT, int NS>
+__device__ __forceinline__ void soft_step(f32x16 (&s)[NS], float mul, float add, float& m, float& l, f32x16 (&o)[NT], u32x4 (&p)[NS][2]) {
+  float mx = fmaxf(fmaxf(s[0][0], s[0][1]), s[0][2]);
 #pragma unroll
-  for (int r = 3; r < 15; r += 2) mx = fmaxf(fmaxf(mx, s[r]), s[r + 1]);
-  mx = xor32_max(fmaxf(mx, s[15]));
-  mx = fmaf(mx, mul, add);
+  for (int r = 3; r < 15; r += 2) mx = fmaxf(fmaxf(mx, s[0][r]), s[0][r + 1]);
+  if (NS == 1) {
+    mx = fmaxf(mx, s[0][15]);
+  } else {
+    mx = fmaxf(fmaxf(mx, s[0][15]), s[NS - 1][0]);
+#pragma unroll
+    for (int r = 1; r < 15; r += 2) mx = fmaxf(fmaxf(mx, s[NS - 1][r]), s[NS - 1][r + 1]);
+    mx = fmaxf(mx, s[NS - 1][15]);
+  }
+  mx = fmaf(xor32_max(mx), mul, add);
   if (__any(mx - m > THR)) {  // always on the first seen key (m = -inf); never while both are -inf (NaN > THR is false)
     const float mn = fmaxf(m, mx);
     const float alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
@@ -31,22 +38,25 @@ __device__ __forceinline__ void soft_step(f32x16& s, float mul, float add, float
       for (int r = 0; r < 16; ++r) o[nt][r] *= alpha;
   }
   const float c = add - (m == -INFINITY ? 0.f : m);
-  float t = 0.f;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, c));
-    t += s[r];
+  for (int i = 0; i < NS; ++i) {
+    float t = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], mul, c));
+      t += s[i][r];
+    }
+    l += t;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[i][kb][j] = Num<T>::pack(s[i][8 * kb + 2 * j], s[i][8 * kb + 2 * j + 1]);
   }
-  l += t;
-#pragma unroll
-  for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p[kb][i] = Num<T>::pack(s[8 * kb + 2 * i], s[8 * kb + 2 * i + 1]);
 }
 
 }  // namespace
 
-template <typename T, int MAPS, int KS, int NT, int KT>
+template <typename T, int MAPS, int KS, int NT, int KT, int NS>
 __global__ __launch_bounds__(256 * MAPS, 2) void mapattn_fwd_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
   constexpr int NW = 4 * MAPS, BQ = 128;
@@ -123,33 +133,41 @@ __global__ __launch_bounds__(256 * MAPS, 2) void mapattn_fwd_kernel(const MapAtt
     const int kt0 = t * KT;
     if (a.causal && kt0 > pw + 31) continue;  // nothing of this tile is seen by this wave
 #pragma unroll
-    for (int sub = 0; sub < KT / 32; ++sub) {
+    for (int sub = 0; sub < KT / 32; sub += NS) {
       const int k0 = kt0 + 32 * sub;
-      f32x16 s = zero16();
+      f32x16 s[NS];
 #pragma unroll
-      for (int kk = 0; kk < KS; ++kk) s = Num<T>::mfma(kr.get(st + m * K_BYTES, sub, kk), qf[kk], s);
+      for (int i = 0; i < NS; ++i) s[i] = zero16();
+#pragma unroll
+      for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+        for (int i = 0; i < NS; ++i) s[i] = Num<T>::mfma(kr.get(st + m * K_BYTES, sub + i, kk), qf[kk], s[i]);
       float mul = a.scale_log2, add = 0.f;
       if (BIAS) {
-        if (k0 + 31 - pw <= -a.R) add = far_lo;
+        if (k0 + 32 * NS - 1 - pw <= -a.R) add = far_lo;
         else if (k0 - (pw + 31) >= a.R) add = far_hi;
         else {
           const float* nb = near + (k0 + 4 * h - (pw + ql) + a.R + E);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mul, nb[acc_row(r)]);
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], mul, nb[32 * i + acc_row(r)]);
           mul = 1.f;
         }
       }
-      if (k0 + 31 >= len || (a.causal && k0 + 31 > pw)) {
+      if (k0 + 32 * NS - 1 >= len || (a.causal && k0 + 32 * NS - 1 > pw)) {
         const int dl = lim - k0 - 4 * h;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = acc_row(r) > dl ? -INFINITY : s[r];
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + acc_row(r) > dl ? -INFINITY : s[i][r];
       }
-      u32x4 p[2];
-      soft_step<T, NT>(s, mul, add, mrun, lrun, o, p);
+      u32x4 p[NS][2];
+      soft_step<T, NT, NS>(s, mul, add, mrun, lrun, o, p);
 #pragma unroll
-      for (int kb2 = 0; kb2 < 2; ++kb2)
+      for (int kb2 = 0; kb2 < 2 * NS; ++kb2)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) o[nt] = Num<T>::mfma(vr.get(st + MAPS * K_BYTES, 2 * sub + kb2, nt), p[kb2], o[nt]);
+        for (int nt = 0; nt < NT; ++nt) o[nt] = Num<T>::mfma(vr.get(st + MAPS * K_BYTES, 2 * sub + kb2, nt), p[kb2 >> 1][kb2 & 1], o[nt]);
     }
   }
 
@@ -306,25 +324,25 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
       if (t >= t1) continue;
     }
     const char* tile = mem + (it & 1) * STAGE;
-    f32x16 s = zero16();
+    f32x16 s[1] = {zero16()};
 #pragma unroll
-    for (int kk = 0; kk < KS; ++kk) s = Num<T>::mfma(kr.get(tile + m * K_BYTES, 0, kk), qf[kk], s);
+    for (int kk = 0; kk < KS; ++kk) s[0] = Num<T>::mfma(kr.get(tile + m * K_BYTES, 0, kk), qf[kk], s[0]);
     if (BIAS && close) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mul, bias[r]);
+      for (int r = 0; r < 16; ++r) s[0][r] = fmaf(s[0][r], mul, bias[r]);
       mul = 1.f;
     }
     if (k0 + 31 >= len || (a.causal && k0 + 31 > start)) {
       const int dl = lim - k0 - 4 * h;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = acc_row(r) > dl ? -INFINITY : s[r];
+      for (int r = 0; r < 16; ++r) s[0][r] = acc_row(r) > dl ? -INFINITY : s[0][r];
     }
-    u32x4 p[2];
-    soft_step<T, NT>(s, mul, add, mrun, lrun, o, p);
+    u32x4 p[1][2];
+    soft_step<T, NT, 1>(s, mul, add, mrun, lrun, o, p);
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) o[nt] = Num<T>::mfma(vr.get(tile + MAPS * K_BYTES, kb2, nt), p[kb2], o[nt]);
+      for (int nt = 0; nt < NT; ++nt) o[nt] = Num<T>::mfma(vr.get(tile + MAPS * K_BYTES, kb2, nt), p[0][kb2], o[nt]);
     // (MAPS = 1) the stage just read is written by the DMA issued in the next turn: its reads have returned before that
     if (MAPS == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   }
@@ -424,18 +442,39 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
 }
 
 // ---- joins the parts of a split forward: o = sum_s 2^(l_s - l) o_s, l = log2 sum_s 2^l_s -----------------------------------------
-// One wave per row: lane s holds the weight of parts s, s + 64, ..; 64 / LR parts are added at once by LR lanes of 4 channels each.
-template <typename T, int MAPS, int LR>
+// Few parts: LR lanes of 4 channels per row.  Many: a wave per row; lane s holds the weight of parts s, s + 64, ..; 64 / LR parts are added at once by LR lanes of 4 channels each.
+template <typename T, int MAPS, int LR, bool FEW>
 __global__ __launch_bounds__(256) void mapattn_combine_kernel(const MapAttnArgs a) {
   constexpr int PG = 64 / LR, MW = 4;  // parts at once; weights of a lane (256 parts at most)
   const int64_t rows = (int64_t)a.B * a.Tq * a.H;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, c0 = (lane % LR) * 4, sg = FEW ? 0 : lane / LR;
+  const int64_t row = FEW ? (int64_t)blockIdx.x * (4 * PG) + threadIdx.x / LR : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= rows) return;
-  const int lane = threadIdx.x & 63, c0 = (lane % LR) * 4, sg = lane / LR;
   float x[MAPS][4], lse2[MAPS];
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
     float lw[MW], mx = -INFINITY;
+    if (FEW) {
+      for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, a.part_l[((int64_t)s * rows + row) * MAPS + m]);
+      const float base = mx == -INFINITY ? 0.f : mx;
+      float sum = 0.f;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+      for (int s = 0; s < a.splits; ++s) {
+        const int64_t at = ((int64_t)s * rows + row) * MAPS + m;
+        const float w = __builtin_amdgcn_exp2f(a.part_l[at] - base);
+        sum += w;
+        f32x4 v = {0.f, 0.f, 0.f, 0.f};
+        if (c0 < a.dv) v = *(const f32x4*)(a.part_o + at * a.dv + c0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+      }
+      const bool none = mx == -INFINITY;
+      lse2[m] = none ? -INFINITY : base + __builtin_amdgcn_logf(sum);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[m][e] = none ? 0.f : acc[e] / sum;
+      continue;
+    }
 #pragma unroll
     for (int i = 0; i < MW; ++i) {
       const int s = lane + 64 * i;
@@ -459,14 +498,20 @@ __global__ __launch_bounds__(256) void mapattn_combine_kernel(const MapAttnArgs 
     for (int i = 0; i < MW; ++i) {
       if (64 * i >= a.splits) break;
       const int n = min(64, a.splits - 64 * i);
-#pragma unroll 4
-      for (int s0 = 0; s0 < n; s0 += PG) {
-        const int s = s0 + sg;  // (a part behind the last weighs nothing)
-        const float w = __shfl(lw[i], s & 63, 64);
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (s < n && c0 < a.dv) v = *(const f32x4*)(a.part_o + (((int64_t)(s + 64 * i) * rows + row) * MAPS + m) * a.dv + c0);
+      for (int s0 = 0; s0 < n; s0 += 4 * PG) {
+        f32x4 v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[e], acc[e]);
+        for (int k = 0; k < 4; ++k) {
+          const int s = s0 + k * PG + sg;
+          v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (s < n && c0 < a.dv) v[k] = *(const f32x4*)(a.part_o + (((int64_t)(s + 64 * i) * rows + row) * MAPS + m) * a.dv + c0);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float w = __shfl(lw[i], (s0 + k * PG + sg) & 63, 64);  // (a part behind the last is zeros)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[k][e], acc[e]);
+        }
       }
     }
 #pragma unroll
@@ -479,7 +524,7 @@ __global__ __launch_bounds__(256) void mapattn_combine_kernel(const MapAttnArgs 
   }
   const int head = (int)(row % a.H);
   const int64_t bt = row / a.H;
-  if (a.lse && lane == 0) {
+  if (a.lse && sg == 0 && c0 == 0) {
     const int64_t b = bt / a.Tq, qi = bt - b * a.Tq;
 #pragma unroll
     for (int m = 0; m < MAPS; ++m) a.lse[((b * a.H + head) * MAPS + m) * a.Tq + qi] = lse2[m] * LN2;
@@ -499,17 +544,17 @@ namespace {
 
 template <typename T, int MAPS, int KS, int NT>
 int run_fwd(const MapAttnArgs& a, hipStream_t s) {
-  constexpr int KT = 64;
+  constexpr int KT = 64, NS = MAPS * NT >= 16 ? 1 : 2;
   constexpr int KCH = 4 * ((KS + 1) / 2), VCH = 4 * NT;
   constexpr int tiles = 2 * KT * 16 * (MAPS * KCH + VCH), hand = MAPS == 2 ? 4 * NT * 16 * 64 * 4 : 0;
   const int lds = (tiles > hand ? tiles : hand) + (MAPS == 1 ? (2 * (a.R + 128 + KT) + 1) * 4 : 0);
-  const void* f = (const void*)mapattn_fwd_kernel<T, MAPS, KS, NT, KT>;
+  const void* f = (const void*)mapattn_fwd_kernel<T, MAPS, KS, NT, KT, NS>;
   if (anip_raise_lds_limit(f, lds) != 0) {
     anip_set_error("mapattn forward: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
   const int nqb = (a.Tq + 127) / 128;
-  hipLaunchKernelGGL((mapattn_fwd_kernel<T, MAPS, KS, NT, KT>), dim3((unsigned)(nqb * a.splits * a.B * a.H)), dim3(256 * MAPS), lds, s, a);
+  hipLaunchKernelGGL((mapattn_fwd_kernel<T, MAPS, KS, NT, KT, NS>), dim3((unsigned)(nqb * a.splits * a.B * a.H)), dim3(256 * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_fwd_kernel");
   return 0;
 }
@@ -537,14 +582,18 @@ int run_token(const MapAttnArgs& a0, hipStream_t s) {
   return 0;
 }
 
-template <typename T, int MAPS>
-int run_combine(const MapAttnArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)cdiv64((int64_t)a.B * a.Tq * a.H, 4));
-  if (a.dv <= 64) hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, 16>), grid, dim3(256), 0, s, a);
-  else if (a.dv <= 128) hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, 32>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, 64>), grid, dim3(256), 0, s, a);
+template <typename T, int MAPS, int LR>
+int run_combine_lr(const MapAttnArgs& a, hipStream_t s) {
+  // (one part after the other up to 8: 8 us against 13 at 29 688 rows x 2; 64 / LR at once beyond: 9 against 17 at 128 rows x 16)
+  const int64_t rows = (int64_t)a.B * a.Tq * a.H;
+  if (a.splits <= 8) hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, true>), dim3((unsigned)cdiv64(rows, 256 / LR)), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, false>), dim3((unsigned)cdiv64(rows, 4)), dim3(256), 0, s, a);
   ANIP_LAUNCH_CHECK("mapattn_combine_kernel");
   return 0;
+}
+template <typename T, int MAPS>
+int run_combine(const MapAttnArgs& a, hipStream_t s) {
+  return a.dv <= 64 ? run_combine_lr<T, MAPS, 16>(a, s) : a.dv <= 128 ? run_combine_lr<T, MAPS, 32>(a, s) : run_combine_lr<T, MAPS, 64>(a, s);
 }
 
 #define TRY1(KS, NT) if (ks <= KS) return run<T, 1, KS, NT>(a, s);

@@ -769,7 +769,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, rope=None, p
     _, B, T, Hq, Hkv, d = head[:6]
     _work(K_QK_NORM, n * 6, f"B{B} T{T} h{Hq}+{Hkv} d{d} bwd")
     with _on_device_of(q) as stream:
-        ws = torch.empty((lib.anip_qk_norm_rope_backward_ws_floats(B * T, Hq + Hkv, d),), dtype=F32, device=q.device)
+        ws = torch.empty((lib.anip_qk_norm_rope_backward_ws_floats(B * T, Hq, Hkv, d),), dtype=F32, device=q.device)
         p = L.QkNormParams(*head, *_heads4(dq, "dq"), *(_NOWHERE if k is None else _heads4(dk, "dk")), *gq, *gk, dwq.data_ptr(),
                            _p(dwk), ws.data_ptr(), ws.numel())
         L.check(lib.anip_qk_norm_rope_backward(C.byref(p), stream), "anip_qk_norm_rope_backward")

@@ -230,7 +230,7 @@ int anip_temporal_qkv_attention(const void* x, const float* gamma, const float* 
  *   (cos, sin) is rope[pos][i] (fp32 [rope_rows][rot / 2][2]); pos = positions[b][t], or t where positions is NULL; positions
  *   outside the table are clamped to it.  An output may be its input (in place), else they must not overlap.
  * anip_qk_norm_rope_backward — q_out / k_out receive dq / dk from dq_out / dk_out and the forward's inputs; dq_weight / dk_weight
- *   (fp32 [d]) are written.  ws: anip_qk_norm_rope_backward_ws_floats(B * T, Hq + Hkv, d) floats. */
+ *   (fp32 [d]) are written.  ws: anip_qk_norm_rope_backward_ws_floats(B * T, Hq, Hkv, d) floats. */
 typedef struct anip_qk_norm_params {
   int dtype;
   int B, T, Hq, Hkv, d, rot, interleaved;
@@ -247,7 +247,7 @@ typedef struct anip_qk_norm_params {
   float* ws; int64_t ws_floats;
 } anip_qk_norm_params;
 int anip_qk_norm_rope(const anip_qk_norm_params* p, void* stream);
-int64_t anip_qk_norm_rope_backward_ws_floats(int64_t M, int heads, int d);
+int64_t anip_qk_norm_rope_backward_ws_floats(int64_t M, int Hq, int Hkv, int d);
 int anip_qk_norm_rope_backward(const anip_qk_norm_params* p, void* stream);
 
 /* anip_relative_attention — o_i = softmax_j(scale q_i.k_j + table[h][buckets[clamp(j - p_i, +-max_distance) + max_distance]]) v_j
