@@ -6,6 +6,7 @@ compute entry points need a gfx950 device.
 """
 import ctypes as C
 import os
+import struct
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # ANIP_LIB: an experiment build of the same ABI (aniportrait_amd/build.py --out=...); the product is the default path
@@ -69,6 +70,12 @@ class AttnParams(C.Structure):
     ]
 
 
+# the same two as formats: packing 50 values into bytes takes 1 us, filling a ctypes.Structure 10
+QK_NORM_PACK = struct.Struct("@8i2f" + "P3q" * 2 + "PPPiP" + "P3q" * 4 + "PPPq")
+ATTN_PACK = struct.Struct("@8if" + "P3q" * 3 + "PPPPiiP" + "PPP" + "P3q" + "PPPPP" + "Pq")
+assert QK_NORM_PACK.size == C.sizeof(QkNormParams) and ATTN_PACK.size == C.sizeof(AttnParams)
+
+
 # name -> (restype, argtypes); must list every symbol declared in include/aniportrait_hip.h
 SIGNATURES = {
     "anip_version": (c_int, []),
@@ -109,15 +116,15 @@ SIGNATURES = {
     "anip_temporal_qkv_attention_supported": (c_int, [c_int, c_int, c_int, c_int]),
     "anip_temporal_qkv_attention": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int,
                                             c_int, c_float, c_float, c_void_p]),
-    "anip_qk_norm_rope": (c_int, [C.POINTER(QkNormParams), c_void_p]),
+    "anip_qk_norm_rope": (c_int, [c_void_p, c_void_p]),
     "anip_qk_norm_rope_backward_ws_floats": (c_int64, [c_int64, c_int, c_int, c_int]),
-    "anip_qk_norm_rope_backward": (c_int, [C.POINTER(QkNormParams), c_void_p]),
-    "anip_relative_attention_ws_bytes": (c_int64, [C.POINTER(AttnParams), c_int]),
-    "anip_relative_attention": (c_int, [C.POINTER(AttnParams), c_void_p]),
-    "anip_relative_attention_backward": (c_int, [C.POINTER(AttnParams), c_void_p]),
-    "anip_differential_attention_ws_bytes": (c_int64, [C.POINTER(AttnParams), c_int]),
-    "anip_differential_attention": (c_int, [C.POINTER(AttnParams), c_void_p]),
-    "anip_differential_attention_backward": (c_int, [C.POINTER(AttnParams), c_void_p]),
+    "anip_qk_norm_rope_backward": (c_int, [c_void_p, c_void_p]),
+    "anip_relative_attention_ws_bytes": (c_int64, [c_void_p, c_int]),
+    "anip_relative_attention": (c_int, [c_void_p, c_void_p]),
+    "anip_relative_attention_backward": (c_int, [c_void_p, c_void_p]),
+    "anip_differential_attention_ws_bytes": (c_int64, [c_void_p, c_int]),
+    "anip_differential_attention": (c_int, [c_void_p, c_void_p]),
+    "anip_differential_attention_backward": (c_int, [c_void_p, c_void_p]),
     "anip_softmax_rows": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_void_p]),
     "anip_linear_small": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p]),
     "anip_add": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),

@@ -81,7 +81,7 @@ int forward(const char* what, const anip_attn_params* p, int maps, int kid, void
   a.splits = splits_of(p);
   const int64_t need = fwd_ws(p, maps);
   ANIP_REQUIRE(need == 0 || (p->workspace != nullptr && ((uintptr_t)p->workspace & 15) == 0 && p->workspace_bytes >= need), "%s: a workspace of %lld bytes is wanted, 16-byte aligned", what, (long long)need);
-  ANIP_REQUIRE((int64_t)((p->Tq + 127) / 128) * a.splits * p->B * p->H < (1ll << 31) && (int64_t)p->B * p->Tq * p->H * a.dv / 1024 < (1ll << 31), "%s: too many queries for one launch", what);
+  ANIP_REQUIRE((int64_t)((p->Tq + 63) / 64) * a.splits * p->B * p->H < (1ll << 31) && (int64_t)p->B * p->Tq * p->H * a.dv / 1024 < (1ll << 31), "%s: too many queries for one launch", what);
   if (a.splits > 1) {
     a.part_o = (float*)p->workspace;
     a.part_l = a.part_o + (int64_t)a.splits * p->B * p->Tq * p->H * maps * a.dv;
@@ -129,9 +129,9 @@ BwdLayout layout(const anip_attn_params* p, int maps) {
   if (maps == 1) {
     l.ND = 2 * p->max_distance + 128;
     const int64_t groups = (int64_t)p->B * l.QW;
-    l.parts = (int)(groups < 32 ? groups : 32);
+    l.parts = (int)(groups < 32 ? groups : 32);  // few query groups: their own sums are the parts
     l.diag = (int64_t)p->H * groups * (l.ND + 2);
-    l.part = (int64_t)p->H * l.parts * (l.ND + 2);
+    l.part = groups > 32 ? (int64_t)p->H * l.parts * (l.ND + 2) : 0;
   } else {
     l.dlam = (int64_t)p->H * p->B * l.QW;
   }
@@ -156,8 +156,8 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   a.rows_lse = a.part_o + l.dkv;
   a.rows_d = a.rows_lse + l.rows;
   a.diag = a.rows_d + l.rows;
-  a.diag_part = a.diag + l.diag;
-  a.dlam_part = a.diag_part + l.part;
+  a.diag_part = l.part ? a.diag + l.diag : a.diag;
+  a.dlam_part = a.diag + l.diag + l.part;
   hipStream_t s = (hipStream_t)stream;
   AnipProfScope prof_(kid, stream);
   int r = mapattn_dq(a, maps, p->dtype, l.nwq, s);

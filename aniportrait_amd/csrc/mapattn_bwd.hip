@@ -627,8 +627,10 @@ int mapattn_reduce(const MapAttnArgs& a, int maps, int bf16, hipStream_t s) {
     ANIP_LAUNCH_CHECK("mapattn_dlam_kernel");
     return 0;
   }
-  hipLaunchKernelGGL(mapattn_diag_kernel, dim3((unsigned)((a.ND + 2 + 255) / 256), (unsigned)a.parts, (unsigned)a.H), dim3(256), 0, s, a);
-  ANIP_LAUNCH_CHECK("mapattn_diag_kernel");
+  if (a.diag_part != a.diag) {
+    hipLaunchKernelGGL(mapattn_diag_kernel, dim3((unsigned)((a.ND + 2 + 255) / 256), (unsigned)a.parts, (unsigned)a.H), dim3(256), 0, s, a);
+    ANIP_LAUNCH_CHECK("mapattn_diag_kernel");
+  }
   const int lds = (a.ND + 2) * 4;
   if (bf16) hipLaunchKernelGGL((mapattn_dtable_kernel<bf16_t>), dim3((unsigned)a.H), dim3(1024), lds, s, a);
   else hipLaunchKernelGGL((mapattn_dtable_kernel<f16>), dim3((unsigned)a.H), dim3(1024), lds, s, a);

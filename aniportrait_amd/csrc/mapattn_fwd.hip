@@ -1,4 +1,4 @@
-// Forward of the attention of mapattn.h: 128 queries of one head per workgroup (4 waves x 32), tiles of KT keys in two LDS
+// Forward of the attention of mapattn.h: QG x 32 queries of one head per workgroup, a wave for each 32, tiles of KT keys in two LDS
 // stages, one pass over the keys with running maxima and sums (base 2).  S^T = K Q^T per 32 keys, so that a lane owns one query:
 // its maximum and sum are 16 register operations and one exchange between the half-waves, and P^T is the B operand of
 // O^T += V^T P^T as it lies.  Differential attention gives each of its two
@@ -56,10 +56,10 @@ __device__ __forceinline__ void soft_step(f32x16 (&s)[NS], float mul, float add,
 
 }  // namespace
 
-template <typename T, int MAPS, int KS, int NT, int KT, int NS>
-__global__ __launch_bounds__(256 * MAPS, 2) void mapattn_fwd_kernel(const MapAttnArgs a) {
+template <typename T, int MAPS, int KS, int NT, int KT, int NS, int QG>
+__global__ __launch_bounds__(64 * QG * MAPS, 2) void mapattn_fwd_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
-  constexpr int NW = 4 * MAPS, BQ = 128;
+  constexpr int NW = QG * MAPS, BQ = 32 * QG;
   constexpr int KCH = 4 * ((KS + 1) / 2), VCH = 4 * NT;
   constexpr int K_BYTES = KT * KCH * 16, V_BYTES = KT * VCH * 16, STAGE = MAPS * K_BYTES + V_BYTES;
   constexpr int E = BQ + KT;
@@ -542,19 +542,26 @@ __global__ __launch_bounds__(256) void mapattn_combine_kernel(const MapAttnArgs 
 // ---- dispatch -----------------------------------------------------------------------------------------------------------
 namespace {
 
+constexpr int fwd_groups(int maps, int nt) { return maps == 1 || nt >= 8 ? 4 : 2; }
+
 template <typename T, int MAPS, int KS, int NT>
 int run_fwd(const MapAttnArgs& a, hipStream_t s) {
-  constexpr int KT = 64, NS = MAPS * NT >= 16 ? 1 : 2;
+  // One map: 128 queries, 64 keys between two maxima (32: 102 us against 94 at 2 x 4096, 8 heads of 40; two waves per 32 queries
+  // on alternating keys, twice the waves, 93).  Two maps: small workgroups of 64 queries and tiles of 32 keys, three to a CU and
+  // each in its own phase (487 us against 527 - 583 with 128 queries or 64 keys at 8192 causal, 16 heads of 64 + 64); the widest
+  // heads' accumulators allow two waves per SIMD either way (237 us against 242 at 2 x 4096 causal, 8 heads of 128 + 128).
+  constexpr bool WIDE = NT >= 8;
+  constexpr int KT = (MAPS == 1 || WIDE) ? 64 : 32, NS = MAPS == 1 ? 2 : 1, QG = fwd_groups(MAPS, NT);
   constexpr int KCH = 4 * ((KS + 1) / 2), VCH = 4 * NT;
-  constexpr int tiles = 2 * KT * 16 * (MAPS * KCH + VCH), hand = MAPS == 2 ? 4 * NT * 16 * 64 * 4 : 0;
-  const int lds = (tiles > hand ? tiles : hand) + (MAPS == 1 ? (2 * (a.R + 128 + KT) + 1) * 4 : 0);
-  const void* f = (const void*)mapattn_fwd_kernel<T, MAPS, KS, NT, KT, NS>;
+  constexpr int tiles = 2 * KT * 16 * (MAPS * KCH + VCH), hand = MAPS == 2 ? QG * NT * 16 * 64 * 4 : 0;
+  const int lds = (tiles > hand ? tiles : hand) + (MAPS == 1 ? (2 * (a.R + 32 * QG + KT) + 1) * 4 : 0);
+  const void* f = (const void*)mapattn_fwd_kernel<T, MAPS, KS, NT, KT, NS, QG>;
   if (anip_raise_lds_limit(f, lds) != 0) {
     anip_set_error("mapattn forward: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
-  const int nqb = (a.Tq + 127) / 128;
-  hipLaunchKernelGGL((mapattn_fwd_kernel<T, MAPS, KS, NT, KT, NS>), dim3((unsigned)(nqb * a.splits * a.B * a.H)), dim3(256 * MAPS), lds, s, a);
+  const int nqb = (a.Tq + 32 * QG - 1) / (32 * QG);
+  hipLaunchKernelGGL((mapattn_fwd_kernel<T, MAPS, KS, NT, KT, NS, QG>), dim3((unsigned)(nqb * a.splits * a.B * a.H)), dim3(64 * QG * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_fwd_kernel");
   return 0;
 }

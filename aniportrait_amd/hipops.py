@@ -625,56 +625,49 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 
 
 def _heads4(t, name, like=None, shape=None):
-    """(device pointer, strides of batch / token / head) of a (batch, token, head, channel) tensor: contiguous channels, the
+    """(device pointer, strides of batch, token, head) of a (batch, token, head, channel) tensor: contiguous channels, the
     rest any strides that keep 16-byte rows"""
     if not t.is_cuda:
         raise L.HipLibraryError(f"{name}: expected a GPU tensor (the hot path has no CPU fallback)")
     if t.dtype not in _DTYPES:
         raise TypeError(f"{name}: expected fp16 or bf16, got {t.dtype}")
-    if t.dim() != 4:
-        raise ValueError(f"{name}: expected (batch, token, head, channel), got shape {tuple(t.shape)}")
+    sz = t.shape
+    if len(sz) != 4:
+        raise ValueError(f"{name}: expected (batch, token, head, channel), got shape {tuple(sz)}")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise TypeError(f"{name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
-    if shape is not None and tuple(t.shape) != shape:
-        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
-    st = t.stride()
-    sz = t.shape
-    if st[3] != 1 and sz[3] != 1:
+    if shape is not None and sz != shape:
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(sz)}")
+    p, (sb, st, sh, sc) = t.data_ptr(), t.stride()
+    if sc != 1 and sz[3] != 1:
         raise ValueError(f"{name}: channels must be contiguous")
-    st = tuple(st[i] if sz[i] != 1 else 0 for i in range(3))
-    if st[0] % 8 or st[1] % 8 or st[2] % 8 or t.data_ptr() % 16:
-        raise ValueError(f"{name}: strides must be multiples of 8 elements and the data 16-byte aligned, got strides "
-                         f"{t.stride()}")
-    return t.data_ptr(), st
+    if (sb | st | sh) & 7 or p & 15:
+        # (the stride of a dimension of one is never taken)
+        sb, st, sh = (0 if n == 1 else x for n, x in zip(sz, (sb, st, sh)))
+        if (sb | st | sh) & 7 or p & 15:
+            raise ValueError(f"{name}: strides must be multiples of 8 elements and the data 16-byte aligned, got strides "
+                             f"{t.stride()}")
+    return p, sb, st, sh
 
 
 def _aux(t, name, dtype, shape, like):
-    """device pointer of a contiguous helper tensor next to `like`; None stays NULL"""
+    """device pointer of a contiguous helper tensor next to `like`; None is NULL"""
     if t is None:
-        return None
+        return 0
     if t.dtype != dtype or t.device != like.device:
         raise TypeError(f"{name}: expected {dtype} on {like.device}, got {t.dtype} on {t.device}")
-    if tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous tensor of shape {shape}, got {tuple(t.shape)}")
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}")
     return t.data_ptr()
 
 
-class _on_device_of:
-    """the launch goes to the tensors' device and torch's current stream there"""
-
-    def __init__(self, t):
-        self.dev, self.ctx = t.device, None
-
-    def __enter__(self):
-        if self.dev.index != torch.cuda.current_device():
-            self.ctx = torch.cuda.device(self.dev)
-            self.ctx.__enter__()
-        return torch.cuda.current_stream(self.dev).cuda_stream
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
-        return False
+def _launch(t, call):
+    """call(stream) with t's device as the current one and torch's current stream there"""
+    index = t.device.index
+    if index == torch.cuda.current_device():
+        return call(torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return call(torch._C._cuda_getCurrentRawStream(index))
 
 
 def rope_table(n_positions, rot_dim, theta=10000.0, device="cuda"):
@@ -687,14 +680,15 @@ def rope_table(n_positions, rot_dim, theta=10000.0, device="cuda"):
     return torch.stack([ang.cos(), ang.sin()], -1).float()
 
 
-_NOWHERE = (None, (0, 0, 0))
+_NOWHERE = (0, 0, 0, 0)
 
 
-def _qk_norm_params(q, k, q_weight, k_weight, rope, positions, eps, interleaved, q_alpha):
+def _qk_norm_fields(q, k, q_weight, k_weight, rope, positions, eps, interleaved, q_alpha):
+    """the fields of anip_qk_norm_params up to positions"""
+    qp = _heads4(q, "q")
     B, T, Hq, d = q.shape
     if d % 8 or not 8 <= d <= 256:
         raise ValueError(f"qk_norm_rope: head width {d}: a multiple of 8 up to 256 is wanted")
-    qp = _heads4(q, "q")
     kp, Hkv = _NOWHERE, 0
     if k is not None:
         Hkv = k.shape[2] if k.dim() == 4 else 0
@@ -703,18 +697,21 @@ def _qk_norm_params(q, k, q_weight, k_weight, rope, positions, eps, interleaved,
         raise ValueError("k_weight without k")
     if q_weight is None or (k is not None and k_weight is None):
         raise ValueError("qk_norm_rope: the weights of the norms are wanted")
-    rot = rows = 0
+    eps = float(eps)
+    if not 0.0 <= eps < 1e30:
+        raise ValueError(f"qk_norm_rope: eps must not be negative, got {eps}")
+    rot = rows = rp = 0
     if rope is not None:
         if rope.dim() != 3 or rope.shape[2] != 2 or not 0 < 2 * rope.shape[1] <= d or rope.shape[1] % 4 or rope.shape[0] < 1:
             raise ValueError(f"rope: expected (positions, rot / 2, 2) with rot a multiple of 8 up to {d}, got {tuple(rope.shape)}")
         rows, rot = rope.shape[0], 2 * rope.shape[1]
         if positions is None and rows < T:
             raise ValueError(f"rope: {rows} positions for {T} tokens")
+        rp = _aux(rope, "rope", F32, rope.shape, q)
     elif positions is not None:
         raise ValueError("positions without rope")
-    return (_DTYPES[q.dtype], B, T, Hq, Hkv, d, rot, int(bool(interleaved)), float(eps), float(q_alpha), *qp, *kp,
-            _aux(q_weight, "q_weight", F32, (d,), q), _aux(k_weight, "k_weight", F32, (d,), q),
-            None if rope is None else _aux(rope, "rope", F32, tuple(rope.shape), q), rows,
+    return (_DTYPES[q.dtype], B, T, Hq, Hkv, d, rot, 1 if interleaved else 0, eps, float(q_alpha), *qp, *kp,
+            _aux(q_weight, "q_weight", F32, (d,), q), _aux(k_weight, "k_weight", F32, (d,), q), rp, rows,
             _aux(positions, "positions", torch.int32, (B, T), q))
 
 
@@ -724,27 +721,29 @@ def qk_norm_rope(q, k, q_weight, k_weight, rope=None, positions=None, eps=1e-6, 
 
     q (B, T, Hq, d), k (B, T, Hkv, d) or None, fp16 / bf16, e.g. slices of one fused projection; q_weight, k_weight (d,) fp32;
     rope from rope_table (None: no rotation; fewer channels than d: the first ones turn); positions (B, T) int32 (default: the
-    token's index); q_alpha: a factor on the queries (attn_q_alpha(d) for ref_attention(q_log2_scaled=True)).  interleaved:
-    channel pairs (2 i, 2 i + 1) instead of (i, i + rot / 2).  q_out / k_out: where the results go, e.g. a slice of a cache, or
-    the input itself.  Returns (q_out, k_out)."""
+    token's index; outside the table: its ends); q_alpha: a factor on the queries (attn_q_alpha(d) for
+    ref_attention(q_log2_scaled=True)).  interleaved: channel pairs (2 i, 2 i + 1) instead of (i, i + rot / 2).  q_out / k_out:
+    where the results go, e.g. a slice of a cache, or the input itself.  Returns (q_out, k_out)."""
     lib = L.load()
-    head = _qk_norm_params(q, k, q_weight, k_weight, rope, positions, eps, interleaved, q_alpha)
+    head = _qk_norm_fields(q, k, q_weight, k_weight, rope, positions, eps, interleaved, q_alpha)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if k is not None and k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    if k is None and k_out is not None:
+        q_out = q.new_empty(q.shape)
+    qo, ko = _heads4(q_out, "q_out", q, q.shape), _NOWHERE
+    if k is not None:
+        if k_out is None:
+            k_out = k.new_empty(k.shape)
+        ko = _heads4(k_out, "k_out", q, k.shape)
+    elif k_out is not None:
         raise ValueError("k_out without k")
-    qo = _heads4(q_out, "q_out", q, tuple(q.shape))
-    ko = _NOWHERE if k is None else _heads4(k_out, "k_out", q, tuple(k.shape))
-    if q.numel() + (0 if k is None else k.numel()) == 0:
+    n = q.numel() + (0 if k is None else k.numel())
+    if n == 0:
         return q_out, k_out
-    p = L.QkNormParams(*head, *qo, *ko)
+    p = L.QK_NORM_PACK.pack(*head, *qo, *ko, *_NOWHERE, *_NOWHERE, 0, 0, 0, 0)
     if _WORK is not None:
-        n = q.numel() + (0 if k is None else k.numel())
-        _work(K_QK_NORM, n * 4, f"B{p.B} T{p.T} h{p.Hq}+{p.Hkv} d{p.d} rot{p.rot}")
-    with _on_device_of(q) as stream:
-        L.check(lib.anip_qk_norm_rope(C.byref(p), stream), "anip_qk_norm_rope")
+        _work(K_QK_NORM, n * 4, f"B{head[1]} T{head[2]} h{head[3]}+{head[4]} d{head[5]} rot{head[6]}")
+    rc = _launch(q, lambda s: lib.anip_qk_norm_rope(p, s))
+    if rc:
+        L.check(rc, "anip_qk_norm_rope")
     return q_out, k_out
 
 
@@ -753,26 +752,31 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, rope=None, p
     """gradients of qk_norm_rope: (dq, dk, dq_weight, dk_weight) from those of its outputs and its inputs; dq, dk contiguous in
     the inputs' type, the weights' in fp32.  k None: dk and dk_weight are None."""
     lib = L.load()
-    head = _qk_norm_params(q, k, q_weight, k_weight, rope, positions, eps, interleaved, q_alpha)
-    gq = _heads4(dq_out, "dq_out", q, tuple(q.shape))
-    gk = _NOWHERE
-    dq, dk, dwk = torch.empty(q.shape, dtype=q.dtype, device=q.device), None, None
-    dwq = torch.empty_like(q_weight)
+    head = _qk_norm_fields(q, k, q_weight, k_weight, rope, positions, eps, interleaved, q_alpha)
+    gq, gk, ko = _heads4(dq_out, "dq_out", q, q.shape), _NOWHERE, _NOWHERE
+    dq, dk, dwk = q.new_empty(q.shape), None, None
+    dwq = q_weight.new_empty(q_weight.shape)
     if k is not None:
-        gk = _heads4(dk_out, "dk_out", q, tuple(k.shape))
-        dk, dwk = torch.empty(k.shape, dtype=k.dtype, device=k.device), torch.empty_like(k_weight)
+        gk = _heads4(dk_out, "dk_out", q, k.shape)
+        dk, dwk = k.new_empty(k.shape), k_weight.new_empty(k_weight.shape)
+        ko = _heads4(dk, "dk")
     elif dk_out is not None:
         raise ValueError("dk_out without k")
     n = q.numel() + (0 if k is None else k.numel())
     if n == 0:
         return dq, dk, dwq.zero_(), None if dwk is None else dwk.zero_()
     _, B, T, Hq, Hkv, d = head[:6]
-    _work(K_QK_NORM, n * 6, f"B{B} T{T} h{Hq}+{Hkv} d{d} bwd")
-    with _on_device_of(q) as stream:
-        ws = torch.empty((lib.anip_qk_norm_rope_backward_ws_floats(B * T, Hq, Hkv, d),), dtype=F32, device=q.device)
-        p = L.QkNormParams(*head, *_heads4(dq, "dq"), *(_NOWHERE if k is None else _heads4(dk, "dk")), *gq, *gk, dwq.data_ptr(),
-                           _p(dwk), ws.data_ptr(), ws.numel())
-        L.check(lib.anip_qk_norm_rope_backward(C.byref(p), stream), "anip_qk_norm_rope_backward")
+    if _WORK is not None:
+        _work(K_QK_NORM, n * 6, f"B{B} T{T} h{Hq}+{Hkv} d{d} bwd")
+
+    def call(stream):
+        need = lib.anip_qk_norm_rope_backward_ws_floats(B * T, Hq, Hkv, d)
+        ws = q_weight.new_empty((need,))
+        p = L.QK_NORM_PACK.pack(*head, *_heads4(dq, "dq"), *ko, *gq, *gk, dwq.data_ptr(), _p(dwk), ws.data_ptr(), need)
+        return lib.anip_qk_norm_rope_backward(p, stream)
+    rc = _launch(q, call)
+    if rc:
+        L.check(rc, "anip_qk_norm_rope_backward")
     return dq, dk, dwq, dwk
 
 
@@ -797,13 +801,13 @@ def relative_buckets(num_buckets, max_distance, bidirectional=True, device="cuda
     return torch.tensor(of[:0:-1] + of[:1] + ahead, dtype=torch.int32, device=device)
 
 
-def _attn_head(what, maps, q, k, v, causal, scale, kv_lens, q_start):
-    """checks of the operands shared by forward and backward -> (fields of AttnParams up to q_start, sizes)"""
+def _attn_fields(what, maps, q, k, v, causal, scale, kv_lens, q_start):
+    """checks of the operands shared by forward and backward -> the fields of anip_attn_params up to q_start"""
     qp = _heads4(q, "q")
     B, Tq, Hq, d = q.shape
     if k.dim() != 4 or v.dim() != 4:
         raise ValueError(f"{what}: k and v: expected (batch, token, head, channel)")
-    Tk, Hk = k.shape[1], k.shape[2]
+    _, Tk, Hk, _ = k.shape
     H, Hkv = Hq // maps, Hk // maps
     kp = _heads4(k, "k", q, (B, Tk, Hkv * maps, d))
     vp = _heads4(v, "v", q, (B, Tk, Hkv, maps * d))
@@ -815,82 +819,87 @@ def _attn_head(what, maps, q, k, v, causal, scale, kv_lens, q_start):
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError(f"{what}: scale must be positive and finite, got {scale}")
-    lens = _aux(kv_lens, "kv_lens", torch.int32, (B,), q)
-    start = _aux(q_start, "q_start", torch.int32, (B,), q)
-    return (_DTYPES[q.dtype], B, Tq, Tk, H, Hkv, d, int(bool(causal)), scale, *qp, *kp, *vp, lens, start), (B, Tq, Tk, H, Hkv, d)
+    return (_DTYPES[q.dtype], B, Tq, Tk, H, Hkv, d, 1 if causal else 0, scale, *qp, *kp, *vp,
+            0 if kv_lens is None else _aux(kv_lens, "kv_lens", torch.int32, (B,), q),
+            0 if q_start is None else _aux(q_start, "q_start", torch.int32, (B,), q))
 
 
 def _bias_fields(what, table, buckets, q, H):
-    if table.dim() != 2 or buckets.dim() != 1 or buckets.shape[0] % 2 == 0:
+    nb, n = table.shape[-1], buckets.shape[0] if buckets.dim() == 1 else 0
+    if table.dim() != 2 or n % 2 == 0 or nb < 1:
         raise ValueError(f"{what}: expected table (heads, buckets) and buckets (2 max_distance + 1), got {tuple(table.shape)}, "
                          f"{tuple(buckets.shape)}")
-    if buckets.shape[0] > 8193:
-        raise ValueError(f"{what}: relative positions up to 4096 can be told apart, {buckets.shape[0] // 2} are asked for")
-    nb = table.shape[1]
-    if nb < 1:
-        raise ValueError(f"{what}: the table holds no buckets")
-    return (_aux(table, "table", q.dtype, (H, nb), q), _aux(buckets, "buckets", torch.int32, tuple(buckets.shape), q), nb,
-            buckets.shape[0] // 2)
+    if n > 8193:
+        raise ValueError(f"{what}: relative positions up to 4096 can be told apart, {n // 2} are asked for")
+    return _aux(table, "table", q.dtype, (H, nb), q), _aux(buckets, "buckets", torch.int32, (n,), q), nb, n // 2
 
 
-def _attn_work(kid, sizes, maps, train, causal):
-    if _WORK is not None:
-        B, Tq, Tk, H, Hkv, d = sizes
-        pairs = Tq * Tk - (Tq * (Tq - 1) // 2 if causal and Tq <= Tk else 0)
-        _work(kid, 2 * B * H * pairs * d * ((5 if train else 2) if maps == 1 else (10 if train else 4)),
-              f"B{B} Tq{Tq} Tk{Tk} h{H}/{Hkv} d{d}{' causal' if causal else ''}{' bwd' if train else ''}",
-              2 * B * d * maps * ((2 if not train else 4) * Tq * H + (2 if not train else 4) * Tk * Hkv))
+def _attn_work(kid, fields, maps, train):
+    _, B, Tq, Tk, H, Hkv, d, causal = fields[:8]
+    pairs = Tq * Tk - (Tq * (Tq - 1) // 2 if causal and Tq <= Tk else 0)
+    n = 4 if train else 2
+    _work(kid, 2 * B * H * pairs * d * ((5 if train else 2) if maps == 1 else (10 if train else 4)),
+          f"B{B} Tq{Tq} Tk{Tk} h{H}/{Hkv} d{d}{' causal' if causal else ''}{' bwd' if train else ''}",
+          2 * B * d * maps * n * (Tq * H + Tk * Hkv))
 
 
-def _attention(what, maps, kid, q, k, v, middle, causal, scale, kv_lens, q_start, for_backward):
-    lib = L.load()
-    head, sizes = _attn_head(what, maps, q, k, v, causal, scale, kv_lens, q_start)
-    B, Tq, Tk, H, Hkv, d = sizes
-    bias, lam = middle(q, H)
-    out = torch.empty((B, Tq, H, maps * d), dtype=q.dtype, device=q.device)
-    out2 = torch.empty_like(out) if for_backward and maps == 2 else None
-    lse = torch.empty((B, H * maps, Tq), dtype=F32, device=q.device) if for_backward else None
+def _attention(what, maps, kid, entry, ws_bytes, q, k, v, fields, bias, lam, for_backward):
+    B, Tq, Tk, H = fields[1:5]
+    out = q.new_empty((B, Tq, H, v.shape[3]))
+    out2 = lse = None
+    if for_backward:
+        out2 = q.new_empty(out.shape) if maps == 2 else None
+        lse = q.new_empty((B, H * maps, Tq), dtype=F32)
     if out.numel() == 0 or Tk == 0:
         for t, fill in ((out, 0.0), (out2, 0.0), (lse, -float("inf"))):
             if t is not None:
                 t.fill_(fill)
         return out, out2, lse
-    p = L.AttnParams(*head, *bias, lam, out.data_ptr(), _p(out2), _p(lse))
-    _attn_work(kid, sizes, maps, False, causal)
-    with _on_device_of(q) as stream:
-        need = getattr(lib, f"anip_{what}_ws_bytes")(C.byref(p), 0)
+    head = (*fields, *bias, lam, out.data_ptr(), _p(out2), _p(lse), *_NOWHERE, 0, 0, 0, 0, 0)
+    if _WORK is not None:
+        _attn_work(kid, fields, maps, False)
+
+    def call(stream):
+        p = L.ATTN_PACK.pack(*head, 0, 0)
+        need = ws_bytes(p, 0)
         if need < 0:
-            L.check(int(need), f"anip_{what}_ws_bytes")
+            return need
         if need:
-            ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
-            p.workspace, p.workspace_bytes = ws.data_ptr(), need
-        L.check(getattr(lib, f"anip_{what}")(C.byref(p), stream), f"anip_{what}")
+            ws = q.new_empty((need,), dtype=torch.uint8)
+            p = L.ATTN_PACK.pack(*head, ws.data_ptr(), need)
+        return entry(p, stream)
+    rc = _launch(q, call)
+    if rc:
+        L.check(rc, f"anip_{what}")
     return out, out2, lse
 
 
-def _attention_backward(what, maps, kid, dout, q, k, v, out, out2, lse, middle, causal, scale, kv_lens, q_start):
-    lib = L.load()
-    head, sizes = _attn_head(what, maps, q, k, v, causal, scale, kv_lens, q_start)
-    B, Tq, Tk, H, Hkv, d = sizes
-    bias, lam, dlast, last = middle(q, H)
-    gp = _heads4(dout, "dout", q, (B, Tq, H, maps * d))
-    op = _aux(out, "out", q.dtype, (B, Tq, H, maps * d), q)
-    o2p = _aux(out2, "out2", q.dtype, (B, Tq, H, maps * d), q)
-    lp = _aux(lse, "lse", F32, (B, H * maps, Tq), q)
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+def _attention_backward(what, maps, kid, entry, ws_bytes, dout, q, k, v, out, out2, lse, fields, bias, lam, dlast, last):
+    B, Tq, Tk, H = fields[1:5]
+    shape = (B, Tq, H, v.shape[3])
+    gp = _heads4(dout, "dout", q, shape)
+    saved = (_aux(out, "out", q.dtype, shape, q), _aux(out2, "out2", q.dtype, shape, q), _aux(lse, "lse", F32, (B, H * maps, Tq), q))
+    if 0 in saved[:maps] or not saved[2]:
+        if q.numel() and k.numel():
+            raise ValueError(f"{what}: out, lse and, for two maps, out2 of the forward are wanted")
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     if q.numel() == 0 or k.numel() == 0:
         for t in (dq, dk, dv, dlast):
             t.zero_()
         return dq, dk, dv, dlast
-    p = L.AttnParams(*head, *bias, lam, op, o2p, lp, *gp, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *last)
-    _attn_work(kid, sizes, maps, True, causal)
-    with _on_device_of(q) as stream:
-        need = getattr(lib, f"anip_{what}_ws_bytes")(C.byref(p), 1)
+    head = (*fields, *bias, lam, *saved, *gp, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), *last)
+    if _WORK is not None:
+        _attn_work(kid, fields, maps, True)
+
+    def call(stream):
+        need = ws_bytes(L.ATTN_PACK.pack(*head, 0, 0), 1)
         if need < 0:
-            L.check(int(need), f"anip_{what}_ws_bytes")
-        ws = torch.empty((need,), dtype=torch.uint8, device=q.device)
-        p.workspace, p.workspace_bytes = ws.data_ptr(), need
-        L.check(getattr(lib, f"anip_{what}_backward")(C.byref(p), stream), f"anip_{what}_backward")
+            return need
+        ws = q.new_empty((need,), dtype=torch.uint8)
+        return entry(L.ATTN_PACK.pack(*head, ws.data_ptr(), need), stream)
+    rc = _launch(q, call)
+    if rc:
+        L.check(rc, f"anip_{what}_backward")
     return dq, dk, dv, dlast
 
 
@@ -904,24 +913,25 @@ def relative_attention(q, k, v, table, buckets, causal=False, scale=None, kv_len
     it are not seen, whatever they hold (padded batch, cache).  q_start (B,) int32: the position of query 0 (default Tk - Tq: the
     queries are the last tokens); causal: query i sees keys up to q_start + i.  A query that sees no key gets zeros.
     Returns out (B, Tq, H, d), or (out, lse) for_backward (lse (B, H, Tq) fp32)."""
-    out, _, lse = _attention("relative_attention", 1, K_REL_ATTN, q, k, v,
-                             lambda q_, H: (_bias_fields("relative_attention", table, buckets, q_, H), None),
-                             causal, scale, kv_lens, q_start, for_backward)
+    lib, what = L.load(), "relative_attention"
+    fields = _attn_fields(what, 1, q, k, v, causal, scale, kv_lens, q_start)
+    out, _, lse = _attention(what, 1, K_REL_ATTN, lib.anip_relative_attention, lib.anip_relative_attention_ws_bytes, q, k, v, fields,
+                             _bias_fields(what, table, buckets, q, fields[4]), 0, for_backward)
     return (out, lse) if for_backward else out
 
 
 def relative_attention_backward(dout, q, k, v, out, lse, table, buckets, causal=False, scale=None, kv_lens=None, q_start=None):
     """gradients of relative_attention from that of its output, its inputs and what it returned for_backward:
     (dq, dk, dv, dtable), in the inputs' type; shared key heads' parts are added, keys behind kv_lens get zeros."""
-    def middle(q_, H):
-        f = _bias_fields("relative_attention_backward", table, buckets, q_, H)
-        dtable = torch.empty_like(table)
-        return f, None, dtable, (dtable.data_ptr(),)
-    return _attention_backward("relative_attention", 1, K_REL_ATTN, dout, q, k, v, out, None, lse, middle, causal, scale, kv_lens,
-                               q_start)
+    lib, what = L.load(), "relative_attention"
+    fields = _attn_fields(what, 1, q, k, v, causal, scale, kv_lens, q_start)
+    bias = _bias_fields(what, table, buckets, q, fields[4])
+    dtable = table.new_empty(table.shape)
+    return _attention_backward(what, 1, K_REL_ATTN, lib.anip_relative_attention_backward, lib.anip_relative_attention_ws_bytes, dout, q, k,
+                               v, out, None, lse, fields, bias, 0, dtable, (dtable.data_ptr(), 0))
 
 
-_NO_BIAS = (None, None, 0, 0)
+_NO_BIAS = (0, 0, 0, 0)
 
 
 def differential_attention(q, k, v, lam, causal=False, scale=None, kv_lens=None, q_start=None, for_backward=False):
@@ -930,20 +940,22 @@ def differential_attention(q, k, v, lam, causal=False, scale=None, kv_lens=None,
     q (B, Tq, 2 H, d), k (B, Tk, 2 Hkv, d): heads 2 h, 2 h + 1 are the two maps of head h; v (B, Tk, Hkv, 2 d); lam (H,) fp32;
     d <= 128.  The rest as relative_attention.  Returns out (B, Tq, H, 2 d), or (out, out2, lse) for_backward: out2 the second
     map's output, lse (B, 2 H, Tq) fp32."""
-    out, out2, lse = _attention("differential_attention", 2, K_DIFF_ATTN, q, k, v,
-                                lambda q_, H: (_NO_BIAS, _aux(lam, "lam", F32, (H,), q_)),
-                                causal, scale, kv_lens, q_start, for_backward)
+    lib, what = L.load(), "differential_attention"
+    fields = _attn_fields(what, 2, q, k, v, causal, scale, kv_lens, q_start)
+    out, out2, lse = _attention(what, 2, K_DIFF_ATTN, lib.anip_differential_attention, lib.anip_differential_attention_ws_bytes, q, k, v,
+                                fields, _NO_BIAS, _aux(lam, "lam", F32, (fields[4],), q), for_backward)
     return (out, out2, lse) if for_backward else out
 
 
 def differential_attention_backward(dout, q, k, v, out, out2, lse, lam, causal=False, scale=None, kv_lens=None, q_start=None):
     """gradients of differential_attention from that of its output, its inputs and what it returned for_backward:
     (dq, dk, dv) in the inputs' type and dlam (H,) fp32."""
-    def middle(q_, H):
-        dlam = torch.empty((H,), dtype=F32, device=q_.device)
-        return _NO_BIAS, _aux(lam, "lam", F32, (H,), q_), dlam, (None, dlam.data_ptr())
-    return _attention_backward("differential_attention", 2, K_DIFF_ATTN, dout, q, k, v, out, out2, lse, middle, causal, scale,
-                               kv_lens, q_start)
+    lib, what = L.load(), "differential_attention"
+    fields = _attn_fields(what, 2, q, k, v, causal, scale, kv_lens, q_start)
+    lp = _aux(lam, "lam", F32, (fields[4],), q)
+    dlam = lam.new_empty(lam.shape)
+    return _attention_backward(what, 2, K_DIFF_ATTN, lib.anip_differential_attention_backward, lib.anip_differential_attention_ws_bytes,
+                               dout, q, k, v, out, out2, lse, fields, _NO_BIAS, lp, dlam, (0, dlam.data_ptr()))
 
 
 def softmax_rows(s):
