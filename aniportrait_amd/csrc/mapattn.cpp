@@ -103,21 +103,18 @@ int forward(const char* what, const anip_attn_params* p, int maps, int kid, void
 // one wave per workgroup on short sequences, which would leave three of four idle
 int waves_for(int T) { return T <= 64 ? 1 : 4; }
 
-// the keys' kernel walks over the queries of all heads that share a key head; where the keys alone make fewer workgroups than the
-// chip holds at once (one of 4 wave groups per CU), the walk is split towards two rounds of them, each with 8 tiles at the least
-int dkv_splits(const anip_attn_params* p, int nwk) {
-  const int64_t blocks = (int64_t)((p->Tk + 32 * nwk - 1) / (32 * nwk)) * p->B * p->Hkv * nwk / 4;
-  const int64_t tiles = (int64_t)((p->Tq + 63) / 64) * (p->H / p->Hkv);
-  if (blocks < 1) return 1;
-  if (blocks > 192) return 1;
-  int64_t s = (512 + blocks - 1) / blocks;
-  s = s < tiles / 8 ? s : tiles / 8;
+// Both kernels of the backward walk over tiles of the other side.  The chip holds two workgroups of 4 wave groups per CU (one, with
+// two maps or the widest heads); where there are fewer, the walk is split towards that, with 4 tiles at the least for each part.
+int walk_splits(int64_t blocks, int64_t tiles) {
+  if (blocks < 1) blocks = 1;
+  int64_t s = 512 / blocks;
+  s = s < tiles / 4 ? s : tiles / 4;
   return (int)(s < 1 ? 1 : (s > 16 ? 16 : s));
 }
 
 struct BwdLayout {
-  int nwq, nwk, Tp, QW, ND, parts, splits;
-  int64_t rows, diag, dlam, part, dkv, total;  // floats
+  int nwq, nwk, Tp, QW, ND, parts, qsplits, ksplits;
+  int64_t rows, diag, dlam, part, dkv, dq, total;  // floats; the parts of dq and dkv share their place
 };
 BwdLayout layout(const anip_attn_params* p, int maps) {
   BwdLayout l{};
@@ -126,17 +123,20 @@ BwdLayout layout(const anip_attn_params* p, int maps) {
   l.Tp = l.nwq == 1 ? (p->Tq + 63) / 64 * 64 : (p->Tq + 127) / 128 * 128;
   l.QW = (p->Tq + 31) / 32;
   l.rows = (int64_t)p->B * p->H * maps * l.Tp;
+  l.qsplits = walk_splits((int64_t)l.Tp / 32 * p->B * p->H / 4, (p->Tk + 63) / 64);
+  l.ksplits = walk_splits((int64_t)((p->Tk + 31) / 32) * p->B * p->Hkv / 4, (int64_t)((p->Tq + 63) / 64) * (p->H / p->Hkv));
   if (maps == 1) {
     l.ND = 2 * p->max_distance + 128;
-    const int64_t groups = (int64_t)p->B * l.QW;
+    const int64_t groups = (int64_t)p->B * l.QW * l.qsplits;
     l.parts = (int)(groups < 32 ? groups : 32);  // few query groups: their own sums are the parts
     l.diag = (int64_t)p->H * groups * (l.ND + 2);
     l.part = groups > 32 ? (int64_t)p->H * l.parts * (l.ND + 2) : 0;
   } else {
-    l.dlam = (int64_t)p->H * p->B * l.QW;
+    l.dlam = (int64_t)p->H * p->B * l.QW * l.qsplits;
   }
-  l.splits = dkv_splits(p, l.nwk);
-  if (l.splits > 1) l.dkv = (int64_t)l.splits * p->B * p->Tk * p->Hkv * 2 * maps * p->d;
+  if (l.qsplits > 1) l.dq = (int64_t)l.qsplits * p->B * p->Tq * p->H * maps * p->d;
+  if (l.ksplits > 1) l.dkv = (int64_t)l.ksplits * p->B * p->Tk * p->Hkv * 2 * maps * p->d;
+  l.dkv = l.dkv > l.dq ? l.dkv : l.dq;
   l.total = l.dkv + 2 * l.rows + l.diag + l.part + l.dlam;
   return l;
 }
@@ -146,7 +146,7 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   if (rc) return rc;
   const BwdLayout l = layout(p, maps);
   ANIP_REQUIRE(p->workspace != nullptr && ((uintptr_t)p->workspace & 15) == 0 && p->workspace_bytes >= l.total * 4, "%s: a workspace of %lld bytes is wanted, 16-byte aligned", what, (long long)l.total * 4);
-  ANIP_REQUIRE((int64_t)(l.Tp / 32) * p->B * p->H < (1ll << 31) && (int64_t)((p->Tk + 31) / 32) * p->B * p->Hkv < (1ll << 31) && (int64_t)p->B * p->Tk * p->Hkv * maps * p->d / 512 < (1ll << 31), "%s: too many rows for one launch", what);
+  ANIP_REQUIRE((int64_t)(l.Tp / 32) * l.qsplits * p->B * p->H < (1ll << 31) && (int64_t)((p->Tk + 31) / 32) * l.ksplits * p->B * p->Hkv < (1ll << 31) && (int64_t)p->B * p->Tq * p->H * maps * p->d / 512 < (1ll << 31) && (int64_t)p->B * p->Tk * p->Hkv * maps * p->d / 512 < (1ll << 31), "%s: too many rows for one launch", what);
   ANIP_REQUIRE((int64_t)((p->Tq + 31) / 32) * (p->H / p->Hkv) < (1ll << 31), "%s: too many query tiles", what);
   MapAttnArgs a = args(p, maps);
   a.dout = p->dout, a.do_sb = p->dout_stride[0], a.do_st = p->dout_stride[1], a.do_sh = p->dout_stride[2];
@@ -160,10 +160,11 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   a.dlam_part = a.diag + l.diag + l.part;
   hipStream_t s = (hipStream_t)stream;
   AnipProfScope prof_(kid, stream);
+  a.splits = l.qsplits;
   int r = mapattn_dq(a, maps, p->dtype, l.nwq, s);
-  a.splits = l.splits;
-  if (!r) r = mapattn_dkv(a, maps, p->dtype, l.nwk, s);
   if (!r) r = mapattn_reduce(a, maps, p->dtype, s);
+  a.splits = l.ksplits;
+  if (!r) r = mapattn_dkv(a, maps, p->dtype, l.nwk, s);
   return r;
 }
 

@@ -31,7 +31,7 @@ __device__ __forceinline__ f32x16 get16(const float* x) {
 
 // ---- dQ: 32 queries per wave (pair), tiles of KT keys -----------------------------------------------------------------------
 template <typename T, int MAPS, int KS, int NT, int KT, int NG>
-__global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) void mapattn_dq_kernel(const MapAttnArgs a) {
+__global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) void mapattn_dq_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
   constexpr int NW = NG * MAPS, BQ = 32 * NG, DT = (KS + 1) / 2, KSV = MAPS == 1 ? KS : NT;  // KSV: steps over this wave's share of dv
   constexpr int KCH = 4 * DT, VCH = 4 * NT;
@@ -48,8 +48,9 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) voi
   float* theirs = (float*)(smem + 2 * STAGE) + (wave ^ 1) * 1024 + lane * 4;
   const int nqb = a.Tp / BQ;
   int qb, bh;
-  if (!place(blockIdx.x, nqb, a.B * a.H, qb, bh)) return;
-  qb = nqb - 1 - qb;
+  if (!place(blockIdx.x, nqb * a.splits, a.B * a.H, qb, bh)) return;
+  const int split = qb % a.splits;
+  qb = nqb - 1 - qb / a.splits;
   const int b = bh / a.H, head = bh - b * a.H, kvh = head / a.G;
   const int len = seq_len(a, b), start = seq_start(a, b);
   const int q0 = qb * BQ + grp * 32, qi = q0 + ql, pw = start + q0;
@@ -58,7 +59,8 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) voi
   int kend = len;
   if (a.causal) kend = min(kend, start + min(qb * BQ + BQ, a.Tq));
   if (qb * BQ >= a.Tq) kend = 0;  // padding rows: only their row statistics are written
-  const int nt_all = kend > 0 ? (kend + KT - 1) / KT : 0;
+  const int nt_keys = kend > 0 ? (kend + KT - 1) / KT : 0;
+  const int nt0 = (int)((int64_t)nt_keys * split / a.splits), nt_all = (int)((int64_t)nt_keys * (split + 1) / a.splits);
 
   const float lam = MAPS == 2 ? a.lam[head] : 0.f;
   u32x4 qf[KS], df[KSV];
@@ -92,7 +94,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) voi
     }
     const float l = valid ? a.lse[((int64_t)bh * MAPS + m) * a.Tq + qi] * LOG2E : -INFINITY;
     nl = l == -INFINITY ? -INFINITY : -l;  // rows without keys: P = 2^-inf = 0
-    if (h == 0) {
+    if (h == 0 && split == 0) {
       const int64_t at = ((int64_t)bh * MAPS + m) * a.Tp + qi;
       a.rows_lse[at] = nl + Num<T>::PSH;
       a.rows_d[at] = D * (1.0f / (1 << Num<T>::PSH));
@@ -101,7 +103,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) voi
 
   float* diag = nullptr;
   if (BIAS && q0 < a.Tq) {
-    diag = a.diag + (((int64_t)head * a.B + b) * a.QW + q0 / 32) * (a.ND + 2);
+    diag = a.diag + ((((int64_t)head * a.B + b) * a.QW + q0 / 32) * a.splits + split) * (a.ND + 2);
     for (int x = lane; x < a.ND + 2; x += 64) diag[x] = 0.f;  // (complete before the first tile's wait; later stores are this wave's own)
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   }
@@ -144,8 +146,8 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) voi
   // dS = wf P W + wd P
   const float wf = m == 0 ? 1.f : -lam, wd = m == 0 ? -D : lam * D;
 
-  if (nt_all > 0) issue(0);
-  for (int t = 0; t < nt_all; ++t) {
+  if (nt0 < nt_all) issue(nt0);
+  for (int t = nt0; t < nt_all; ++t) {
     MAPATTN_WAIT_DMA();
     __syncthreads();
     if (t + 1 < nt_all) issue(t + 1);
@@ -242,9 +244,21 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) voi
   }
   if (MAPS == 2 && m == 1 && q0 < a.Tq) {
     const float t = wave_sum(dl_sum);
-    if (lane == 0) a.dlam_part[((int64_t)head * a.B + b) * a.QW + q0 / 32] = -t;
+    if (lane == 0) a.dlam_part[(((int64_t)head * a.B + b) * a.QW + q0 / 32) * a.splits + split] = -t;
   }
   if (!valid) return;
+  if (a.splits > 1) {
+    float* pp = a.part_o + (((int64_t)split * a.B * a.Tq + (int64_t)b * a.Tq + qi) * a.H * MAPS + head * MAPS + m) * a.d;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int rq = 0; rq < 4; ++rq) {
+        const int c0 = dt * 32 + rq * 8 + h * 4;
+        const f32x16& x = dq[dt];
+        if (c0 < a.d) *(f32x4*)(pp + c0) = f32x4{x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale, x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale};
+      }
+    return;
+  }
   char* op = (char*)a.dq + ((((int64_t)b * a.Tq + qi) * a.H + head) * MAPS + m) * a.d * 2;
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt)
@@ -259,7 +273,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) voi
 
 // ---- dK, dV: 32 keys per wave (pair; K and V rows in registers), tiles of QT queries of every head that shares them ------------
 template <typename T, int MAPS, int KS, int NT, int QT, int NG>
-__global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) void mapattn_dkv_kernel(const MapAttnArgs a) {
+__global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 2 : 1)) void mapattn_dkv_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
   constexpr int NW = NG * MAPS, BK = 32 * NG, DT = (KS + 1) / 2;
   constexpr int KSV = MAPS == 1 ? KS : NT;               // steps over this wave's share of dv in W
@@ -493,19 +507,24 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 2 && NG == 4 ? 2 : 1)) voi
     }
 }
 
-// dK, dV from the parts of a split walk: one thread per 4 channels, the parts in their order
-template <typename T>
-__global__ __launch_bounds__(256) void mapattn_dkv_join_kernel(const MapAttnArgs a) {
-  const int64_t rows = (int64_t)a.B * a.Tk * a.Hkv;
-  const int qn = a.dv / 2;
+// gradients from the 32-bit parts of a split walk, the parts in their order, one thread per 4 channels: rows of `a.dv` channels of
+// dK and as many of dV (KV), or rows of dQ
+template <typename T, bool KV>
+__global__ __launch_bounds__(256) void mapattn_join_kernel(const MapAttnArgs a) {
+  const int64_t rows = KV ? (int64_t)a.B * a.Tk * a.Hkv : (int64_t)a.B * a.Tq * a.H;
+  const int qn = KV ? a.dv / 2 : a.dv / 4;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * qn) return;
-  const int64_t row = i / qn;
-  const int c0 = (int)(i - row * qn) * 4;
-  const float* p = a.part_o + row * (2 * a.dv) + c0;
+  const float* p = a.part_o + i * 4;
   f32x4 t = *(const f32x4*)p;
 #pragma unroll 4
-  for (int s = 1; s < a.splits; ++s) t += *(const f32x4*)(p + (int64_t)s * rows * (2 * a.dv));
+  for (int s = 1; s < a.splits; ++s) t += *(const f32x4*)(p + s * rows * qn * 4);
+  if (!KV) {
+    *(u32x2*)((char*)a.dq + i * 8) = u32x2{Num<T>::pack(t[0], t[1]), Num<T>::pack(t[2], t[3])};
+    return;
+  }
+  const int64_t row = i / qn;
+  const int c0 = (int)(i - row * qn) * 4;
   char* op = c0 < a.dv ? (char*)a.dk + (row * a.dv + c0) * 2 : (char*)a.dvo + (row * a.dv + c0 - a.dv) * 2;
   *(u32x2*)op = u32x2{Num<T>::pack(t[0], t[1]), Num<T>::pack(t[2], t[3])};
 }
@@ -515,7 +534,7 @@ __global__ __launch_bounds__(256) void mapattn_dkv_join_kernel(const MapAttnArgs
 __global__ __launch_bounds__(256) void mapattn_diag_kernel(const MapAttnArgs a) {
   const int slot = blockIdx.x * 256 + threadIdx.x, part = blockIdx.y, head = blockIdx.z;
   if (slot >= a.ND + 2) return;
-  const int64_t rows = (int64_t)a.B * a.QW, r0 = rows * part / a.parts, r1 = rows * (part + 1) / a.parts;
+  const int64_t rows = (int64_t)a.B * a.QW * a.splits, r0 = rows * part / a.parts, r1 = rows * (part + 1) / a.parts;
   const float* p = a.diag + ((int64_t)head * rows) * (a.ND + 2) + slot;
   float t = 0.f;
 #pragma unroll 8
@@ -548,7 +567,7 @@ __global__ __launch_bounds__(1024) void mapattn_dtable_kernel(const MapAttnArgs 
 }
 __global__ __launch_bounds__(256) void mapattn_dlam_kernel(const MapAttnArgs a) {
   __shared__ float part[4];
-  const int64_t rows = (int64_t)a.B * a.QW;
+  const int64_t rows = (int64_t)a.B * a.QW * a.splits;
   const float* p = a.dlam_part + blockIdx.x * rows;
   float t = 0.f;
   for (int64_t r = threadIdx.x; r < rows; r += 256) t += p[r];
@@ -571,7 +590,7 @@ int run_dq(const MapAttnArgs& a, hipStream_t s) {
     anip_set_error("mapattn dq: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
-  hipLaunchKernelGGL((mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG>), dim3((unsigned)(a.Tp / (32 * NG) * a.B * a.H)), dim3(64 * NG * MAPS), lds, s, a);
+  hipLaunchKernelGGL((mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG>), dim3((unsigned)(a.Tp / (32 * NG) * a.splits * a.B * a.H)), dim3(64 * NG * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dq_kernel");
   return 0;
 }
@@ -611,15 +630,22 @@ int dkv_t(const MapAttnArgs& a, int maps, int nw, hipStream_t s) {
 
 }  // namespace
 
-int mapattn_dq(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) { return bf16 ? dq_t<bf16_t>(a, maps, nw, s) : dq_t<f16>(a, maps, nw, s); }
+template <bool KV>
+static int join(const MapAttnArgs& a, int bf16, hipStream_t s) {
+  if (a.splits == 1) return 0;
+  const dim3 grid((unsigned)cdiv64(KV ? (int64_t)a.B * a.Tk * a.Hkv * (a.dv / 2) : (int64_t)a.B * a.Tq * a.H * (a.dv / 4), 256));
+  if (bf16) hipLaunchKernelGGL((mapattn_join_kernel<bf16_t, KV>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((mapattn_join_kernel<f16, KV>), grid, dim3(256), 0, s, a);
+  ANIP_LAUNCH_CHECK("mapattn_join_kernel");
+  return 0;
+}
+int mapattn_dq(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) {
+  const int r = bf16 ? dq_t<bf16_t>(a, maps, nw, s) : dq_t<f16>(a, maps, nw, s);
+  return r ? r : join<false>(a, bf16, s);
+}
 int mapattn_dkv(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) {
   const int r = bf16 ? dkv_t<bf16_t>(a, maps, nw, s) : dkv_t<f16>(a, maps, nw, s);
-  if (r || a.splits == 1) return r;
-  const dim3 grid((unsigned)cdiv64((int64_t)a.B * a.Tk * a.Hkv * (a.dv / 2), 256));
-  if (bf16) hipLaunchKernelGGL((mapattn_dkv_join_kernel<bf16_t>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((mapattn_dkv_join_kernel<f16>), grid, dim3(256), 0, s, a);
-  ANIP_LAUNCH_CHECK("mapattn_dkv_join_kernel");
-  return 0;
+  return r ? r : join<true>(a, bf16, s);
 }
 int mapattn_reduce(const MapAttnArgs& a, int maps, int bf16, hipStream_t s) {
   if (maps == 2) {
