@@ -29,7 +29,7 @@ struct MapAttnArgs {
   int splits;
   float *part_o, *part_l;  // [split][(b Tq + t) H + h][MAPS][dv], [split][..][MAPS] (base 2)
   // single-token kernel
-  int kw;  // waves that share a problem (1 or 4)
+  int kw, teams;  // teams (a wave per map) that share a problem: 1 or all of the workgroup's
   // backward
   const void* dout;
   int64_t do_sb, do_st, do_sh;

@@ -227,25 +227,27 @@ __global__ __launch_bounds__(64 * QG * MAPS, 2) void mapattn_fwd_kernel(const Ma
 
 // ---- single tokens: few queries against many keys -----------------------------------------------------------------------
 // The Tq x G queries that share a key head are at most 32 columns of one tile.  Bound by reading the keys and values once, so a
-// team of MAPS waves (one for each map, sharing the V tile) walks its own 32-key tiles with its own two LDS stages; the kw = NTEAM
-// teams of a workgroup share a problem (tiles t, t + kw, ..) and join their results in LDS, or each team has its own problem
-// (kw = 1: many short sequences).  A team of one wave waits for its own DMA alone and needs no barrier.
-template <typename T, int MAPS, int KS, int NT, int NTEAM>
-__global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(const MapAttnArgs a) {
+// team of MAPS waves (one for each map, sharing the V tile) walks its own 32-key tiles; the kw = teams teams of a workgroup share a
+// problem (tiles t, t + kw, ..) and join their results in LDS, or each team has its own problem (kw = 1: many short sequences).
+// One map: a team is one wave and needs no barrier; it has one K and one V tile in LDS and refills each as soon as it is read, so
+// that eight waves fit a CU and nearly a tile of each is in flight.  Two maps: two stages, a barrier per tile.
+template <typename T, int MAPS, int KS, int NT, int MAXT>
+__global__ __launch_bounds__(64 * MAXT * MAPS, (MAPS == 1 ? 2 : 1)) void mapattn_token_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
   constexpr int KT = 32;
   constexpr int KCH = 4 * ((KS + 1) / 2), VCH = 4 * NT;
   constexpr int K_BYTES = KT * KCH * 16, V_BYTES = KT * VCH * 16, STAGE = MAPS * K_BYTES + V_BYTES;
+  constexpr int TEAM = MAPS == 1 ? STAGE : 2 * STAGE;
   constexpr int OW = NT * 16 * 64;  // floats of a wave's result
   extern __shared__ __attribute__((aligned(1024))) char smem[];
 
   const int tid = threadIdx.x, lane = tid & 63, ql = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int team = wave / MAPS, m = wave % MAPS;
-  const int ppb = NTEAM / a.kw, kwi = team % a.kw;
+  const int ppb = a.teams / a.kw, kwi = team % a.kw;
   const int problems = a.B * a.Hkv * a.splits;
   const int prob = blockIdx.x * ppb + team / a.kw;
-  const bool live = prob < problems;  // (kw = NTEAM: the same for all waves)
+  const bool live = prob < problems;  // (kw = teams: the same for all waves)
   const int split = prob % a.splits, bk = live ? prob / a.splits : 0;
   const int b = bk / a.Hkv, kvh = bk - b * a.Hkv;
   const int len = live ? seq_len(a, b) : 0, start = seq_start(a, b);
@@ -261,9 +263,6 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
   // turns of the loop: with barriers inside, the same for all teams of the workgroup
   const int turns = MAPS == 1 ? (t1 - t0 - kwi + a.kw - 1) / a.kw : (a.kw == 1 ? (a.Tk + KT - 1) / KT : (t1 - t0 + a.kw - 1) / a.kw);
 
-  u32x4 qf[KS];
-  load_row<KS>(qf, (const char*)a.q + 2 * (b * a.q_sb + (int64_t)qi * a.q_st + (int64_t)(head * MAPS + m) * a.q_sh), mine, h, a.d);
-
   const char* kb[MAPS];
 #pragma unroll
   for (int i = 0; i < MAPS; ++i) kb[i] = (const char*)a.k + 2 * (b * a.k_sb + (int64_t)(kvh * MAPS + i) * a.k_sh);
@@ -272,16 +271,24 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
   TileDma<VCH, KT, MAPS> vd;
   kd.init(m, lane, a.k_st, a.d);
   vd.init(m, lane, a.v_st, a.dv);
-  char* mem = smem + team * 2 * STAGE;
-  auto issue = [&](int t, int st) {
-    char* p = mem + st * STAGE;
-    const int64_t row = (int64_t)t * KT;
-    const int valid = len - t * KT;
+  char* mem = smem + team * TEAM;
+  auto issue_k = [&](int t, char* p) {
 #pragma unroll
-    for (int i = 0; i < MAPS; ++i) kd.issue(kb[i] + row * a.k_st * 2, valid, p + i * K_BYTES, m);
-    vd.issue(vb + row * a.v_st * 2, valid, p + MAPS * K_BYTES, m);
+    for (int i = 0; i < MAPS; ++i) kd.issue(kb[i] + (int64_t)t * KT * a.k_st * 2, len - t * KT, p + i * K_BYTES, m);
   };
-  constexpr int PIECES = TileDma<KCH, KT, 1>::P + TileDma<VCH, KT, 1>::P;  // (MAPS = 1)
+  auto issue_v = [&](int t, char* p) { vd.issue(vb + (int64_t)t * KT * a.v_st * 2, len - t * KT, p + MAPS * K_BYTES, m); };
+  constexpr int KP = TileDma<KCH, KT, 1>::P, VP = TileDma<VCH, KT, 1>::P;  // pieces of a tile (one map: all of them this wave's)
+
+  u32x4 qf[KS];
+  load_row<KS>(qf, (const char*)a.q + 2 * (b * a.q_sb + (int64_t)qi * a.q_st + (int64_t)(head * MAPS + m) * a.q_sh), mine, h, a.d);
+  const float far_lo = BIAS && mine ? bias_at<T>(a, head, -a.R) : 0.f, far_hi = BIAS && mine ? bias_at<T>(a, head, a.R) : 0.f;
+  // (one map) bias of a tile near the queries: [G][31 + Tq] relative positions k0 - (start + Tq - 1) ..
+  float* near = (float*)(smem + a.teams * TEAM) + team * (a.G * (31 + a.Tq));
+  const float* nq = mine ? near + (ql - qi * a.G) * (31 + a.Tq) + (a.Tq - 1 - qi) + 4 * h : near;
+  if (t0 + kwi < t1) {
+    issue_k(t0 + kwi, mem);
+    issue_v(t0 + kwi, mem);
+  }
   RowRead<KCH> kr;
   TrRead<VCH> vr;
   kr.init(lane);
@@ -291,14 +298,11 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
   float mrun = -INFINITY, lrun = 0.f;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) o[nt] = zero16();
-  const float far_lo = BIAS && mine ? bias_at<T>(a, head, -a.R) : 0.f, far_hi = BIAS && mine ? bias_at<T>(a, head, a.R) : 0.f;
 
-  if (t0 + kwi < t1) issue(t0 + kwi, 0);
   for (int it = 0; it < turns; ++it) {
     const int t = t0 + kwi + it * a.kw;
     const int k0 = t * KT;
-    // the bias is fetched before the next tile's DMA is issued, so that waiting for it does not wait for that
-    f32x16 bias;
+    const bool more = t + a.kw < t1;
     float mul = a.scale_log2, add = 0.f;
     bool close = false;
     if (BIAS) {
@@ -306,30 +310,33 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
       else if (k0 - (start + a.Tq - 1) >= a.R) add = far_hi;
       else {
         close = true;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) bias[r] = mine ? bias_at<T>(a, head, k0 + acc_row(r) + 4 * h - (start + qi)) : 0.f;
+        const int w = 31 + a.Tq;
+        for (int e = lane; e < a.G * w; e += 64) near[e] = bias_at<T>(a, kvh * a.G + e / w, k0 - (start + a.Tq - 1) + e % w);
       }
     }
+    const char* tile = mem;
     if (MAPS == 1) {
-      if (t + a.kw < t1) {
-        issue(t + a.kw, (it + 1) & 1);
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(PIECES) : "memory");
-      } else {
-        MAPATTN_WAIT_DMA();
-      }
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"(VP) : "memory");  // K is there; V, issued behind it, may be on its way
     } else {
       MAPATTN_WAIT_DMA();
       __syncthreads();
-      if (t + a.kw < t1) issue(t + a.kw, (it + 1) & 1);
+      if (more) {
+        issue_k(t + a.kw, mem + ((it + 1) & 1) * STAGE);
+        issue_v(t + a.kw, mem + ((it + 1) & 1) * STAGE);
+      }
       if (t >= t1) continue;
+      tile = mem + (it & 1) * STAGE;
     }
-    const char* tile = mem + (it & 1) * STAGE;
     f32x16 s[1] = {zero16()};
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) s[0] = Num<T>::mfma(kr.get(tile + m * K_BYTES, 0, kk), qf[kk], s[0]);
+    if (MAPS == 1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // K is read: its place may be filled again
+      if (more) issue_k(t + a.kw, mem);
+    }
     if (BIAS && close) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[0][r] = fmaf(s[0][r], mul, bias[r]);
+      for (int r = 0; r < 16; ++r) s[0][r] = fmaf(s[0][r], mul, nq[acc_row(r)]);
       mul = 1.f;
     }
     if (k0 + 31 >= len || (a.causal && k0 + 31 > start)) {
@@ -339,19 +346,25 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
     }
     u32x4 p[1][2];
     soft_step<T, NT, 1>(s, mul, add, mrun, lrun, o, p);
+    if (MAPS == 1) {
+      if (more) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(KP) : "memory");
+      else MAPATTN_WAIT_DMA();
+    }
 #pragma unroll
     for (int kb2 = 0; kb2 < 2; ++kb2)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) o[nt] = Num<T>::mfma(vr.get(tile + MAPS * K_BYTES, kb2, nt), p[0][kb2], o[nt]);
-    // (MAPS = 1) the stage just read is written by the DMA issued in the next turn: its reads have returned before that
-    if (MAPS == 1) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (MAPS == 1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) issue_v(t + a.kw, mem);
+    }
   }
   lrun = xor32_sum(lrun);
 
   // ---- join the teams of a problem: team 0 adds the others' results scaled to the common maximum ---------------------------
   if (a.kw > 1) {
     float* jo = (float*)smem;
-    float* jm = jo + (NTEAM - 1) * MAPS * OW;
+    float* jm = jo + (a.teams - 1) * MAPS * OW;
     __syncthreads();  // all tiles read
     if (kwi > 0) {
       const int w = (kwi - 1) * MAPS + m;
@@ -364,12 +377,8 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
     }
     __syncthreads();
     if (kwi == 0) {
-      float mw[NTEAM], all = mrun;
-#pragma unroll
-      for (int i = 0; i < NTEAM - 1; ++i) {
-        mw[i] = jm[(i * MAPS + m) * 128 + lane];
-        all = fmaxf(all, mw[i]);
-      }
+      float all = mrun;
+      for (int i = 0; i < a.teams - 1; ++i) all = fmaxf(all, jm[(i * MAPS + m) * 128 + lane]);
       const float base = all == -INFINITY ? 0.f : all;
       float f = __builtin_amdgcn_exp2f(mrun - base);
       lrun *= f;
@@ -377,10 +386,9 @@ __global__ __launch_bounds__(64 * NTEAM * MAPS, 1) void mapattn_token_kernel(con
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[nt][r] *= f;
-#pragma unroll
-      for (int i = 0; i < NTEAM - 1; ++i) {
+      for (int i = 0; i < a.teams - 1; ++i) {
         const int w = i * MAPS + m;
-        f = __builtin_amdgcn_exp2f(mw[i] - base);
+        f = __builtin_amdgcn_exp2f(jm[w * 128 + lane] - base);
         lrun += f * jm[w * 128 + 64 + lane];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -566,25 +574,30 @@ int run_fwd(const MapAttnArgs& a, hipStream_t s) {
   return 0;
 }
 
-// bytes of a team's two stages of 32 keys; as many teams to a workgroup, up to four, as fit the CU's LDS
-constexpr int token_team_lds(int maps, int ks, int nt) { return 2 * 32 * 16 * (maps * 4 * ((ks + 1) / 2) + 4 * nt); }
-constexpr int token_teams(int maps, int ks, int nt) { return 4 * token_team_lds(maps, ks, nt) <= 160 * 1024 ? 4 : 2; }
+// LDS of a team without the near bias, and the most teams of a workgroup: eight waves, fewer where the CU's LDS does not hold them
+constexpr int token_team_lds(int maps, int ks, int nt) { return maps * 32 * 16 * (maps * 4 * ((ks + 1) / 2) + 4 * nt); }
+constexpr int token_max_teams(int maps, int ks, int nt) {
+  const int fit = 160 * 1024 / (token_team_lds(maps, ks, nt) + (maps == 1 ? 4096 : 0)), most = maps == 1 ? 8 : 4;
+  return fit < most ? fit : most;
+}
 
 template <typename T, int MAPS, int KS, int NT>
 int run_token(const MapAttnArgs& a0, hipStream_t s) {
-  constexpr int NTEAM = token_teams(MAPS, KS, NT), OW = NT * 16 * 64 * 4;
-  constexpr int tiles = NTEAM * token_team_lds(MAPS, KS, NT), join = (NTEAM - 1) * MAPS * (OW + 512), hand = MAPS == 2 ? NTEAM * OW : 0;
-  constexpr int lds = tiles > join ? (tiles > hand ? tiles : hand) : (join > hand ? join : hand);
-  static_assert(lds <= 160 * 1024, "LDS of a CU");
+  constexpr int MAXT = token_max_teams(MAPS, KS, NT), OW = NT * 16 * 64 * 4;
   MapAttnArgs a = a0;
-  if (a.kw > 1) a.kw = NTEAM;
-  const void* f = (const void*)mapattn_token_kernel<T, MAPS, KS, NT, NTEAM>;
+  a.teams = MAXT;  // (4 of 8 teams to a workgroup at one each: 20.2 us against 19.2 at 1024 x 24, 8 heads of 40)
+  if (a.kw > 1) a.kw = a.teams;
+  const int tiles = a.teams * (token_team_lds(MAPS, KS, NT) + (MAPS == 1 ? a.G * (31 + a.Tq) * 4 : 0));
+  const int join = a.kw > 1 ? (a.teams - 1) * MAPS * (OW + 512) : 0, hand = MAPS == 2 ? a.teams * OW : 0;
+  const int lds = tiles > join ? (tiles > hand ? tiles : hand) : (join > hand ? join : hand);
+  static_assert(MAXT >= 2 && (MAXT - 1) * MAPS * (OW + 512) <= 160 * 1024 && MAXT * (token_team_lds(MAPS, KS, NT) + (MAPS == 1 ? 4096 : 0)) <= 160 * 1024, "LDS of a CU");
+  const void* f = (const void*)mapattn_token_kernel<T, MAPS, KS, NT, MAXT>;
   if (anip_raise_lds_limit(f, lds) != 0) {
     anip_set_error("mapattn token: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
-  const int ppb = NTEAM / a.kw;
-  hipLaunchKernelGGL((mapattn_token_kernel<T, MAPS, KS, NT, NTEAM>), dim3((unsigned)((a.B * a.Hkv * a.splits + ppb - 1) / ppb)), dim3(64 * NTEAM * MAPS), lds, s, a);
+  const int ppb = a.teams / a.kw;
+  hipLaunchKernelGGL((mapattn_token_kernel<T, MAPS, KS, NT, MAXT>), dim3((unsigned)((a.B * a.Hkv * a.splits + ppb - 1) / ppb)), dim3(64 * a.teams * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_token_kernel");
   return 0;
 }
