@@ -627,38 +627,48 @@ _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 def _heads4(t, name, like=None, shape=None):
     """(device pointer, strides of batch, token, head) of a (batch, token, head, channel) tensor: contiguous channels, the
     rest any strides that keep 16-byte rows"""
+    p, st, sz = t.data_ptr(), t.stride(), t.shape
+    if len(st) == 4 and st[3] == 1 and not ((st[0] | st[1] | st[2]) & 7 or p & 15) and t.is_cuda and t.dtype in _DTYPES and (
+            like is None or (t.dtype == like.dtype and t.device == like.device)) and (shape is None or sz == shape):
+        return p, st[0], st[1], st[2]
     if not t.is_cuda:
         raise L.HipLibraryError(f"{name}: expected a GPU tensor (the hot path has no CPU fallback)")
     if t.dtype not in _DTYPES:
         raise TypeError(f"{name}: expected fp16 or bf16, got {t.dtype}")
-    sz = t.shape
     if len(sz) != 4:
         raise ValueError(f"{name}: expected (batch, token, head, channel), got shape {tuple(sz)}")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
         raise TypeError(f"{name}: expected {like.dtype} on {like.device}, got {t.dtype} on {t.device}")
     if shape is not None and sz != shape:
         raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(sz)}")
-    p, (sb, st, sh, sc) = t.data_ptr(), t.stride()
-    if sc != 1 and sz[3] != 1:
+    if st[3] != 1 and sz[3] != 1:
         raise ValueError(f"{name}: channels must be contiguous")
-    if (sb | st | sh) & 7 or p & 15:
-        # (the stride of a dimension of one is never taken)
-        sb, st, sh = (0 if n == 1 else x for n, x in zip(sz, (sb, st, sh)))
-        if (sb | st | sh) & 7 or p & 15:
-            raise ValueError(f"{name}: strides must be multiples of 8 elements and the data 16-byte aligned, got strides "
-                             f"{t.stride()}")
-    return p, sb, st, sh
+    sb, st_, sh = (0 if n == 1 else x for n, x in zip(sz, st[:3]))   # (the stride of a dimension of one is never taken)
+    if (sb | st_ | sh) & 7 or p & 15:
+        raise ValueError(f"{name}: strides must be multiples of 8 elements and the data 16-byte aligned, got strides {st}")
+    return p, sb, st_, sh
+
+
+def _packed4(t):
+    """the same of a contiguous tensor of our own"""
+    _, T, H, d = t.shape
+    return t.data_ptr(), T * H * d, H * d, d
 
 
 def _aux(t, name, dtype, shape, like):
     """device pointer of a contiguous helper tensor next to `like`; None is NULL"""
     if t is None:
         return 0
+    if t.dtype == dtype and t.shape == shape and t.is_contiguous() and t.device == like.device:
+        return t.data_ptr()
     if t.dtype != dtype or t.device != like.device:
         raise TypeError(f"{name}: expected {dtype} on {like.device}, got {t.dtype} on {t.device}")
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}")
-    return t.data_ptr()
+    raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _new(t):
+    """uninitialised, contiguous, of t's shape and type"""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 def _launch(t, call):
@@ -727,20 +737,25 @@ def qk_norm_rope(q, k, q_weight, k_weight, rope=None, positions=None, eps=1e-6, 
     lib = L.load()
     head = _qk_norm_fields(q, k, q_weight, k_weight, rope, positions, eps, interleaved, q_alpha)
     if q_out is None:
-        q_out = q.new_empty(q.shape)
-    qo, ko = _heads4(q_out, "q_out", q, q.shape), _NOWHERE
+        q_out = _new(q)
+        qo = _packed4(q_out)
+    else:
+        qo = _heads4(q_out, "q_out", q, q.shape)
+    ko = _NOWHERE
     if k is not None:
         if k_out is None:
-            k_out = k.new_empty(k.shape)
-        ko = _heads4(k_out, "k_out", q, k.shape)
+            k_out = _new(k)
+            ko = _packed4(k_out)
+        else:
+            ko = _heads4(k_out, "k_out", q, k.shape)
     elif k_out is not None:
         raise ValueError("k_out without k")
-    n = q.numel() + (0 if k is None else k.numel())
-    if n == 0:
+    _, B, T, Hq, Hkv = head[:5]
+    if B * T * (Hq + Hkv) == 0:
         return q_out, k_out
     p = L.QK_NORM_PACK.pack(*head, *qo, *ko, *_NOWHERE, *_NOWHERE, 0, 0, 0, 0)
     if _WORK is not None:
-        _work(K_QK_NORM, n * 4, f"B{head[1]} T{head[2]} h{head[3]}+{head[4]} d{head[5]} rot{head[6]}")
+        _work(K_QK_NORM, B * T * (Hq + Hkv) * head[5] * 4, f"B{head[1]} T{head[2]} h{head[3]}+{head[4]} d{head[5]} rot{head[6]}")
     rc = _launch(q, lambda s: lib.anip_qk_norm_rope(p, s))
     if rc:
         L.check(rc, "anip_qk_norm_rope")
@@ -754,12 +769,12 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, rope=None, p
     lib = L.load()
     head = _qk_norm_fields(q, k, q_weight, k_weight, rope, positions, eps, interleaved, q_alpha)
     gq, gk, ko = _heads4(dq_out, "dq_out", q, q.shape), _NOWHERE, _NOWHERE
-    dq, dk, dwk = q.new_empty(q.shape), None, None
-    dwq = q_weight.new_empty(q_weight.shape)
+    dq, dk, dwk = _new(q), None, None
+    dwq = _new(q_weight)
     if k is not None:
         gk = _heads4(dk_out, "dk_out", q, k.shape)
-        dk, dwk = k.new_empty(k.shape), k_weight.new_empty(k_weight.shape)
-        ko = _heads4(dk, "dk")
+        dk, dwk = _new(k), _new(k_weight)
+        ko = _packed4(dk)
     elif dk_out is not None:
         raise ValueError("dk_out without k")
     n = q.numel() + (0 if k is None else k.numel())
@@ -772,7 +787,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, rope=None, p
     def call(stream):
         need = lib.anip_qk_norm_rope_backward_ws_floats(B * T, Hq, Hkv, d)
         ws = q_weight.new_empty((need,))
-        p = L.QK_NORM_PACK.pack(*head, *_heads4(dq, "dq"), *ko, *gq, *gk, dwq.data_ptr(), _p(dwk), ws.data_ptr(), need)
+        p = L.QK_NORM_PACK.pack(*head, *_packed4(dq), *ko, *gq, *gk, dwq.data_ptr(), _p(dwk), ws.data_ptr(), need)
         return lib.anip_qk_norm_rope_backward(p, stream)
     rc = _launch(q, call)
     if rc:
@@ -848,9 +863,9 @@ def _attention(what, maps, kid, entry, ws_bytes, q, k, v, fields, bias, lam, for
     out = q.new_empty((B, Tq, H, v.shape[3]))
     out2 = lse = None
     if for_backward:
-        out2 = q.new_empty(out.shape) if maps == 2 else None
+        out2 = _new(out) if maps == 2 else None
         lse = q.new_empty((B, H * maps, Tq), dtype=F32)
-    if out.numel() == 0 or Tk == 0:
+    if B * Tq * Tk == 0:
         for t, fill in ((out, 0.0), (out2, 0.0), (lse, -float("inf"))):
             if t is not None:
                 t.fill_(fill)
@@ -882,7 +897,7 @@ def _attention_backward(what, maps, kid, entry, ws_bytes, dout, q, k, v, out, ou
     if 0 in saved[:maps] or not saved[2]:
         if q.numel() and k.numel():
             raise ValueError(f"{what}: out, lse and, for two maps, out2 of the forward are wanted")
-    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    dq, dk, dv = _new(q), _new(k), _new(v)
     if q.numel() == 0 or k.numel() == 0:
         for t in (dq, dk, dv, dlast):
             t.zero_()
@@ -926,7 +941,7 @@ def relative_attention_backward(dout, q, k, v, out, lse, table, buckets, causal=
     lib, what = L.load(), "relative_attention"
     fields = _attn_fields(what, 1, q, k, v, causal, scale, kv_lens, q_start)
     bias = _bias_fields(what, table, buckets, q, fields[4])
-    dtable = table.new_empty(table.shape)
+    dtable = _new(table)
     return _attention_backward(what, 1, K_REL_ATTN, lib.anip_relative_attention_backward, lib.anip_relative_attention_ws_bytes, dout, q, k,
                                v, out, None, lse, fields, bias, 0, dtable, (dtable.data_ptr(), 0))
 
@@ -953,7 +968,7 @@ def differential_attention_backward(dout, q, k, v, out, out2, lse, lam, causal=F
     lib, what = L.load(), "differential_attention"
     fields = _attn_fields(what, 2, q, k, v, causal, scale, kv_lens, q_start)
     lp = _aux(lam, "lam", F32, (fields[4],), q)
-    dlam = lam.new_empty(lam.shape)
+    dlam = _new(lam)
     return _attention_backward(what, 2, K_DIFF_ATTN, lib.anip_differential_attention_backward, lib.anip_differential_attention_ws_bytes,
                                dout, q, k, v, out, out2, lse, fields, _NO_BIAS, lp, dlam, (0, dlam.data_ptr()))
 
