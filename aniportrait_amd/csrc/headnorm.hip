@@ -348,7 +348,9 @@ int bwd_blocks(int64_t items, int L) {
 
 template <typename T, bool INTER>
 int run_fwd(const HeadNormArgs& a, int L, hipStream_t s) {
-  const dim3 grid((unsigned)cdiv64(a.items, 256 / L));
+  const unsigned n = mapattn_grid("head_norm_kernel", cdiv64(a.items, 256 / L), 256);
+  if (!n) return -1;
+  const dim3 grid(n);
   switch (L) {
     case 4: hipLaunchKernelGGL((head_norm_kernel<T, 4, INTER>), grid, dim3(256), 0, s, a); break;
     case 8: hipLaunchKernelGGL((head_norm_kernel<T, 8, INTER>), grid, dim3(256), 0, s, a); break;

@@ -11,6 +11,7 @@ int check(const char* what, const anip_attn_params* p, int maps, bool backward) 
   ANIP_REQUIRE(p->B >= 1 && p->Tq >= 1 && p->Tk >= 1 && p->H >= 1 && p->Hkv >= 1, "%s: sizes must be positive", what);
   ANIP_REQUIRE(p->H % p->Hkv == 0, "%s: %d query heads do not divide into %d key heads", what, p->H, p->Hkv);
   ANIP_REQUIRE(p->Tq <= (1 << 28) && p->Tk <= (1 << 28), "%s: sequences are longer than 2^28", what);
+  ANIP_REQUIRE(p->H <= (1 << 20) && (int64_t)p->B * p->H < (1ll << 31), "%s: too many heads", what);
   const int dmax = maps == 1 ? 160 : 128;
   ANIP_REQUIRE(p->d >= 8 && p->d <= dmax && p->d % 8 == 0, "%s: head width %d: a multiple of 8 up to %d is wanted", what, p->d, dmax);
   ANIP_REQUIRE(p->scale > 0.f && p->scale < 1e30f, "%s: scale must be positive and finite", what);
@@ -25,7 +26,7 @@ int check(const char* what, const anip_attn_params* p, int maps, bool backward) 
     ANIP_REQUIRE(t.s[0] % 8 == 0 && t.s[1] % 8 == 0 && t.s[2] % 8 == 0, "%s: %s: strides must be multiples of 8 elements", what, t.name);
     ANIP_REQUIRE(t.s[1] >= 0 && t.s[1] < (1 << 24), "%s: %s: the distance between tokens must be below 2^24 elements", what, t.name);
   }
-  ANIP_REQUIRE(p->out != nullptr && ((uintptr_t)p->out & 15) == 0, "%s: out must be a 16-byte aligned device pointer", what);
+  ANIP_REQUIRE(p->out != nullptr && (((uintptr_t)p->out | (uintptr_t)p->out2) & 15) == 0, "%s: out and out2 must be 16-byte aligned device pointers", what);
   if (maps == 1) {
     ANIP_REQUIRE(p->table != nullptr && p->buckets != nullptr && p->n_buckets >= 1, "%s: the bias needs its table and the buckets of the relative positions", what);
     ANIP_REQUIRE(p->max_distance >= 0 && p->max_distance <= MAX_R, "%s: relative positions up to %d can be told apart, %d are asked for", what, MAX_R, p->max_distance);
@@ -34,6 +35,7 @@ int check(const char* what, const anip_attn_params* p, int maps, bool backward) 
   }
   if (backward) {
     ANIP_REQUIRE(p->lse != nullptr && p->dq != nullptr && p->dk != nullptr && p->dv != nullptr, "%s: lse, dq, dk and dv are wanted", what);
+    ANIP_REQUIRE((((uintptr_t)p->dq | (uintptr_t)p->dk | (uintptr_t)p->dv) & 15) == 0, "%s: dq, dk and dv must be 16-byte aligned", what);
     ANIP_REQUIRE(maps == 1 ? p->dtable != nullptr : (p->dlam != nullptr && p->out2 != nullptr), "%s: %s wanted", what, maps == 1 ? "dtable is" : "out2 and dlam are");
   }
   return 0;
@@ -58,14 +60,15 @@ MapAttnArgs args(const anip_attn_params* p, int maps) {
 bool few_rows(const anip_attn_params* p) { return (int64_t)p->Tq * (p->H / p->Hkv) <= 32; }
 
 // how the keys are split over workgroups where the queries alone do not fill the chip (256 CUs): towards two workgroups per CU of
-// the 128-query kernel, one of the single-token kernel (its LDS holds one), with four tiles at the least for each
+// the kernel for many queries (8 tiles of 64 keys at the least for each: 4 x 500, 8 heads of 64 take 12.7 us whole, 17.4 in two), and
+// of the single-token kernel (4 of 128)
 int splits_of(const anip_attn_params* p) {
   const bool few = few_rows(p);
   const int64_t blocks = few ? (int64_t)p->B * p->Hkv : (int64_t)((p->Tq + 127) / 128) * p->B * p->H;
   const int64_t tiles = few ? (p->Tk + 127) / 128 : (p->Tk + 63) / 64;
   if (blocks * 2 > 512) return 1;
   int64_t s = 512 / blocks;  // (single tokens, 256 and 1024: 33 and 39 us against 29 at 8 x 16384; 59 and 68 against 59 at 16 x 8192)
-  const int64_t most = tiles / 4;
+  const int64_t most = tiles / (few ? 4 : 8);
   s = s < most ? s : most;
   return (int)(s < 1 ? 1 : (s > 256 ? 256 : s));
 }
@@ -81,7 +84,6 @@ int forward(const char* what, const anip_attn_params* p, int maps, int kid, void
   a.splits = splits_of(p);
   const int64_t need = fwd_ws(p, maps);
   ANIP_REQUIRE(need == 0 || (p->workspace != nullptr && ((uintptr_t)p->workspace & 15) == 0 && p->workspace_bytes >= need), "%s: a workspace of %lld bytes is wanted, 16-byte aligned", what, (long long)need);
-  ANIP_REQUIRE((int64_t)((p->Tq + 63) / 64) * a.splits * p->B * p->H < (1ll << 31) && (int64_t)p->B * p->Tq * p->H * a.dv / 1024 < (1ll << 31), "%s: too many queries for one launch", what);
   if (a.splits > 1) {
     a.part_o = (float*)p->workspace;
     a.part_l = a.part_o + (int64_t)a.splits * p->B * p->Tq * p->H * maps * a.dv;
@@ -104,8 +106,10 @@ int forward(const char* what, const anip_attn_params* p, int maps, int kid, void
 int waves_for(int T) { return T <= 64 ? 1 : 4; }
 
 // Both kernels of the backward walk over tiles of the other side.  The chip holds two workgroups of 4 wave groups per CU (one, with
-// two maps or the widest heads); where there are fewer, the walk is split towards that, with 4 tiles at the least for each part.
+// two maps or the widest heads); where there are fewer, a walk of 12 tiles or more is split towards that, with 4 at the least for each
+// part (whole step at 1 x 1000, 8 heads of 128: 95 us, 114 with 8; at 4 x 500, 8 heads of 64, 8 tiles: 69 split, 62 whole).
 int walk_splits(int64_t blocks, int64_t tiles) {
+  if (tiles < 12) return 1;
   if (blocks < 1) blocks = 1;
   int64_t s = 512 / blocks;
   s = s < tiles / 4 ? s : tiles / 4;
@@ -146,7 +150,6 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   if (rc) return rc;
   const BwdLayout l = layout(p, maps);
   ANIP_REQUIRE(p->workspace != nullptr && ((uintptr_t)p->workspace & 15) == 0 && p->workspace_bytes >= l.total * 4, "%s: a workspace of %lld bytes is wanted, 16-byte aligned", what, (long long)l.total * 4);
-  ANIP_REQUIRE((int64_t)(l.Tp / 32) * l.qsplits * p->B * p->H < (1ll << 31) && (int64_t)((p->Tk + 31) / 32) * l.ksplits * p->B * p->Hkv < (1ll << 31) && (int64_t)p->B * p->Tq * p->H * maps * p->d / 512 < (1ll << 31) && (int64_t)p->B * p->Tk * p->Hkv * maps * p->d / 512 < (1ll << 31), "%s: too many rows for one launch", what);
   ANIP_REQUIRE((int64_t)((p->Tq + 31) / 32) * (p->H / p->Hkv) < (1ll << 31), "%s: too many query tiles", what);
   MapAttnArgs a = args(p, maps);
   a.dout = p->dout, a.do_sb = p->dout_stride[0], a.do_st = p->dout_stride[1], a.do_sh = p->dout_stride[2];

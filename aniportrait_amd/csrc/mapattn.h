@@ -150,6 +150,14 @@ __device__ __forceinline__ void dma4(const void* base, uint32_t bytes, char* lds
 }
 #define MAPATTN_WAIT_DMA() asm volatile("s_waitcnt vmcnt(0)" ::: "memory")
 
+// a barrier for values that cross in LDS: waits for this wave's LDS operations alone.  (__syncthreads also waits for the global
+// operations, and with them for the next tile's DMA.)
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // a tile's way into LDS: piece p (1 KiB = 64 chunks) is fetched by wave p % NW; rows behind the last one and channels behind d
 // arrive as zeros (the buffer descriptor's bound), whatever lies there in memory
 template <int CH, int ROWS, int NW>
@@ -256,6 +264,13 @@ __device__ __forceinline__ bool place(int lin, int slots, int nbh, int& slot, in
 #define MAPATTN_GEOS_2(X) X(2, 2) X(3, 3) X(4, 4) X(5, 5) X(8, 8)
 
 }  // namespace mapattn
+
+// a launch's workgroups, checked against what one launch takes (2^31 of them, 2^32 threads); 0 and the error set otherwise
+static inline unsigned mapattn_grid(const char* name, int64_t blocks, int threads) {
+  if (blocks >= 1 && blocks < (1ll << 31) && blocks * threads < (1ll << 32)) return (unsigned)blocks;
+  anip_set_error("%s: %lld workgroups of %d threads are too many for one launch", name, (long long)blocks, threads);
+  return 0;
+}
 
 int mapattn_forward(const MapAttnArgs& a, int maps, int bf16, hipStream_t s);
 int mapattn_token(const MapAttnArgs& a, int maps, int bf16, hipStream_t s);

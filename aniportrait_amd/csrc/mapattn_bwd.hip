@@ -187,7 +187,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) voi
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, c));
       if (MAPS == 2) {
-        __syncthreads();  // the other half of W is there (the next tile's comes behind its own first barrier)
+        lds_barrier();  // the other half of W is there (the next tile's comes behind its own first barrier)
         if (skip) continue;
         const f32x16 w2 = get16(theirs);
 #pragma unroll
@@ -271,6 +271,10 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) voi
     }
 }
 
+// fragments of a wave's K rows in LDS instead of registers (the widest heads: 477 us against 503 at 2 x 4096 causal, 8 heads of
+// 128 + 128, where 18 registers went to scratch)
+constexpr int dkv_held(int maps, int nt) { return maps * nt >= 16 ? 3 : 0; }
+
 // ---- dK, dV: 32 keys per wave (pair; K and V rows in registers), tiles of QT queries of every head that shares them ------------
 template <typename T, int MAPS, int KS, int NT, int QT, int NG>
 __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 2 : 1)) void mapattn_dkv_kernel(const MapAttnArgs a) {
@@ -301,9 +305,15 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
   const int kw0 = kblk * BK + grp * 32, key = kw0 + kl;
   const bool valid = key < len;
 
+  // the last KL fragments of the K rows wait in LDS where registers are short; in scratch, their loads would wait for the DMA
+  constexpr int KL = dkv_held(MAPS, NT);
+  char* klds = smem + 2 * STAGE + NW * 8192 + wave * (KL * 1024) + lane * 16;
   u32x4 kf[KS], vf[KSV];
   load_row<KS>(kf, (const char*)a.k + 2 * (b * a.k_sb + (int64_t)key * a.k_st + (int64_t)(kvh * MAPS + m) * a.k_sh), valid, h, a.d);
   load_row<KSV, MAPS>(vf, (const char*)a.v + 2 * (b * a.v_sb + (int64_t)key * a.v_st + (int64_t)kvh * a.v_sh), valid, h, a.dv, m);
+
+#pragma unroll
+  for (int i = 0; i < KL; ++i) *(u32x4*)(klds + i * 1024) = kf[KS - KL + i];
 
   // ---- query tiles that meet these keys -----------------------------------------------------------------------------------
   const int nqt = (a.Tq + QT - 1) / QT;
@@ -390,7 +400,8 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
         for (int kk = 0; kk < KSV; ++kk) w = Num<T>::mfma(orr.get(st + MAPS * Q_BYTES, sub, kk), vf[kk], w);
         if (MAPS == 2) put16(mine, w);
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) s = Num<T>::mfma(qr.get(st + m * Q_BYTES, sub, kk), kf[kk], s);
+        for (int kk = 0; kk < KS; ++kk)
+          s = Num<T>::mfma(qr.get(st + m * Q_BYTES, sub, kk), kk < KS - KL ? kf[kk] : lds16(klds + (kk - (KS - KL)) * 1024), s);
       }
       float mul = a.scale_log2, add = 0.f;
       if (BIAS) {
@@ -421,7 +432,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
         for (int i = 0; i < 8; ++i) pv[i >> 2][i & 3] = Num<T>::pack(s[2 * i], s[2 * i + 1]);
       } else {
         if (!skip) put16(mine + 1024, s);
-        __syncthreads();
+        lds_barrier();
         if (skip) continue;
         const float f1 = m == 0 ? 1.f : -lam, f2 = m == 0 ? -lam : 1.f;
 #pragma unroll
@@ -590,7 +601,9 @@ int run_dq(const MapAttnArgs& a, hipStream_t s) {
     anip_set_error("mapattn dq: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
-  hipLaunchKernelGGL((mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG>), dim3((unsigned)(a.Tp / (32 * NG) * a.splits * a.B * a.H)), dim3(64 * NG * MAPS), lds, s, a);
+  const unsigned grid = mapattn_grid("mapattn_dq_kernel", (int64_t)(a.Tp / (32 * NG)) * a.splits * a.B * a.H, 64 * NG * MAPS);
+  if (!grid) return -1;
+  hipLaunchKernelGGL((mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG>), dim3(grid), dim3(64 * NG * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dq_kernel");
   return 0;
 }
@@ -598,13 +611,15 @@ template <typename T, int MAPS, int KS, int NT, int NG>
 int run_dkv(const MapAttnArgs& a, hipStream_t s) {
   constexpr int ROW = 16 * (MAPS * 4 * ((KS + 1) / 2) + 4 * NT);
   constexpr int QT = (MAPS == 2 || NG == 1 || 2 * 64 * ROW > 64 * 1024) ? 32 : 64;
-  const int lds = 2 * (QT * ROW + 2 * MAPS * 256) + (MAPS == 1 ? (2 * (a.R + 32 * NG + QT) + 1) * 4 : 2 * NG * 8192);
+  const int lds = 2 * (QT * ROW + 2 * MAPS * 256) + (MAPS == 1 ? (2 * (a.R + 32 * NG + QT) + 1) * 4 : 2 * NG * (8192 + dkv_held(MAPS, NT) * 1024));
   const void* f = (const void*)mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG>;
   if (anip_raise_lds_limit(f, lds) != 0) {
     anip_set_error("mapattn dkv: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
-  hipLaunchKernelGGL((mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG>), dim3((unsigned)((a.Tk + 32 * NG - 1) / (32 * NG) * a.splits * a.B * a.Hkv)), dim3(64 * NG * MAPS), lds, s, a);
+  const unsigned grid = mapattn_grid("mapattn_dkv_kernel", (int64_t)((a.Tk + 32 * NG - 1) / (32 * NG)) * a.splits * a.B * a.Hkv, 64 * NG * MAPS);
+  if (!grid) return -1;
+  hipLaunchKernelGGL((mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG>), dim3(grid), dim3(64 * NG * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dkv_kernel");
   return 0;
 }
@@ -633,9 +648,10 @@ int dkv_t(const MapAttnArgs& a, int maps, int nw, hipStream_t s) {
 template <bool KV>
 static int join(const MapAttnArgs& a, int bf16, hipStream_t s) {
   if (a.splits == 1) return 0;
-  const dim3 grid((unsigned)cdiv64(KV ? (int64_t)a.B * a.Tk * a.Hkv * (a.dv / 2) : (int64_t)a.B * a.Tq * a.H * (a.dv / 4), 256));
-  if (bf16) hipLaunchKernelGGL((mapattn_join_kernel<bf16_t, KV>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((mapattn_join_kernel<f16, KV>), grid, dim3(256), 0, s, a);
+  const unsigned grid = mapattn_grid("mapattn_join_kernel", cdiv64(KV ? (int64_t)a.B * a.Tk * a.Hkv * (a.dv / 2) : (int64_t)a.B * a.Tq * a.H * (a.dv / 4), 256), 256);
+  if (!grid) return -1;
+  if (bf16) hipLaunchKernelGGL((mapattn_join_kernel<bf16_t, KV>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((mapattn_join_kernel<f16, KV>), dim3(grid), dim3(256), 0, s, a);
   ANIP_LAUNCH_CHECK("mapattn_join_kernel");
   return 0;
 }

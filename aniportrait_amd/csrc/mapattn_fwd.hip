@@ -245,7 +245,7 @@ __global__ __launch_bounds__(64 * MAXT * MAPS, (MAPS == 1 ? 2 : 1)) void mapattn
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int team = wave / MAPS, m = wave % MAPS;
   const int ppb = a.teams / a.kw, kwi = team % a.kw;
-  const int problems = a.B * a.Hkv * a.splits;
+  const int problems = a.B * a.Hkv * a.splits;  // (fewer than 2^31: mapattn_grid)
   const int prob = blockIdx.x * ppb + team / a.kw;
   const bool live = prob < problems;  // (kw = teams: the same for all waves)
   const int split = prob % a.splits, bk = live ? prob / a.splits : 0;
@@ -569,7 +569,9 @@ int run_fwd(const MapAttnArgs& a, hipStream_t s) {
     return -2;
   }
   const int nqb = (a.Tq + 32 * QG - 1) / (32 * QG);
-  hipLaunchKernelGGL((mapattn_fwd_kernel<T, MAPS, KS, NT, KT, NS, QG>), dim3((unsigned)(nqb * a.splits * a.B * a.H)), dim3(64 * QG * MAPS), lds, s, a);
+  const unsigned grid = mapattn_grid("mapattn_fwd_kernel", (int64_t)nqb * a.splits * a.B * a.H, 64 * QG * MAPS);
+  if (!grid) return -1;
+  hipLaunchKernelGGL((mapattn_fwd_kernel<T, MAPS, KS, NT, KT, NS, QG>), dim3(grid), dim3(64 * QG * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_fwd_kernel");
   return 0;
 }
@@ -597,7 +599,9 @@ int run_token(const MapAttnArgs& a0, hipStream_t s) {
     return -2;
   }
   const int ppb = a.teams / a.kw;
-  hipLaunchKernelGGL((mapattn_token_kernel<T, MAPS, KS, NT, MAXT>), dim3((unsigned)((a.B * a.Hkv * a.splits + ppb - 1) / ppb)), dim3(64 * a.teams * MAPS), lds, s, a);
+  const unsigned grid = mapattn_grid("mapattn_token_kernel", cdiv64((int64_t)a.B * a.Hkv * a.splits, ppb), 64 * a.teams * MAPS);
+  if (!grid) return -1;
+  hipLaunchKernelGGL((mapattn_token_kernel<T, MAPS, KS, NT, MAXT>), dim3(grid), dim3(64 * a.teams * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_token_kernel");
   return 0;
 }
@@ -606,8 +610,11 @@ template <typename T, int MAPS, int LR>
 int run_combine_lr(const MapAttnArgs& a, hipStream_t s) {
   // (one part after the other up to 8: 8 us against 13 at 29 688 rows x 2; 64 / LR at once beyond: 9 against 17 at 128 rows x 16)
   const int64_t rows = (int64_t)a.B * a.Tq * a.H;
-  if (a.splits <= 8) hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, true>), dim3((unsigned)cdiv64(rows, 256 / LR)), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, false>), dim3((unsigned)cdiv64(rows, 4)), dim3(256), 0, s, a);
+  const bool few = a.splits <= 8;
+  const unsigned grid = mapattn_grid("mapattn_combine_kernel", cdiv64(rows, few ? 256 / LR : 4), 256);
+  if (!grid) return -1;
+  if (few) hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, true>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, false>), dim3(grid), dim3(256), 0, s, a);
   ANIP_LAUNCH_CHECK("mapattn_combine_kernel");
   return 0;
 }

@@ -60,7 +60,7 @@ def _attn_params(maps, **kw):
 BAD = [dict(dtype=2), dict(B=0), dict(Tq=0), dict(Tk=0), dict(H=3), dict(H=0), dict(Hkv=0), dict(d=0), dict(d=12), dict(d=168), dict(scale=0.0),
        dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=0), dict(k=264), dict(v=0), dict(out=0),
        dict(q_stride=(64 * 256, 252, 64)), dict(k_stride=(64 * 256, 1 << 24, 64)), dict(v_stride=(64 * 256, -256, 64)),
-       dict(Tq=(1 << 28) + 1)]
+       dict(Tq=(1 << 28) + 1), dict(H=1 << 21, Hkv=1 << 21), dict(B=1 << 30), dict(out2=8)]
 
 
 @pytest.mark.parametrize("maps", [1, 2])
@@ -78,7 +78,7 @@ def test_attention_refuses(maps, bad):
 
 
 @pytest.mark.parametrize("maps,bad", [(1, dict(dtable=0)), (2, dict(dlam=0)), (2, dict(out2=0)), (1, dict(lse=0)), (2, dict(dq=0)), (1, dict(dk=0)),
-                                      (1, dict(dv=0)), (2, dict(dout=0)), (1, dict(dout_stride=(8, 4, 8))), (1, {}), (2, dict(workspace=256, workspace_bytes=64))])
+                                      (1, dict(dv=0)), (2, dict(dq=264)), (1, dict(dk=8)), (2, dict(dout=0)), (1, dict(dout_stride=(8, 4, 8))), (1, {}), (2, dict(workspace=256, workspace_bytes=64))])
 def test_attention_backward_refuses(maps, bad):
     """missing outputs, and a workspace that is missing or too small"""
     lib = _ops().L.load()
@@ -223,6 +223,33 @@ def test_qk_norm_rope(B, T, Hq, Hkv, d, rot, inter, far, dtype):
 
 
 @pytest.mark.gpu
+def test_qk_norm_rope_into_a_cache():
+    """new keys written into their place of a longer cache: the rest of it stays"""
+    ops = _ops()
+    q, k, w = rnd(2, 3, 4, 64, dtype=torch.bfloat16, seed=1).to(DEV), rnd(2, 3, 2, 64, dtype=torch.bfloat16, seed=2).to(DEV), torch.ones(64, device=DEV)
+    cache = rnd(2, 50, 2, 64, dtype=torch.bfloat16, seed=3).to(DEV)
+    before = cache.clone()
+    _, want = ops.qk_norm_rope(q, k, w, w)
+    _, got = ops.qk_norm_rope(q, k, w, w, k_out=cache[:, 20:23])
+    assert got.data_ptr() == cache[:, 20:23].data_ptr() and torch.equal(cache[:, 20:23], want)
+    assert torch.equal(cache[:, :20], before[:, :20]) and torch.equal(cache[:, 23:], before[:, 23:])
+
+
+@pytest.mark.gpu
+def test_qk_norm_rope_without_eps():
+    """eps = 0 is a legal value: heads that do not exist in a group add nothing to the weights' gradient"""
+    ops = _ops()
+    q, k = rnd(1, 1000, 9, 64, dtype=torch.float16, seed=1), rnd(1, 1000, 3, 64, dtype=torch.float16, seed=2)
+    w = rnd(64, shift=1.0, scale=0.2, seed=3)
+    gq, gk = rnd(1, 1000, 9, 64, dtype=torch.float16, seed=4), rnd(1, 1000, 3, 64, dtype=torch.float16, seed=5)
+    r = ops.qk_norm_rope_backward(gq.to(DEV), gk.to(DEV), q.to(DEV), k.to(DEV), w.to(DEV), w.to(DEV), eps=0.0)
+    for x, g, dx, dw in ((q, gq, r[0], r[2]), (k, gk, r[1], r[3])):
+        want = O.head_norm(x, w, eps=0.0, dy=g)
+        within(dx, want["dx"], "dx")
+        within(dw, want["dw"], "dw")
+
+
+@pytest.mark.gpu
 def test_qk_norm_rope_gradient_against_differences():
     """the backward's dx along a direction against central differences of the 64-bit forward"""
     ops = _ops()
@@ -313,7 +340,9 @@ SHAPES = [  # (B, Tq, Tk, H, Hkv, d), causal, lens, start
     ((2, 65, 31, 1, 1, 72), False, [-3, 99], [5, -5]),      # lengths outside [0, Tk]
     ((1, 40, 2100, 2, 2, 64), True, None, None),            # keys split over workgroups
     ((2, 1, 3001, 8, 2, 128), True, [3001, 1700], [3000, 1699]),
-    ((1, 257, 257, 1, 1, 120), False, None, None)]
+    ((1, 257, 257, 1, 1, 120), False, None, None),
+    ((1, 900, 900, 4, 1, 64), True, None, None),            # both walks of the backward split
+    ((1, 1000, 40, 2, 2, 128), False, [37], None)]
 
 
 @pytest.mark.gpu
@@ -534,6 +563,28 @@ def test_equal_calls_give_equal_bits_and_graphs_replay():
             torch.cuda.synchronize()
             for a, b in zip(outs[i], eager[src]):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_first_calls_inside_a_capture():
+    """a geometry that no call has launched before is captured and replayed like any other"""
+    ops = _ops()
+    q, k, v, do, _ = _inputs(2, 1, 200, 200, 1, 1, 104, torch.bfloat16, None)
+    q, k, v, do, lam = (t.to(DEV) for t in (q, k, v, do, torch.tensor([0.5])))
+
+    def step():
+        out, out2, lse = ops.differential_attention(q, k, v, lam, causal=True, for_backward=True)
+        return [out, *ops.differential_attention_backward(do, q, k, v, out, out2, lse, lam, causal=True)]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        held = step()
+    for _ in range(3):
+        for t in held:
+            t.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
 
 
 @pytest.mark.gpu
