@@ -246,17 +246,24 @@ __device__ __forceinline__ void fill_near(const MapAttnArgs& a, int h, int E, fl
 }
 
 // block -> (slot among `slots` tiles, (batch, head) among nbh): all tiles of a (batch, head) on one XCD where the heads can be
-// spread evenly over the 8 of them, so that K and V are fetched into one L2 only
-__device__ __forceinline__ bool place(int lin, int slots, int nbh, int& slot, int& bh) {
-  if ((nbh & 7) == 0) {
-    const int x = lin & 7, y = lin >> 3;
-    slot = y % slots;
-    bh = (y / slots) * 8 + x;
+// spread evenly over the 8 of them, so that K and V are fetched into one L2 only.  `falling`: the work falls with the slot
+// (causal).  Then all heads' heaviest tiles come first, and where a CU holds two workgroups (TWO) and gets no more, the second ones
+// in the opposite order: a heavy one beside a light one (2 x 2048, 16 heads of 64: forward 48 -> 40 us, dQ 72 -> 60).
+template <bool TWO>
+__device__ __forceinline__ void place(int lin, int slots, int nbh, bool falling, int& slot, int& bh) {
+  const bool even = (nbh & 7) == 0;
+  const int x = even ? lin & 7 : 0, step = even ? 8 : 1, nb = even ? nbh >> 3 : nbh;
+  int y = even ? lin >> 3 : lin;
+  if (falling) {
+    const int n = slots * nb, cus = even ? 32 : 256;
+    if (TWO && n > cus && n <= 2 * cus && y >= cus) y = n - 1 - (y - cus);
+    slot = y / nb;
+    bh = (y - slot * nb) * step + x;
   } else {
-    slot = lin % slots;
-    bh = lin / slots;
+    bh = y / slots;
+    slot = y - bh * slots;
+    bh = bh * step + x;
   }
-  return bh < nbh;
 }
 
 // (contraction steps over d, 32-channel tiles of V) of the instances; d, dv round up to the next one

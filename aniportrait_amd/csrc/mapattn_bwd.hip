@@ -48,7 +48,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) voi
   float* theirs = (float*)(smem + 2 * STAGE) + (wave ^ 1) * 1024 + lane * 4;
   const int nqb = a.Tp / BQ;
   int qb, bh;
-  if (!place(blockIdx.x, nqb * a.splits, a.B * a.H, qb, bh)) return;
+  place<MAPS == 1>(blockIdx.x, nqb * a.splits, a.B * a.H, a.causal, qb, bh);
   const int split = qb % a.splits;
   qb = nqb - 1 - qb / a.splits;
   const int b = bh / a.H, head = bh - b * a.H, kvh = head / a.G;
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
   float* theirs = (float*)(smem + 2 * STAGE) + (wave ^ 1) * 2048 + lane * 4;
   const int nkb = (a.Tk + BK - 1) / BK;
   int kblk, bk;
-  if (!place(blockIdx.x, nkb * a.splits, a.B * a.Hkv, kblk, bk)) return;  // causal: the first keys meet the most queries
+  place<MAPS == 1 && (KS <= 5)>(blockIdx.x, nkb * a.splits, a.B * a.Hkv, a.causal, kblk, bk);  // causal: the first keys meet the most queries
   const int split = kblk % a.splits;
   kblk /= a.splits;
   const int b = bk / a.Hkv, kvh = bk - b * a.Hkv;

@@ -71,7 +71,7 @@ __global__ __launch_bounds__(64 * QG * MAPS, 2) void mapattn_fwd_kernel(const Ma
   const int grp = wave / MAPS, m = wave % MAPS;  // 32 queries, and the map that this wave computes for them
   const int nqb = (a.Tq + BQ - 1) / BQ;
   int slot, bh;
-  if (!place(blockIdx.x, nqb * a.splits, a.B * a.H, slot, bh)) return;
+  place<MAPS == 1 || (NT < 8)>(blockIdx.x, nqb * a.splits, a.B * a.H, a.causal, slot, bh);
   const int split = slot % a.splits, qb = nqb - 1 - slot / a.splits;  // causal: the longest rows first
   const int b = bh / a.H, head = bh - b * a.H, kvh = head / a.G;
   const int len = seq_len(a, b), start = seq_start(a, b);
