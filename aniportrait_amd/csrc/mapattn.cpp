@@ -130,7 +130,7 @@ BwdLayout layout(const anip_attn_params* p, int maps) {
   l.qsplits = walk_splits((int64_t)l.Tp / 32 * p->B * p->H / 4, (p->Tk + 63) / 64);
   l.ksplits = walk_splits((int64_t)((p->Tk + 31) / 32) * p->B * p->Hkv / 4, (int64_t)((p->Tq + 63) / 64) * (p->H / p->Hkv));
   if (maps == 1) {
-    l.ND = 2 * p->max_distance + 128;
+    l.ND = 2 * p->max_distance + 2 * mapattn::DIAG_PAD;
     const int64_t groups = (int64_t)p->B * l.QW * l.qsplits;
     l.parts = (int)(groups < 32 ? groups : 32);  // few query groups: their own sums are the parts
     l.diag = (int64_t)p->H * groups * (l.ND + 2);

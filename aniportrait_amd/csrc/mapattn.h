@@ -54,6 +54,7 @@ typedef f16 f16x2v __attribute__((ext_vector_type(2)));
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
+constexpr int DIAG_PAD = 96;  // a step of 64 keys x 32 queries that touches (-R, R) reaches less than that beyond
 
 template <typename T>
 struct Num;

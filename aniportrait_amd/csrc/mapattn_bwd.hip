@@ -30,7 +30,7 @@ __device__ __forceinline__ f32x16 get16(const float* x) {
 }
 
 // ---- dQ: 32 queries per wave (pair), tiles of KT keys -----------------------------------------------------------------------
-template <typename T, int MAPS, int KS, int NT, int KT, int NG>
+template <typename T, int MAPS, int KS, int NT, int KT, int NG, int NS>
 __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) void mapattn_dq_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
   constexpr int NW = NG * MAPS, BQ = 32 * NG, DT = (KS + 1) / 2, KSV = MAPS == 1 ? KS : NT;  // KSV: steps over this wave's share of dv
@@ -156,77 +156,97 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) voi
     const bool skip = a.causal && kt0 > pw + 31;
     if (MAPS == 1 && skip) continue;
 #pragma unroll
-    for (int sub = 0; sub < KT / 32; ++sub) {
+    for (int sub = 0; sub < KT / 32; sub += NS) {
       const int k0 = kt0 + 32 * sub;
-      f32x16 s = zero16(), w = zero16();
+      f32x16 s[NS], w[NS];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) s[i] = w[i] = zero16();
       if (MAPS == 1 || !skip) {
 #pragma unroll
-        for (int kk = 0; kk < KSV; ++kk) w = Num<T>::mfma(vr.get(st + MAPS * K_BYTES, sub, kk), df[kk], w);
-        if (MAPS == 2) put16(mine, w);
+        for (int kk = 0; kk < KSV; ++kk)
 #pragma unroll
-        for (int kk = 0; kk < KS; ++kk) s = Num<T>::mfma(kr.get(st + m * K_BYTES, sub, kk), qf[kk], s);
+          for (int i = 0; i < NS; ++i) w[i] = Num<T>::mfma(vr.get(st + MAPS * K_BYTES, sub + i, kk), df[kk], w[i]);
+        if (MAPS == 2) put16(mine, w[0]);
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk)
+#pragma unroll
+          for (int i = 0; i < NS; ++i) s[i] = Num<T>::mfma(kr.get(st + m * K_BYTES, sub + i, kk), qf[kk], s[i]);
       }
       float mul = a.scale_log2, add = 0.f;
-      int zone = 0;  // -1, 1: the whole of these 32 x 32 pairs beyond the bias's reach
+      int zone = 0;  // -1, 1: all of these pairs beyond the bias's reach
       if (BIAS) {
-        if (k0 + 31 - pw <= -a.R) { add = far_lo; zone = -1; }
+        if (k0 + 32 * NS - 1 - pw <= -a.R) { add = far_lo; zone = -1; }
         else if (k0 - (pw + 31) >= a.R) { add = far_hi; zone = 1; }
         else {
           const float* nb = near + (k0 + 4 * h - (pw + ql) + a.R + E);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mul, nb[acc_row(r)]);
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], mul, nb[32 * i + acc_row(r)]);
           mul = 1.f;
         }
       }
-      if (k0 + 31 >= len || (a.causal && k0 + 31 > pw)) {
+      if (k0 + 32 * NS - 1 >= len || (a.causal && k0 + 32 * NS - 1 > pw)) {
         const int dl = lim - k0 - 4 * h;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = acc_row(r) > dl ? -INFINITY : s[r];
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + acc_row(r) > dl ? -INFINITY : s[i][r];
       }
       const float c = add + nl;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], mul, c));
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[i][r] = __builtin_amdgcn_exp2f(fmaf(s[i][r], mul, c));
       if (MAPS == 2) {
         lds_barrier();  // the other half of W is there (the next tile's comes behind its own first barrier)
         if (skip) continue;
         const f32x16 w2 = get16(theirs);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) w[r] += w2[r];
+        for (int r = 0; r < 16; ++r) w[0][r] += w2[r];
         if (m == 1)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) dl_sum = fmaf(s[r], w[r], dl_sum);
+          for (int r = 0; r < 16; ++r) dl_sum = fmaf(s[0][r], w[0][r], dl_sum);
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] *= MAPS == 1 ? w[r] - D : fmaf(w[r], wf, wd);
+      for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[i][r] *= MAPS == 1 ? w[i][r] - D : fmaf(w[i][r], wf, wd);
       if (BIAS) {
         if (zone != 0) {
           float t16 = 0.f;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) t16 += s[r];
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) t16 += s[i][r];
           if (zone < 0) sum_lo += t16;
           else sum_hi += t16;
         } else {
           // value of (key k0 + ko, query ql) belongs to diagonal ko - ql: lane x takes it from lane (ko - x) mod 32 of its half
           open = true;
-          next_base = k0 + 32 - pw;
+          next_base = k0 + 32 * NS - pw;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int ko = acc_row(r) + 4 * h;
-            const float v = __uint_as_float(__builtin_amdgcn_ds_bpermute((((ko - ql) & 31) | (lane & 32)) << 2, __float_as_uint(s[r])));
-            dpos += ql <= ko ? v : 0.f;
-            dneg += ql <= ko ? 0.f : v;
+          for (int i = 0; i < NS; ++i) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int ko = acc_row(r) + 4 * h;
+              const float v = __uint_as_float(__builtin_amdgcn_ds_bpermute((((ko - ql) & 31) | (lane & 32)) << 2, __float_as_uint(s[i][r])));
+              dpos += ql <= ko ? v : 0.f;
+              dneg += ql <= ko ? 0.f : v;
+            }
+            const float done = xor32_sum(dneg);  // no later key reaches these 32 diagonals
+            if (diag && h == 0) diag[k0 + 32 * i - pw - 32 + ql + a.R + DIAG_PAD] = done;
+            dneg = dpos;
+            dpos = 0.f;
           }
-          const float done = xor32_sum(dneg);  // no later key reaches these 32 diagonals
-          if (diag && h == 0) diag[k0 - pw - 32 + ql + a.R + 64] = done;
-          dneg = dpos;
-          dpos = 0.f;
         }
       }
 #pragma unroll
-      for (int kb2 = 0; kb2 < 2; ++kb2) {
+      for (int kb2 = 0; kb2 < 2 * NS; ++kb2) {
+        const f32x16& x = s[kb2 >> 1];
         u32x4 p;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = Num<T>::pack(s[8 * kb2 + 2 * i], s[8 * kb2 + 2 * i + 1]);
+        for (int i = 0; i < 4; ++i) p[i] = Num<T>::pack(x[8 * (kb2 & 1) + 2 * i], x[8 * (kb2 & 1) + 2 * i + 1]);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) dq[dt] = Num<T>::mfma(kt.get(st + m * K_BYTES, 2 * sub + kb2, dt), p, dq[dt]);
       }
@@ -235,7 +255,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) voi
 
   if (BIAS && diag) {
     const float done = xor32_sum(dneg);
-    if (open && h == 0) diag[next_base - 32 + ql + a.R + 64] = done;
+    if (open && h == 0) diag[next_base - 32 + ql + a.R + DIAG_PAD] = done;
     const float lo = wave_sum(sum_lo), hi = wave_sum(sum_hi);
     if (lane == 0) {
       diag[a.ND] = lo;
@@ -276,7 +296,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) voi
 constexpr int dkv_held(int maps, int nt) { return maps * nt >= 16 ? 3 : 0; }
 
 // ---- dK, dV: 32 keys per wave (pair; K and V rows in registers), tiles of QT queries of every head that shares them ------------
-template <typename T, int MAPS, int KS, int NT, int QT, int NG>
+template <typename T, int MAPS, int KS, int NT, int QT, int NG, int NS>
 __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 2 : 1)) void mapattn_dkv_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
   constexpr int NW = NG * MAPS, BK = 32 * NG, DT = (KS + 1) / 2;
@@ -392,46 +412,60 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
     const bool skip = a.causal && pt + QT - 1 < kw0;  // no query of the tile sees this wave's keys
     if (MAPS == 1 && skip) continue;
 #pragma unroll
-    for (int sub = 0; sub < QT / 32; ++sub) {
+    for (int sub = 0; sub < QT / 32; sub += NS) {
       const int pq = pt + 32 * sub;
-      f32x16 s = zero16(), w = zero16();
+      f32x16 s[NS], w[NS];
+#pragma unroll
+      for (int i = 0; i < NS; ++i) s[i] = w[i] = zero16();
       if (MAPS == 1 || !skip) {
 #pragma unroll
-        for (int kk = 0; kk < KSV; ++kk) w = Num<T>::mfma(orr.get(st + MAPS * Q_BYTES, sub, kk), vf[kk], w);
-        if (MAPS == 2) put16(mine, w);
+        for (int kk = 0; kk < KSV; ++kk)
+#pragma unroll
+          for (int i = 0; i < NS; ++i) w[i] = Num<T>::mfma(orr.get(st + MAPS * Q_BYTES, sub + i, kk), vf[kk], w[i]);
+        if (MAPS == 2) put16(mine, w[0]);
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk)
-          s = Num<T>::mfma(qr.get(st + m * Q_BYTES, sub, kk), kk < KS - KL ? kf[kk] : lds16(klds + (kk - (KS - KL)) * 1024), s);
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+            s[i] = Num<T>::mfma(qr.get(st + m * Q_BYTES, sub + i, kk), kk < KS - KL ? kf[kk] : lds16(klds + (kk - (KS - KL)) * 1024), s[i]);
       }
       float mul = a.scale_log2, add = 0.f;
       if (BIAS) {
         if (kw0 + 31 - pq <= -a.R) add = far_lo;
-        else if (kw0 - (pq + 31) >= a.R) add = far_hi;
+        else if (kw0 - (pq + 32 * NS - 1) >= a.R) add = far_hi;
         else {
           const float* nb = near + (key - pq - 4 * h + a.R + E);
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fmaf(s[r], mul, nb[-acc_row(r)]);
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[i][r] = fmaf(s[i][r], mul, nb[-32 * i - acc_row(r)]);
           mul = 1.f;
         }
       }
       if (kw0 + 31 >= len || (a.causal && kw0 + 31 > pq)) {
-        const int dl = !valid ? 64 : (a.causal ? key - pq - 4 * h : -64);  // rows before dl do not see this lane's key
+        const int dl = !valid ? 128 : (a.causal ? key - pq - 4 * h : -128);  // rows before dl do not see this lane's key
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = acc_row(r) < dl ? -INFINITY : s[r];
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[i][r] = 32 * i + acc_row(r) < dl ? -INFINITY : s[i][r];
       }
       // P' = 2^PSH P; rows_lse and rows_d carry 2^PSH and 2^-PSH
 #pragma unroll
-      for (int rq = 0; rq < 4; ++rq) {
-        const f32x4 nl = *(const f32x4*)(rt + m * R_BYTES + (32 * sub + 8 * rq + 4 * h) * 4);
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[4 * rq + e] = __builtin_amdgcn_exp2f(fmaf(s[4 * rq + e], mul, nl[e] + add));
-      }
-      u32x4 pv[2];  // what meets dO in dV
+        for (int rq = 0; rq < 4; ++rq) {
+          const f32x4 nl = *(const f32x4*)(rt + m * R_BYTES + (32 * (sub + i) + 8 * rq + 4 * h) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[i][4 * rq + e] = __builtin_amdgcn_exp2f(fmaf(s[i][4 * rq + e], mul, nl[e] + add));
+        }
+      u32x4 pv[NS][2];  // what meets dO in dV
       if (MAPS == 1) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) pv[i >> 2][i & 3] = Num<T>::pack(s[2 * i], s[2 * i + 1]);
+        for (int j = 0; j < NS; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) pv[j][i >> 2][i & 3] = Num<T>::pack(s[j][2 * i], s[j][2 * i + 1]);
       } else {
-        if (!skip) put16(mine + 1024, s);
+        if (!skip) put16(mine + 1024, s[0]);
         lds_barrier();
         if (skip) continue;
         const float f1 = m == 0 ? 1.f : -lam, f2 = m == 0 ? -lam : 1.f;
@@ -441,33 +475,36 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
           float pc[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            w[4 * i + e] += w2[e];
-            pc[e] = fmaf(f1, s[4 * i + e], f2 * p2[e]);
+            w[0][4 * i + e] += w2[e];
+            pc[e] = fmaf(f1, s[0][4 * i + e], f2 * p2[e]);
           }
-          pv[i >> 1][2 * (i & 1)] = Num<T>::pack(pc[0], pc[1]);
-          pv[i >> 1][2 * (i & 1) + 1] = Num<T>::pack(pc[2], pc[3]);
+          pv[0][i >> 1][2 * (i & 1)] = Num<T>::pack(pc[0], pc[1]);
+          pv[0][i >> 1][2 * (i & 1) + 1] = Num<T>::pack(pc[2], pc[3]);
         }
       }
 #pragma unroll
-      for (int kb2 = 0; kb2 < 2; ++kb2)
+      for (int kb2 = 0; kb2 < 2 * NS; ++kb2)
 #pragma unroll
         for (int nt = 0; nt < VT; ++nt)
-          if (MAPS == 1 || NT % 2 == 0 || m * VT + nt < NT) dv[nt] = Num<T>::mfma(ot.get(st + MAPS * Q_BYTES, 2 * sub + kb2, nt), pv[kb2], dv[nt]);
+          if (MAPS == 1 || NT % 2 == 0 || m * VT + nt < NT) dv[nt] = Num<T>::mfma(ot.get(st + MAPS * Q_BYTES, 2 * sub + kb2, nt), pv[kb2 >> 1][kb2 & 1], dv[nt]);
       const float wf = m == 0 ? PF : -lam * PF, wd = m == 0 ? -1.f : lam;
 #pragma unroll
-      for (int rq = 0; rq < 4; ++rq) {
-        const f32x4 D = *(const f32x4*)(rt + (MAPS + m) * R_BYTES + (32 * sub + 8 * rq + 4 * h) * 4);
+      for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * rq + e;
-          s[r] *= MAPS == 1 ? fmaf(w[r], PF, -D[e]) : fmaf(w[r], wf, wd * D[e]);
+        for (int rq = 0; rq < 4; ++rq) {
+          const f32x4 D = *(const f32x4*)(rt + (MAPS + m) * R_BYTES + (32 * (sub + i) + 8 * rq + 4 * h) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * rq + e;
+            s[i][r] *= MAPS == 1 ? fmaf(w[i][r], PF, -D[e]) : fmaf(w[i][r], wf, wd * D[e]);
+          }
         }
-      }
 #pragma unroll
-      for (int kb2 = 0; kb2 < 2; ++kb2) {
+      for (int kb2 = 0; kb2 < 2 * NS; ++kb2) {
+        const f32x16& x = s[kb2 >> 1];
         u32x4 p;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = Num<T>::pack(s[8 * kb2 + 2 * i], s[8 * kb2 + 2 * i + 1]);
+        for (int i = 0; i < 4; ++i) p[i] = Num<T>::pack(x[8 * (kb2 & 1) + 2 * i], x[8 * (kb2 & 1) + 2 * i + 1]);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) dk[dt] = Num<T>::mfma(qt.get(st + m * Q_BYTES, 2 * sub + kb2, dt), p, dk[dt]);
       }
@@ -566,11 +603,11 @@ __global__ __launch_bounds__(1024) void mapattn_dtable_kernel(const MapAttnArgs 
   __syncthreads();
   for (int c = threadIdx.x >> 6; c < a.NB; c += 16) {
     float t = 0.f;
-    for (int x = lane; x < a.ND; x += 64) {  // slot x: relative position x - R - 64, beyond +-R as +-R
-      const int r = x < 64 ? 0 : (x > 2 * a.R + 64 ? 2 * a.R : x - 64);
+    for (int x = lane; x < a.ND; x += 64) {  // slot x: relative position x - R - DIAG_PAD, beyond +-R as +-R
+      const int r = x < DIAG_PAD ? 0 : (x > 2 * a.R + DIAG_PAD ? 2 * a.R : x - DIAG_PAD);
       int bx = a.buckets[r];
       bx = bx < 0 ? 0 : (bx >= a.NB ? a.NB - 1 : bx);
-      if (bx == c) t += sums[x] + (x == 64 ? sums[a.ND] : 0.f) + (x == 2 * a.R + 64 ? sums[a.ND + 1] : 0.f);
+      if (bx == c) t += sums[x] + (x == DIAG_PAD ? sums[a.ND] : 0.f) + (x == 2 * a.R + DIAG_PAD ? sums[a.ND + 1] : 0.f);
     }
     t = wave_sum(t);
     if (lane == 0) ((T*)a.dtable)[(int64_t)head * a.NB + c] = (T)t;
@@ -595,15 +632,18 @@ template <typename T, int MAPS, int KS, int NT, int NG>
 int run_dq(const MapAttnArgs& a, hipStream_t s) {
   constexpr int ROW = 16 * (MAPS * 4 * ((KS + 1) / 2) + 4 * NT);
   constexpr int KT = (MAPS == 2 || NG == 1 || 2 * 64 * ROW > 64 * 1024) ? 32 : 64;
+  // two sub-tiles of 32 at once where the registers allow two waves per SIMD all the same: two chains of products beside each other
+  // (2 x 2048, 16 / 4 heads of 64: 54 us against 59, the keys' kernel 63 against 70; heads of 80: no difference)
+  constexpr int NS = (KT == 64 && KS <= 4) ? 2 : 1;
   const int lds = 2 * KT * ROW + (MAPS == 1 ? (2 * (a.R + 32 * NG + KT) + 1) * 4 : 2 * NG * 4096);
-  const void* f = (const void*)mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG>;
+  const void* f = (const void*)mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG, NS>;
   if (anip_raise_lds_limit(f, lds) != 0) {
     anip_set_error("mapattn dq: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
   const unsigned grid = mapattn_grid("mapattn_dq_kernel", (int64_t)(a.Tp / (32 * NG)) * a.splits * a.B * a.H, 64 * NG * MAPS);
   if (!grid) return -1;
-  hipLaunchKernelGGL((mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG>), dim3(grid), dim3(64 * NG * MAPS), lds, s, a);
+  hipLaunchKernelGGL((mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG, NS>), dim3(grid), dim3(64 * NG * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dq_kernel");
   return 0;
 }
@@ -611,15 +651,16 @@ template <typename T, int MAPS, int KS, int NT, int NG>
 int run_dkv(const MapAttnArgs& a, hipStream_t s) {
   constexpr int ROW = 16 * (MAPS * 4 * ((KS + 1) / 2) + 4 * NT);
   constexpr int QT = (MAPS == 2 || NG == 1 || 2 * 64 * ROW > 64 * 1024) ? 32 : 64;
+  constexpr int NS = (QT == 64 && KS <= 4) ? 2 : 1;  // (see run_dq)
   const int lds = 2 * (QT * ROW + 2 * MAPS * 256) + (MAPS == 1 ? (2 * (a.R + 32 * NG + QT) + 1) * 4 : 2 * NG * (8192 + dkv_held(MAPS, NT) * 1024));
-  const void* f = (const void*)mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG>;
+  const void* f = (const void*)mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG, NS>;
   if (anip_raise_lds_limit(f, lds) != 0) {
     anip_set_error("mapattn dkv: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
   const unsigned grid = mapattn_grid("mapattn_dkv_kernel", (int64_t)((a.Tk + 32 * NG - 1) / (32 * NG)) * a.splits * a.B * a.Hkv, 64 * NG * MAPS);
   if (!grid) return -1;
-  hipLaunchKernelGGL((mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG>), dim3(grid), dim3(64 * NG * MAPS), lds, s, a);
+  hipLaunchKernelGGL((mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG, NS>), dim3(grid), dim3(64 * NG * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dkv_kernel");
   return 0;
 }
