@@ -118,7 +118,7 @@ int walk_splits(int64_t blocks, int64_t tiles) {
 
 struct BwdLayout {
   int nwq, nwk, Tp, QW, ND, parts, qsplits, ksplits;
-  int64_t rows, diag, dlam, part, dkv, dq, total;  // floats; the parts of dq and dkv share their place
+  int64_t rows, diag, dlam, part, dkv, dq, total;  // floats
 };
 BwdLayout layout(const anip_attn_params* p, int maps) {
   BwdLayout l{};
@@ -140,8 +140,7 @@ BwdLayout layout(const anip_attn_params* p, int maps) {
   }
   if (l.qsplits > 1) l.dq = (int64_t)l.qsplits * p->B * p->Tq * p->H * maps * p->d;
   if (l.ksplits > 1) l.dkv = (int64_t)l.ksplits * p->B * p->Tk * p->Hkv * 2 * maps * p->d;
-  l.dkv = l.dkv > l.dq ? l.dkv : l.dq;
-  l.total = l.dkv + 2 * l.rows + l.diag + l.part + l.dlam;
+  l.total = l.dq + l.dkv + 2 * l.rows + l.diag + l.part + l.dlam;
   return l;
 }
 
@@ -155,7 +154,8 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   a.dout = p->dout, a.do_sb = p->dout_stride[0], a.do_st = p->dout_stride[1], a.do_sh = p->dout_stride[2];
   a.dq = p->dq, a.dk = p->dk, a.dvo = p->dv, a.dtable = p->dtable, a.dlam = p->dlam;
   a.Tp = l.Tp, a.QW = l.QW, a.ND = l.ND, a.parts = l.parts;
-  a.part_o = (float*)p->workspace;
+  a.part_q = (float*)p->workspace;
+  a.part_o = a.part_q + l.dq;
   a.rows_lse = a.part_o + l.dkv;
   a.rows_d = a.rows_lse + l.rows;
   a.diag = a.rows_d + l.rows;
@@ -163,9 +163,8 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   a.dlam_part = a.diag + l.diag + l.part;
   hipStream_t s = (hipStream_t)stream;
   AnipProfScope prof_(kid, stream);
-  a.splits = l.qsplits;
+  a.splits = a.qsplits = l.qsplits;
   int r = mapattn_dq(a, maps, p->dtype, l.nwq, s);
-  if (!r) r = mapattn_reduce(a, maps, p->dtype, s);
   a.splits = l.ksplits;
   if (!r) r = mapattn_dkv(a, maps, p->dtype, l.nwk, s);
   return r;

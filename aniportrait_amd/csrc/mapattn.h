@@ -42,6 +42,10 @@ struct MapAttnArgs {
   float* dlam_part;   // [h][b][group]
   float* diag_part;   // [h][parts][ND + 2]
   int parts;
+  // ahead of the keys' kernel, in its launch: workgroups that add the parts of dtable / dlam, and those of a split dQ
+  int qsplits;        // parts of the queries' kernel
+  float* part_q;
+  int sum_blocks, join_blocks;
 };
 
 namespace mapattn {
@@ -285,4 +289,3 @@ int mapattn_token(const MapAttnArgs& a, int maps, int bf16, hipStream_t s);
 int mapattn_combine(const MapAttnArgs& a, int maps, int bf16, hipStream_t s);
 int mapattn_dq(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s);
 int mapattn_dkv(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s);
-int mapattn_reduce(const MapAttnArgs& a, int maps, int bf16, hipStream_t s);

@@ -268,7 +268,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) voi
   }
   if (!valid) return;
   if (a.splits > 1) {
-    float* pp = a.part_o + (((int64_t)split * a.B * a.Tq + (int64_t)b * a.Tq + qi) * a.H * MAPS + head * MAPS + m) * a.d;
+    float* pp = a.part_q + (((int64_t)split * a.B * a.Tq + (int64_t)b * a.Tq + qi) * a.H * MAPS + head * MAPS + m) * a.d;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -289,6 +289,63 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) voi
       if (c0 < a.d)
         *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale), Num<T>::pack(x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale)};
     }
+}
+
+// ---- sums of parts, in a fixed order ----------------------------------------------------------------------------------------
+// The queries' kernel leaves sums for each 32 queries (dtable's diagonals, dlam) and, split, dQ in parts.  They are added by the
+// first workgroups of the keys' launch, beside its own work; dtable of many groups by two kernels of its own.
+
+// four channels of a gradient from the 32-bit parts of a split walk, `n` values apart
+__device__ __forceinline__ f32x4 add_parts(const float* p, int parts, int64_t n) {
+  f32x4 t = *(const f32x4*)p;
+#pragma unroll 4
+  for (int s = 1; s < parts; ++s) t += *(const f32x4*)(p + s * n);
+  return t;
+}
+template <typename T>
+__device__ __forceinline__ void join_dq(const MapAttnArgs& a, int block) {
+  const int64_t n = (int64_t)a.B * a.Tq * a.H * a.dv, i = ((int64_t)block * blockDim.x + threadIdx.x) * 4;
+  if (i >= n) return;
+  const f32x4 t = add_parts(a.part_q + i, a.qsplits, n);
+  *(u32x2*)((char*)a.dq + i * 2) = u32x2{Num<T>::pack(t[0], t[1]), Num<T>::pack(t[2], t[3])};
+}
+// a head's bucket sums from `parts` rows of diagonals: the rows added per slot, then a wave per bucket adds the slots that belong to it
+template <typename T>
+__device__ __forceinline__ void sum_table(const MapAttnArgs& a, int head, const float* rows, int parts, float* sums) {
+  const int n = a.ND + 2, lane = threadIdx.x & 63;
+  const float* p = rows + (int64_t)head * parts * n;
+  for (int x = threadIdx.x; x < n; x += blockDim.x) {
+    float t = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) t += p[(int64_t)i * n + x];
+    sums[x] = t;
+  }
+  __syncthreads();
+  for (int c = threadIdx.x >> 6; c < a.NB; c += blockDim.x >> 6) {
+    float t = 0.f;
+    for (int x = lane; x < a.ND; x += 64) {  // slot x: relative position x - R - DIAG_PAD, beyond +-R as +-R
+      const int r = x < DIAG_PAD ? 0 : (x > 2 * a.R + DIAG_PAD ? 2 * a.R : x - DIAG_PAD);
+      int bx = a.buckets[r];
+      bx = bx < 0 ? 0 : (bx >= a.NB ? a.NB - 1 : bx);
+      if (bx == c) t += sums[x] + (x == DIAG_PAD ? sums[a.ND] : 0.f) + (x == 2 * a.R + DIAG_PAD ? sums[a.ND + 1] : 0.f);
+    }
+    t = wave_sum(t);
+    if (lane == 0) ((T*)a.dtable)[(int64_t)head * a.NB + c] = (T)t;
+  }
+}
+__device__ __forceinline__ void sum_lam(const MapAttnArgs& a, int head, float* sums) {
+  const int64_t rows = (int64_t)a.B * a.QW * a.qsplits;
+  const float* p = a.dlam_part + head * rows;
+  float t = 0.f;
+  for (int64_t r = threadIdx.x; r < rows; r += blockDim.x) t += p[r];
+  t = wave_sum(t);
+  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = t;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    t = 0.f;
+    for (int w = 0; w < (int)blockDim.x >> 6; ++w) t += sums[w];
+    a.dlam[head] = t;
+  }
 }
 
 // fragments of a wave's K rows in LDS instead of registers (the widest heads: 477 us against 503 at 2 x 4096 causal, 8 heads of
@@ -316,8 +373,17 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
   float* mine = (float*)(smem + 2 * STAGE) + wave * 2048 + lane * 4;         // (two maps) 16 values of W, 16 of P of each lane
   float* theirs = (float*)(smem + 2 * STAGE) + (wave ^ 1) * 2048 + lane * 4;
   const int nkb = (a.Tk + BK - 1) / BK;
+  int lin = blockIdx.x;
+  if (lin < a.sum_blocks) {
+    if (MAPS == 1) sum_table<T>(a, lin, a.diag, a.B * a.QW * a.qsplits, (float*)smem);
+    else sum_lam(a, lin, (float*)smem);
+    return;
+  }
+  lin -= a.sum_blocks;
+  if (lin < a.join_blocks) return join_dq<T>(a, lin);
+  lin -= a.join_blocks;
   int kblk, bk;
-  place<MAPS == 1 && (KS <= 5)>(blockIdx.x, nkb * a.splits, a.B * a.Hkv, a.causal, kblk, bk);  // causal: the first keys meet the most queries
+  place<MAPS == 1 && (KS <= 5)>(lin, nkb * a.splits, a.B * a.Hkv, a.causal, kblk, bk);  // causal: the first keys meet the most queries
   const int split = kblk % a.splits;
   kblk /= a.splits;
   const int b = bk / a.Hkv, kvh = bk - b * a.Hkv;
@@ -555,74 +621,35 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
     }
 }
 
-// gradients from the 32-bit parts of a split walk, the parts in their order, one thread per 4 channels: rows of `a.dv` channels of
-// dK and as many of dV (KV), or rows of dQ
-template <typename T, bool KV>
+// dK, dV from the parts of a split walk: one thread per 4 channels
+template <typename T>
 __global__ __launch_bounds__(256) void mapattn_join_kernel(const MapAttnArgs a) {
-  const int64_t rows = KV ? (int64_t)a.B * a.Tk * a.Hkv : (int64_t)a.B * a.Tq * a.H;
-  const int qn = KV ? a.dv / 2 : a.dv / 4;
+  const int64_t rows = (int64_t)a.B * a.Tk * a.Hkv;
+  const int qn = a.dv / 2;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= rows * qn) return;
-  const float* p = a.part_o + i * 4;
-  f32x4 t = *(const f32x4*)p;
-#pragma unroll 4
-  for (int s = 1; s < a.splits; ++s) t += *(const f32x4*)(p + s * rows * qn * 4);
-  if (!KV) {
-    *(u32x2*)((char*)a.dq + i * 8) = u32x2{Num<T>::pack(t[0], t[1]), Num<T>::pack(t[2], t[3])};
-    return;
-  }
+  const f32x4 t = add_parts(a.part_o + i * 4, a.splits, rows * qn * 4);
   const int64_t row = i / qn;
   const int c0 = (int)(i - row * qn) * 4;
   char* op = c0 < a.dv ? (char*)a.dk + (row * a.dv + c0) * 2 : (char*)a.dvo + (row * a.dv + c0 - a.dv) * 2;
   *(u32x2*)op = u32x2{Num<T>::pack(t[0], t[1]), Num<T>::pack(t[2], t[3])};
 }
 
-// ---- sums of the query groups' parts, in a fixed order --------------------------------------------------------------------
-// part sums of dtable's diagonals: block (slots, part, head), one thread per slot
+// dtable of many query groups: part sums of the diagonals, block (slots, part, head), one thread per slot; then a workgroup per head
 __global__ __launch_bounds__(256) void mapattn_diag_kernel(const MapAttnArgs a) {
   const int slot = blockIdx.x * 256 + threadIdx.x, part = blockIdx.y, head = blockIdx.z;
   if (slot >= a.ND + 2) return;
-  const int64_t rows = (int64_t)a.B * a.QW * a.splits, r0 = rows * part / a.parts, r1 = rows * (part + 1) / a.parts;
+  const int64_t rows = (int64_t)a.B * a.QW * a.qsplits, r0 = rows * part / a.parts, r1 = rows * (part + 1) / a.parts;
   const float* p = a.diag + ((int64_t)head * rows) * (a.ND + 2) + slot;
   float t = 0.f;
 #pragma unroll 8
   for (int64_t r = r0; r < r1; ++r) t += p[r * (a.ND + 2)];
   a.diag_part[((int64_t)head * a.parts + part) * (a.ND + 2) + slot] = t;
 }
-// a head's bucket sums: the parts added per slot, then a wave per bucket adds the slots that belong to it
 template <typename T>
 __global__ __launch_bounds__(1024) void mapattn_dtable_kernel(const MapAttnArgs a) {
   extern __shared__ float sums[];
-  const int head = blockIdx.x, n = a.ND + 2, lane = threadIdx.x & 63;
-  for (int x = threadIdx.x; x < n; x += 1024) {
-    float t = 0.f;
-#pragma unroll 8
-    for (int p = 0; p < a.parts; ++p) t += a.diag_part[((int64_t)head * a.parts + p) * n + x];
-    sums[x] = t;
-  }
-  __syncthreads();
-  for (int c = threadIdx.x >> 6; c < a.NB; c += 16) {
-    float t = 0.f;
-    for (int x = lane; x < a.ND; x += 64) {  // slot x: relative position x - R - DIAG_PAD, beyond +-R as +-R
-      const int r = x < DIAG_PAD ? 0 : (x > 2 * a.R + DIAG_PAD ? 2 * a.R : x - DIAG_PAD);
-      int bx = a.buckets[r];
-      bx = bx < 0 ? 0 : (bx >= a.NB ? a.NB - 1 : bx);
-      if (bx == c) t += sums[x] + (x == DIAG_PAD ? sums[a.ND] : 0.f) + (x == 2 * a.R + DIAG_PAD ? sums[a.ND + 1] : 0.f);
-    }
-    t = wave_sum(t);
-    if (lane == 0) ((T*)a.dtable)[(int64_t)head * a.NB + c] = (T)t;
-  }
-}
-__global__ __launch_bounds__(256) void mapattn_dlam_kernel(const MapAttnArgs a) {
-  __shared__ float part[4];
-  const int64_t rows = (int64_t)a.B * a.QW * a.splits;
-  const float* p = a.dlam_part + blockIdx.x * rows;
-  float t = 0.f;
-  for (int64_t r = threadIdx.x; r < rows; r += 256) t += p[r];
-  t = wave_sum(t);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = t;
-  __syncthreads();
-  if (threadIdx.x == 0) a.dlam[blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+  sum_table<T>(a, blockIdx.x, a.diag_part, a.parts, sums);
 }
 
 // ---- dispatch -----------------------------------------------------------------------------------------------------------
@@ -647,8 +674,21 @@ int run_dq(const MapAttnArgs& a, hipStream_t s) {
   ANIP_LAUNCH_CHECK("mapattn_dq_kernel");
   return 0;
 }
+template <typename T>
+int table_sums(const MapAttnArgs& a, hipStream_t s) {
+  const int lds = (a.ND + 2) * 4;
+  if (a.diag_part != a.diag) {
+    hipLaunchKernelGGL(mapattn_diag_kernel, dim3((unsigned)((a.ND + 2 + 255) / 256), (unsigned)a.parts, (unsigned)a.H), dim3(256), 0, s, a);
+    ANIP_LAUNCH_CHECK("mapattn_diag_kernel");
+  }
+  hipLaunchKernelGGL((mapattn_dtable_kernel<T>), dim3((unsigned)a.H), dim3(1024), lds, s, a);
+  ANIP_LAUNCH_CHECK("mapattn_dtable_kernel");
+  return 0;
+}
+
 template <typename T, int MAPS, int KS, int NT, int NG>
-int run_dkv(const MapAttnArgs& a, hipStream_t s) {
+int run_dkv(const MapAttnArgs& a0, hipStream_t s) {
+  MapAttnArgs a = a0;
   constexpr int ROW = 16 * (MAPS * 4 * ((KS + 1) / 2) + 4 * NT);
   constexpr int QT = (MAPS == 2 || NG == 1 || 2 * 64 * ROW > 64 * 1024) ? 32 : 64;
   constexpr int NS = (QT == 64 && KS <= 4) ? 2 : 1;  // (see run_dq)
@@ -658,8 +698,17 @@ int run_dkv(const MapAttnArgs& a, hipStream_t s) {
     anip_set_error("mapattn dkv: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
-  const unsigned grid = mapattn_grid("mapattn_dkv_kernel", (int64_t)((a.Tk + 32 * NG - 1) / (32 * NG)) * a.splits * a.B * a.Hkv, 64 * NG * MAPS);
+  // sums beside the keys' work: dlam always, dtable up to 512 loads for a thread (2 x 2048, 16 heads: 11 us of two kernels saved)
+  const int64_t groups = (int64_t)a.B * a.QW * a.qsplits;
+  a.sum_blocks = MAPS == 2 || groups * ((a.ND + 2 + 64 * NG - 1) / (64 * NG)) <= 512 ? a.H : 0;
+  if (!a.sum_blocks) {
+    const int r = table_sums<T>(a, s);
+    if (r) return r;
+  }
+  const int64_t joins = a.qsplits > 1 ? cdiv64((int64_t)a.B * a.Tq * a.H * (a.dv / 4), 64 * NG * MAPS) : 0;
+  const unsigned grid = mapattn_grid("mapattn_dkv_kernel", (int64_t)((a.Tk + 32 * NG - 1) / (32 * NG)) * a.splits * a.B * a.Hkv + a.sum_blocks + joins, 64 * NG * MAPS);
   if (!grid) return -1;
+  a.join_blocks = (int)joins;
   hipLaunchKernelGGL((mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG, NS>), dim3(grid), dim3(64 * NG * MAPS), lds, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dkv_kernel");
   return 0;
@@ -686,37 +735,14 @@ int dkv_t(const MapAttnArgs& a, int maps, int nw, hipStream_t s) {
 
 }  // namespace
 
-template <bool KV>
-static int join(const MapAttnArgs& a, int bf16, hipStream_t s) {
-  if (a.splits == 1) return 0;
-  const unsigned grid = mapattn_grid("mapattn_join_kernel", cdiv64(KV ? (int64_t)a.B * a.Tk * a.Hkv * (a.dv / 2) : (int64_t)a.B * a.Tq * a.H * (a.dv / 4), 256), 256);
-  if (!grid) return -1;
-  if (bf16) hipLaunchKernelGGL((mapattn_join_kernel<bf16_t, KV>), dim3(grid), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((mapattn_join_kernel<f16, KV>), dim3(grid), dim3(256), 0, s, a);
-  ANIP_LAUNCH_CHECK("mapattn_join_kernel");
-  return 0;
-}
-int mapattn_dq(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) {
-  const int r = bf16 ? dq_t<bf16_t>(a, maps, nw, s) : dq_t<f16>(a, maps, nw, s);
-  return r ? r : join<false>(a, bf16, s);
-}
+int mapattn_dq(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) { return bf16 ? dq_t<bf16_t>(a, maps, nw, s) : dq_t<f16>(a, maps, nw, s); }
 int mapattn_dkv(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) {
   const int r = bf16 ? dkv_t<bf16_t>(a, maps, nw, s) : dkv_t<f16>(a, maps, nw, s);
-  return r ? r : join<true>(a, bf16, s);
-}
-int mapattn_reduce(const MapAttnArgs& a, int maps, int bf16, hipStream_t s) {
-  if (maps == 2) {
-    hipLaunchKernelGGL(mapattn_dlam_kernel, dim3((unsigned)a.H), dim3(256), 0, s, a);
-    ANIP_LAUNCH_CHECK("mapattn_dlam_kernel");
-    return 0;
-  }
-  if (a.diag_part != a.diag) {
-    hipLaunchKernelGGL(mapattn_diag_kernel, dim3((unsigned)((a.ND + 2 + 255) / 256), (unsigned)a.parts, (unsigned)a.H), dim3(256), 0, s, a);
-    ANIP_LAUNCH_CHECK("mapattn_diag_kernel");
-  }
-  const int lds = (a.ND + 2) * 4;
-  if (bf16) hipLaunchKernelGGL((mapattn_dtable_kernel<bf16_t>), dim3((unsigned)a.H), dim3(1024), lds, s, a);
-  else hipLaunchKernelGGL((mapattn_dtable_kernel<f16>), dim3((unsigned)a.H), dim3(1024), lds, s, a);
-  ANIP_LAUNCH_CHECK("mapattn_dtable_kernel");
+  if (r || a.splits == 1) return r;
+  const unsigned grid = mapattn_grid("mapattn_join_kernel", cdiv64((int64_t)a.B * a.Tk * a.Hkv * (a.dv / 2), 256), 256);
+  if (!grid) return -1;
+  if (bf16) hipLaunchKernelGGL((mapattn_join_kernel<bf16_t>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((mapattn_join_kernel<f16>), dim3(grid), dim3(256), 0, s, a);
+  ANIP_LAUNCH_CHECK("mapattn_join_kernel");
   return 0;
 }
