@@ -348,13 +348,17 @@ __device__ __forceinline__ void sum_lam(const MapAttnArgs& a, int head, float* s
   }
 }
 
-// fragments of a wave's K rows in LDS instead of registers (the widest heads: 477 us against 503 at 2 x 4096 causal, 8 heads of
-// 128 + 128, where 18 registers went to scratch)
-constexpr int dkv_held(int maps, int nt) { return maps * nt >= 16 ? 3 : 0; }
+// fragments of a wave's K rows in LDS instead of registers.  Two maps, the widest heads: 477 us against 503 at 2 x 4096 causal, 8
+// heads of 128 + 128, where 18 registers went to scratch.  One map of up to 128 channels: with 6 of 8 there (and 32 queries a step)
+// two waves share a SIMD where there was one: 168 -> 139 us at 2 x 2048 causal, 16 heads of 128, 86 -> 46 at 16 x 500 (4 of 8: 12
+// registers in scratch, 170 us; all 8: 147).
+constexpr int dkv_held(int maps, int ks, int ng) { return maps == 2 ? (ks >= 8 ? 3 : 0) : (ks == 8 && ng == 4 ? 6 : 0); }
+// two waves of the kernel on a SIMD
+constexpr bool dkv_two(int maps, int ks, int ng) { return (maps == 1 && ks <= 5) || (ng == 4 && (maps == 2 || ks <= 8)); }
 
 // ---- dK, dV: 32 keys per wave (pair; K and V rows in registers), tiles of QT queries of every head that shares them ------------
 template <typename T, int MAPS, int KS, int NT, int QT, int NG, int NS>
-__global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 2 : 1)) void mapattn_dkv_kernel(const MapAttnArgs a) {
+__global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void mapattn_dkv_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
   constexpr int NW = NG * MAPS, BK = 32 * NG, DT = (KS + 1) / 2;
   constexpr int KSV = MAPS == 1 ? KS : NT;               // steps over this wave's share of dv in W
@@ -365,7 +369,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
   constexpr int E = BK + QT;
   static_assert(MAPS == 1 || QT == 32, "the pair's exchange has one slot per tile");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  float* near = (float*)(smem + 2 * STAGE);  // (one map)
+  float* near = (float*)(smem + 2 * STAGE + NW * dkv_held(MAPS, KS, NG) * 1024);  // (one map)
 
   const int tid = threadIdx.x, lane = tid & 63, kl = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -383,7 +387,8 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
   if (lin < a.join_blocks) return join_dq<T>(a, lin);
   lin -= a.join_blocks;
   int kblk, bk;
-  place<MAPS == 1 && (KS <= 5)>(lin, nkb * a.splits, a.B * a.Hkv, a.causal, kblk, bk);  // causal: the first keys meet the most queries
+  // causal: the first keys meet the most queries (128 channels, the second half reversed: 53 us against 46 at 16 x 500, 143 against 139)
+  place<MAPS == 1 && (KS <= 5)>(lin, nkb * a.splits, a.B * a.Hkv, a.causal, kblk, bk);
   const int split = kblk % a.splits;
   kblk /= a.splits;
   const int b = bk / a.Hkv, kvh = bk - b * a.Hkv;
@@ -392,8 +397,8 @@ __global__ __launch_bounds__(64 * NG * MAPS, ((MAPS == 1 ? KS <= 5 : NG == 4) ? 
   const bool valid = key < len;
 
   // the last KL fragments of the K rows wait in LDS where registers are short; in scratch, their loads would wait for the DMA
-  constexpr int KL = dkv_held(MAPS, NT);
-  char* klds = smem + 2 * STAGE + NW * 8192 + wave * (KL * 1024) + lane * 16;
+  constexpr int KL = dkv_held(MAPS, KS, NG);
+  char* klds = smem + 2 * STAGE + (MAPS == 2 ? NW * 8192 : 0) + wave * (KL * 1024) + lane * 16;
   u32x4 kf[KS], vf[KSV];
   load_row<KS>(kf, (const char*)a.k + 2 * (b * a.k_sb + (int64_t)key * a.k_st + (int64_t)(kvh * MAPS + m) * a.k_sh), valid, h, a.d);
   load_row<KSV, MAPS>(vf, (const char*)a.v + 2 * (b * a.v_sb + (int64_t)key * a.v_st + (int64_t)kvh * a.v_sh), valid, h, a.dv, m);
@@ -690,9 +695,9 @@ template <typename T, int MAPS, int KS, int NT, int NG>
 int run_dkv(const MapAttnArgs& a0, hipStream_t s) {
   MapAttnArgs a = a0;
   constexpr int ROW = 16 * (MAPS * 4 * ((KS + 1) / 2) + 4 * NT);
-  constexpr int QT = (MAPS == 2 || NG == 1 || 2 * 64 * ROW > 64 * 1024) ? 32 : 64;
+  constexpr int QT = (MAPS == 2 || NG == 1 || KS >= 8) ? 32 : 64;
   constexpr int NS = (QT == 64 && KS <= 4) ? 2 : 1;  // (see run_dq)
-  const int lds = 2 * (QT * ROW + 2 * MAPS * 256) + (MAPS == 1 ? (2 * (a.R + 32 * NG + QT) + 1) * 4 : 2 * NG * (8192 + dkv_held(MAPS, NT) * 1024));
+  const int lds = 2 * (QT * ROW + 2 * MAPS * 256) + MAPS * NG * dkv_held(MAPS, KS, NG) * 1024 + (MAPS == 1 ? (2 * (a.R + 32 * NG + QT) + 1) * 4 : 2 * NG * 8192);
   const void* f = (const void*)mapattn_dkv_kernel<T, MAPS, KS, NT, QT, NG, NS>;
   if (anip_raise_lds_limit(f, lds) != 0) {
     anip_set_error("mapattn dkv: cannot raise the dynamic LDS limit to %d bytes", lds);
