@@ -19,12 +19,13 @@ int check(const char* what, const anip_attn_params* p, int maps, bool backward) 
     const char* name;
     const void* x;
     const int64_t* s;
-  } sides[4] = {{"q", p->q, p->q_stride}, {"k", p->k, p->k_stride}, {"v", p->v, p->v_stride}, {"dout", p->dout, p->dout_stride}};
+    int T;
+  } sides[4] = {{"q", p->q, p->q_stride, p->Tq}, {"k", p->k, p->k_stride, p->Tk}, {"v", p->v, p->v_stride, p->Tk}, {"dout", p->dout, p->dout_stride, p->Tq}};
   for (int i = 0; i < (backward ? 4 : 3); ++i) {
     const Side& t = sides[i];
     ANIP_REQUIRE(t.x != nullptr && ((uintptr_t)t.x & 15) == 0, "%s: %s must be a 16-byte aligned device pointer", what, t.name);
     ANIP_REQUIRE(t.s[0] % 8 == 0 && t.s[1] % 8 == 0 && t.s[2] % 8 == 0, "%s: %s: strides must be multiples of 8 elements", what, t.name);
-    ANIP_REQUIRE(t.s[1] >= 0 && t.s[1] < (1 << 24), "%s: %s: the distance between tokens must be below 2^24 elements", what, t.name);
+    ANIP_REQUIRE(t.T == 1 || (t.s[1] >= 0 && t.s[1] < (1 << 24)), "%s: %s: the distance between tokens must be below 2^24 elements", what, t.name);
   }
   ANIP_REQUIRE(p->out != nullptr && (((uintptr_t)p->out | (uintptr_t)p->out2) & 15) == 0, "%s: out and out2 must be 16-byte aligned device pointers", what);
   if (maps == 1) {
@@ -41,11 +42,14 @@ int check(const char* what, const anip_attn_params* p, int maps, bool backward) 
   return 0;
 }
 
+// the distance between tokens; of a lone one it may be anything, and any that clears its channels does
+int64_t token_stride(int T, const int64_t* s) { return T == 1 ? 256 : s[1]; }
+
 MapAttnArgs args(const anip_attn_params* p, int maps) {
   MapAttnArgs a{};
-  a.q = p->q, a.q_sb = p->q_stride[0], a.q_st = p->q_stride[1], a.q_sh = p->q_stride[2];
-  a.k = p->k, a.k_sb = p->k_stride[0], a.k_st = p->k_stride[1], a.k_sh = p->k_stride[2];
-  a.v = p->v, a.v_sb = p->v_stride[0], a.v_st = p->v_stride[1], a.v_sh = p->v_stride[2];
+  a.q = p->q, a.q_sb = p->q_stride[0], a.q_st = token_stride(p->Tq, p->q_stride), a.q_sh = p->q_stride[2];
+  a.k = p->k, a.k_sb = p->k_stride[0], a.k_st = token_stride(p->Tk, p->k_stride), a.k_sh = p->k_stride[2];
+  a.v = p->v, a.v_sb = p->v_stride[0], a.v_st = token_stride(p->Tk, p->v_stride), a.v_sh = p->v_stride[2];
   a.B = p->B, a.Tq = p->Tq, a.Tk = p->Tk, a.H = p->H, a.Hkv = p->Hkv, a.G = p->H / p->Hkv;
   a.d = p->d, a.dv = p->d * maps, a.causal = p->causal != 0;
   a.scale = p->scale, a.scale_log2 = p->scale * mapattn::LOG2E;
@@ -151,7 +155,7 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   ANIP_REQUIRE(p->workspace != nullptr && ((uintptr_t)p->workspace & 15) == 0 && p->workspace_bytes >= l.total * 4, "%s: a workspace of %lld bytes is wanted, 16-byte aligned", what, (long long)l.total * 4);
   ANIP_REQUIRE((int64_t)((p->Tq + 31) / 32) * (p->H / p->Hkv) < (1ll << 31), "%s: too many query tiles", what);
   MapAttnArgs a = args(p, maps);
-  a.dout = p->dout, a.do_sb = p->dout_stride[0], a.do_st = p->dout_stride[1], a.do_sh = p->dout_stride[2];
+  a.dout = p->dout, a.do_sb = p->dout_stride[0], a.do_st = token_stride(p->Tq, p->dout_stride), a.do_sh = p->dout_stride[2];
   a.dq = p->dq, a.dk = p->dk, a.dvo = p->dv, a.dtable = p->dtable, a.dlam = p->dlam;
   a.Tp = l.Tp, a.QW = l.QW, a.ND = l.ND, a.parts = l.parts;
   a.part_q = (float*)p->workspace;

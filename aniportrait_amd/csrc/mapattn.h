@@ -201,10 +201,6 @@ __device__ __forceinline__ void load_row(u32x4 (&f)[KS], const void* row, bool e
   }
 }
 
-__device__ __forceinline__ float xor32(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
-}
 __device__ __forceinline__ float xor32_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
@@ -222,26 +218,24 @@ __device__ __forceinline__ f32x16 zero16() {
 // row of register r in the lower half-wave; the upper one holds 4 rows on
 __device__ __forceinline__ constexpr int acc_row(int r) { return 8 * (r >> 2) + (r & 3); }
 
-__device__ __forceinline__ int seq_len(const MapAttnArgs& a, int b) {
-  if (a.kv_lens == nullptr) return a.Tk;
-  const int n = a.kv_lens[b];
-  return n < 0 ? 0 : (n > a.Tk ? a.Tk : n);
-}
 __device__ __forceinline__ int seq_start(const MapAttnArgs& a, int b) {
   if (a.q_start == nullptr) return a.start0;
   const int n = a.q_start[b];
   return n < -(1 << 29) ? -(1 << 29) : (n > (1 << 29) ? (1 << 29) : n);
 }
-
-template <typename T>
-__device__ __forceinline__ float load_scalar(const void* p, int64_t i) { return (float)((const T*)p)[i]; }
+// keys that a query of the sequence may see; causal: none behind the last query (a cache's rows that nothing was written to yet)
+__device__ __forceinline__ int seq_len(const MapAttnArgs& a, int b) {
+  int n = a.kv_lens == nullptr ? a.Tk : min(a.kv_lens[b], a.Tk);
+  if (a.causal) n = min(n, seq_start(a, b) + a.Tq);
+  return max(n, 0);
+}
 
 template <typename T>
 __device__ __forceinline__ float bias_at(const MapAttnArgs& a, int h, int rel) {
   const int x = rel < -a.R ? 0 : (rel > a.R ? 2 * a.R : rel + a.R);
   int n = a.buckets[x];
   n = n < 0 ? 0 : (n >= a.NB ? a.NB - 1 : n);
-  return load_scalar<T>(a.table, (int64_t)h * a.NB + n) * LOG2E;
+  return (float)((const T*)a.table)[(int64_t)h * a.NB + n] * LOG2E;
 }
 // near[x] = bias (base 2) of relative position x - R - E, x = 0 .. 2 (R + E): the saturated ends repeat over E entries, so that a
 // tile that touches (-R, R) reads without clamping

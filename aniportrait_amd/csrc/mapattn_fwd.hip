@@ -256,9 +256,7 @@ __global__ __launch_bounds__(64 * MAXT * MAPS, (MAPS == 1 ? 2 : 1)) void mapattn
   const bool mine = live && ql < nrow;
   const int lim = mine ? (a.causal ? min(len - 1, start + qi) : len - 1) : -1;
 
-  int kend = len;
-  if (a.causal) kend = min(kend, start + a.Tq);
-  const int nt_all = kend > 0 ? (kend + KT - 1) / KT : 0;
+  const int nt_all = (len + KT - 1) / KT;
   const int t0 = (int)((int64_t)nt_all * split / a.splits), t1 = (int)((int64_t)nt_all * (split + 1) / a.splits);
   // turns of the loop: with barriers inside, the same for all teams of the workgroup
   const int turns = MAPS == 1 ? (t1 - t0 - kwi + a.kw - 1) / a.kw : (a.kw == 1 ? (a.Tk + KT - 1) / KT : (t1 - t0 + a.kw - 1) / a.kw);

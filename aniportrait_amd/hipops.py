@@ -649,6 +649,13 @@ def _heads4(t, name, like=None, shape=None):
     return p, sb, st_, sh
 
 
+def _out4(t, name, like, shape):
+    """the same of a tensor that is written: every element has a place of its own"""
+    if any(n > 1 and x == 0 for n, x in zip(t.shape, t.stride())):
+        raise ValueError(f"{name}: an expanded tensor cannot take results, got strides {t.stride()}")
+    return _heads4(t, name, like, shape)
+
+
 def _packed4(t):
     """the same of a contiguous tensor of our own"""
     _, T, H, d = t.shape
@@ -740,14 +747,14 @@ def qk_norm_rope(q, k, q_weight, k_weight, rope=None, positions=None, eps=1e-6, 
         q_out = _new(q)
         qo = _packed4(q_out)
     else:
-        qo = _heads4(q_out, "q_out", q, q.shape)
+        qo = _out4(q_out, "q_out", q, q.shape)
     ko = _NOWHERE
     if k is not None:
         if k_out is None:
             k_out = _new(k)
             ko = _packed4(k_out)
         else:
-            ko = _heads4(k_out, "k_out", q, k.shape)
+            ko = _out4(k_out, "k_out", q, k.shape)
     elif k_out is not None:
         raise ValueError("k_out without k")
     _, B, T, Hq, Hkv = head[:5]
@@ -840,8 +847,8 @@ def _attn_fields(what, maps, q, k, v, causal, scale, kv_lens, q_start):
 
 
 def _bias_fields(what, table, buckets, q, H):
-    nb, n = table.shape[-1], buckets.shape[0] if buckets.dim() == 1 else 0
-    if table.dim() != 2 or n % 2 == 0 or nb < 1:
+    nb, n = table.shape[-1] if table.dim() == 2 else 0, buckets.shape[0] if buckets.dim() == 1 else 0
+    if n % 2 == 0 or nb < 1:
         raise ValueError(f"{what}: expected table (heads, buckets) and buckets (2 max_distance + 1), got {tuple(table.shape)}, "
                          f"{tuple(buckets.shape)}")
     if n > 8193:
@@ -926,7 +933,9 @@ def relative_attention(q, k, v, table, buckets, causal=False, scale=None, kv_len
     d <= 160; table (H, n_buckets) in the same type; buckets from relative_buckets, or any int32 (2 R + 1) of the buckets of the
     relative positions -R .. R (R <= 4096; further ones take the ends').  scale: default d^-1/2.  kv_lens (B,) int32: keys behind
     it are not seen, whatever they hold (padded batch, cache).  q_start (B,) int32: the position of query 0 (default Tk - Tq: the
-    queries are the last tokens); causal: query i sees keys up to q_start + i.  A query that sees no key gets zeros.
+    queries are the last tokens); causal: query i sees keys up to q_start + i, and what lies behind the last query's is not read
+    either (a later token's inf or NaN may reach the queries before it: it enters their sums times zero).  A query that sees no
+    key gets zeros.
     Returns out (B, Tq, H, d), or (out, lse) for_backward (lse (B, H, Tq) fp32)."""
     lib, what = L.load(), "relative_attention"
     fields = _attn_fields(what, 1, q, k, v, causal, scale, kv_lens, q_start)

@@ -259,7 +259,8 @@ int anip_qk_norm_rope_backward(const anip_qk_norm_params* p, void* stream);
  *   d a multiple of 8 up to 128; out (B, Tq, H, 2 d).
  * Both: p_i = q_start[b] + i is the position of query i (int32 [B]; NULL: Tk - Tq + i).  Query i sees key j if j < kv_lens[b]
  *   (int32 [B], clamped to [0, Tk]; NULL: Tk) and, when causal, j <= p_i; a query that sees no key gets zeros.  Keys and values
- *   behind kv_lens[b] are never used, whatever they hold.  out, dq, dk, dv are contiguous.  lse (fp32 [B][H * maps][Tq], natural
+ *   behind kv_lens[b], and causal ones behind the last query, are never used, whatever they hold; a value that causal hides from
+ *   some queries only enters their sums times zero (inf and NaN in it may reach them).  out, dq, dk, dv are contiguous.  lse (fp32 [B][H * maps][Tq], natural
  *   logarithm, -inf for rows without keys) and, for two maps, out2 (the second map's own output, as out) may be NULL where no
  *   backward follows.
  * Backward: dq, dk, dv, dtable [H][n_buckets] (inputs' type) or dlam fp32 [H] from dout and the forward's out, out2, lse.  Keys

@@ -97,6 +97,16 @@ def test_split_forward_wants_its_workspace():
     assert lib.anip_relative_attention_ws_bytes(C.byref(_attn_params(1, B=64, Tq=512, Tk=512)), 0) == 0
 
 
+@pytest.mark.parametrize("maps", [1, 2])
+def test_stride_of_a_lone_token_is_not_looked_at(maps):
+    lib = _ops().L.load()
+    f = lib.anip_relative_attention_ws_bytes if maps == 1 else lib.anip_differential_attention_ws_bytes
+    far = (64 * 256, 1 << 25, 64)
+    assert f(C.byref(_attn_params(maps, Tq=1, q_stride=far)), 0) >= 0
+    assert f(C.byref(_attn_params(maps, Tk=1, k_stride=far, v_stride=far)), 0) >= 0
+    assert f(C.byref(_attn_params(maps, Tk=1, q_stride=far)), 0) == -1
+
+
 def _norm_params(**kw):
     from aniportrait_amd import _lib as L
     p = L.QkNormParams()
@@ -371,6 +381,51 @@ def test_attention_of_many_short_sequences(maps):
 @pytest.mark.parametrize("shape", [(2, 70, 150, 2, 1, 64), (2, 3, 150, 4, 2, 40)])
 def test_attention_of_strided_tensors(maps, shape):
     _check(maps, shape, "bf16", True, strided=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("maps", [1, 2], ids=["relative", "differential"])
+def test_lone_tokens_of_far_strides(maps):
+    """one query or one key cut from a token-major tensor of very long rows"""
+    ops, dt = _ops(), torch.float16
+    far = lambda t: t.as_strided(t.shape, (t.stride(0), 1 << 25, t.stride(2), 1)) if t.shape[1] == 1 else t   # noqa: E731
+    for Tq, Tk in ((1, 50), (40, 1), (1, 1)):
+        q, k, v, do, _ = (x if x is None else x.to(DEV) for x in _inputs(maps, 1, Tq, Tk, 2, 2, 64, dt, None))
+        if maps == 1:
+            more = (rnd(2, 32, dtype=dt, seed=9).to(DEV), ops.relative_buckets(32, 128, device=DEV))
+            fwd, bwd = ops.relative_attention, ops.relative_attention_backward
+        else:
+            more, fwd, bwd = (torch.tensor([0.3, 0.6], device=DEV),), ops.differential_attention, ops.differential_attention_backward
+        want = fwd(q, k, v, *more, for_backward=True)
+        got = fwd(far(q), far(k), far(v), *more, for_backward=True)
+        for x, y in zip(got + bwd(far(do), far(q), far(k), far(v), *got, *more), want + bwd(do, q, k, v, *want, *more)):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Tq,starts", [(1, [0, 100, 37]), (70, [0, 65, -20]), (70, [-70, 230, 31])])
+@pytest.mark.parametrize("maps", [1, 2], ids=["relative", "differential"])
+def test_keys_behind_the_last_query_of_a_causal_call_are_never_used(maps, Tq, starts):
+    """a cache without kv_lens: rows that no query reaches may hold anything, and get zero gradients"""
+    ops, Tk = _ops(), 300
+    ends = [min(max(s + Tq, 0), Tk) for s in starts]
+    q, k, v, do, lens = _inputs(maps, len(starts), Tq, Tk, 4, 2, 64, torch.float16, ends)
+    q, k, v, do, lens = (t.to(DEV) for t in (q, k, v, do, lens))
+    if maps == 1:
+        more = (rnd(4, 32, dtype=torch.float16, seed=9).to(DEV), ops.relative_buckets(32, 128, False, device=DEV))
+        fwd, bwd = ops.relative_attention, ops.relative_attention_backward
+    else:
+        more = (torch.rand(4, generator=torch.Generator().manual_seed(3)).to(DEV),)
+        fwd, bwd = ops.differential_attention, ops.differential_attention_backward
+    kw = dict(causal=True, q_start=torch.tensor(starts, dtype=torch.int32, device=DEV))
+    want = fwd(q, k, v, *more, for_backward=True, kv_lens=lens, **kw)
+    got = fwd(q, k, v, *more, for_backward=True, **kw)
+    grads = bwd(do, q, k, v, *got, *more, **kw)
+    for x, y in zip(got + grads, want + bwd(do, q, k, v, *want, *more, kv_lens=lens, **kw)):
+        assert torch.equal(x, y)
+        assert not x.isnan().any()
+    for b, n in enumerate(ends):
+        assert grads[1][b, n:].abs().sum() == 0 and grads[2][b, n:].abs().sum() == 0
 
 
 @pytest.mark.gpu
@@ -716,6 +771,17 @@ def test_norm_wrapper_refuses(change):
         a["q"] = rnd(2, 8, 4, 60, dtype=torch.float16).to(DEV)
     with pytest.raises((TypeError, ValueError)):
         ops.qk_norm_rope(*a.values(), **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("side", [0, 1])
+def test_norm_wrapper_refuses_expanded_outputs(side):
+    ops = _ops()
+    q, w = rnd(2, 8, 4, 64, dtype=torch.float16).to(DEV), torch.ones(64, device=DEV)
+    shared = torch.zeros((1, 8, 4, 64), dtype=torch.float16, device=DEV).expand(2, -1, -1, -1)
+    with pytest.raises(ValueError, match="expanded"):
+        ops.qk_norm_rope(q, q.clone(), w, w, **{("q_out", "k_out")[side]: shared})
+    assert shared.abs().max() == 0
 
 
 @pytest.mark.gpu
