@@ -448,83 +448,81 @@ __global__ __launch_bounds__(64 * MAXT * MAPS, (MAPS == 1 ? 2 : 1)) void mapattn
 }
 
 // ---- joins the parts of a split forward: o = sum_s 2^(l_s - l) o_s, l = log2 sum_s 2^l_s -----------------------------------------
-// Few parts: LR lanes of 4 channels per row.  Many: a wave per row; lane s holds the weight of parts s, s + 64, ..; 64 / LR parts are added at once by LR lanes of 4 channels each.
-template <typename T, int MAPS, int LR, bool FEW>
+// Up to PARTS of them: LR lanes of 4 channels per row.  More (PARTS = 0): a wave per row; lane s holds the weight of parts s, s + 64,
+// ..; 64 / LR parts are added at once by LR lanes of 4 channels each.  Bound by latency: rows are few and each load is some 600 ns
+// away, so all loads of a row, of both maps (of many parts, the first 8 steps'), are on their way before the first weight is needed.
+template <typename T, int MAPS, int LR, int PARTS>
 __global__ __launch_bounds__(256) void mapattn_combine_kernel(const MapAttnArgs a) {
-  constexpr int PG = 64 / LR, MW = 4;  // parts at once; weights of a lane (256 parts at most)
+  constexpr bool SHORT = PARTS > 0;
+  constexpr int PG = 64 / LR, MW = 4, N = SHORT ? PARTS : 8;  // parts at once; weights of a lane (256 parts at most); loads in flight
   const int64_t rows = (int64_t)a.B * a.Tq * a.H;
-  const int lane = threadIdx.x & 63, c0 = (lane % LR) * 4, sg = FEW ? 0 : lane / LR;
-  const int64_t row = FEW ? (int64_t)blockIdx.x * (4 * PG) + threadIdx.x / LR : (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, c0 = (lane % LR) * 4, sg = SHORT ? 0 : lane / LR;
+  const int64_t row = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / (SHORT ? LR : 64);
   if (row >= rows) return;
-  float x[MAPS][4], lse2[MAPS];
+  constexpr int NW = SHORT ? N : MW;
+  float lw[MAPS][NW], x[MAPS][4], lse2[MAPS];
+  f32x4 v[MAPS][N];
+  auto load = [&](int m, int s) {
+    f32x4 r = {0.f, 0.f, 0.f, 0.f};
+    if (s < a.splits && c0 < a.dv) r = *(const f32x4*)(a.part_o + (((int64_t)s * rows + row) * MAPS + m) * a.dv + c0);
+    return r;
+  };
 #pragma unroll
   for (int m = 0; m < MAPS; ++m) {
-    float lw[MW], mx = -INFINITY;
-    if (FEW) {
-      for (int s = 0; s < a.splits; ++s) mx = fmaxf(mx, a.part_l[((int64_t)s * rows + row) * MAPS + m]);
-      const float base = mx == -INFINITY ? 0.f : mx;
-      float sum = 0.f;
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-      for (int s = 0; s < a.splits; ++s) {
-        const int64_t at = ((int64_t)s * rows + row) * MAPS + m;
-        const float w = __builtin_amdgcn_exp2f(a.part_l[at] - base);
-        sum += w;
-        f32x4 v = {0.f, 0.f, 0.f, 0.f};
-        if (c0 < a.dv) v = *(const f32x4*)(a.part_o + at * a.dv + c0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[e], acc[e]);
-      }
-      const bool none = mx == -INFINITY;
-      lse2[m] = none ? -INFINITY : base + __builtin_amdgcn_logf(sum);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[m][e] = none ? 0.f : acc[e] / sum;
-      continue;
+    for (int i = 0; i < NW; ++i) {
+      const int s = SHORT ? i : lane + 64 * i;
+      lw[m][i] = s < a.splits ? a.part_l[((int64_t)s * rows + row) * MAPS + m] : -INFINITY;
     }
 #pragma unroll
-    for (int i = 0; i < MW; ++i) {
-      const int s = lane + 64 * i;
-      lw[i] = s < a.splits ? a.part_l[((int64_t)s * rows + row) * MAPS + m] : -INFINITY;
-      mx = fmaxf(mx, lw[i]);
-    }
-    mx = wave_max(mx);
+    for (int k = 0; k < N; ++k) v[m][k] = load(m, SHORT ? k : k * PG + sg);
+  }
+#pragma unroll
+  for (int m = 0; m < MAPS; ++m) {
+    float mx = lw[m][0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) mx = fmaxf(mx, lw[m][i]);
+    if (!SHORT) mx = wave_max(mx);
     const float base = mx == -INFINITY ? 0.f : mx;
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < MW; ++i) {
-      lw[i] = __builtin_amdgcn_exp2f(lw[i] - base);
-      sum += lw[i];
+    for (int i = 0; i < NW; ++i) {
+      lw[m][i] = __builtin_amdgcn_exp2f(lw[m][i] - base);
+      sum += lw[m][i];
     }
-    sum = wave_sum(sum);
+    if (!SHORT) sum = wave_sum(sum);
     const bool none = mx == -INFINITY;
     const float inv = none ? 0.f : 1.0f / sum;
     lse2[m] = none ? -INFINITY : base + __builtin_amdgcn_logf(sum);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](float w, const f32x4& p) {
 #pragma unroll
-    for (int i = 0; i < MW; ++i) {
-      if (64 * i >= a.splits) break;
-      const int n = min(64, a.splits - 64 * i);
-      for (int s0 = 0; s0 < n; s0 += 4 * PG) {
-        f32x4 v[4];
+      for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, p[e], acc[e]);
+    };
+    if (SHORT) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int s = s0 + k * PG + sg;
-          v[k] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (s < n && c0 < a.dv) v[k] = *(const f32x4*)(a.part_o + (((int64_t)(s + 64 * i) * rows + row) * MAPS + m) * a.dv + c0);
-        }
+      for (int k = 0; k < N; ++k) add(lw[m][k % NW], v[m][k]);
+    } else {
+      // (64 parts are a whole number of steps, and a part behind the last is zeros)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float w = __shfl(lw[i], (s0 + k * PG + sg) & 63, 64);  // (a part behind the last is zeros)
+      for (int i = 0; i < MW; ++i) {
+        for (int s0 = 0; s0 < 64 && 64 * i + s0 < a.splits; s0 += N * PG) {
+          if (i + s0 > 0) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) acc[e] = fmaf(w, v[k][e], acc[e]);
+            for (int k = 0; k < N; ++k) v[m][k] = load(m, 64 * i + s0 + k * PG + sg);
+          }
+#pragma unroll
+          for (int k = 0; k < N; ++k) add(__shfl(lw[m][i % NW], s0 + k * PG + sg, 64), v[m][k]);
         }
       }
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float t = acc[e];
+      if (!SHORT) {
 #pragma unroll
-      for (int o = LR; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
+        for (int o = LR; o < 64; o <<= 1) t += __shfl_xor(t, o, 64);
+      }
       x[m][e] = t * inv;
     }
   }
@@ -606,13 +604,16 @@ int run_token(const MapAttnArgs& a0, hipStream_t s) {
 
 template <typename T, int MAPS, int LR>
 int run_combine_lr(const MapAttnArgs& a, hipStream_t s) {
-  // (one part after the other up to 8: 8 us against 13 at 29 688 rows x 2; 64 / LR at once beyond: 9 against 17 at 128 rows x 16)
+  // (up to 16 parts by LR lanes: 4.9 us at 128 rows x 16, two maps, 7 by a wave; with room for 16 where there are 2: 10.8 at 29 688
+  // rows, 7.4 with 8.  Workgroups of one wave where rows are few: 16 parts by waves, 7 us against 7.8)
   const int64_t rows = (int64_t)a.B * a.Tq * a.H;
-  const bool few = a.splits <= 8;
-  const unsigned grid = mapattn_grid("mapattn_combine_kernel", cdiv64(rows, few ? 256 / LR : 4), 256);
+  const int64_t lanes = rows * (a.splits <= 16 ? LR : 64);
+  const int threads = lanes <= 32768 ? 64 : 256;
+  const unsigned grid = mapattn_grid("mapattn_combine_kernel", cdiv64(lanes, threads), threads);
   if (!grid) return -1;
-  if (few) hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, true>), dim3(grid), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, false>), dim3(grid), dim3(256), 0, s, a);
+  if (a.splits <= 8) hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, 8>), dim3(grid), dim3(threads), 0, s, a);
+  else if (a.splits <= 16) hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, 16>), dim3(grid), dim3(threads), 0, s, a);
+  else hipLaunchKernelGGL((mapattn_combine_kernel<T, MAPS, LR, 0>), dim3(grid), dim3(threads), 0, s, a);
   ANIP_LAUNCH_CHECK("mapattn_combine_kernel");
   return 0;
 }

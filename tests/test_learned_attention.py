@@ -498,6 +498,15 @@ def test_attention_of_a_long_cache(maps):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape,lens", [((1, 1, 9001, 1, 1, 64), None), ((1, 2, 36000, 2, 1, 40), None), ((2, 1, 36000, 1, 1, 128), [36000, 130]),
+                                        ((1, 40, 20000, 1, 1, 64), [19000])], ids=str)
+@pytest.mark.parametrize("maps", [1, 2], ids=["relative", "differential"])
+def test_attention_joined_from_many_parts(maps, shape, lens):
+    """few problems with many keys: 17 to more than 64 parts, some of them without keys"""
+    _check(maps, shape, "fp16", True, lens, None if lens is None else [n - shape[1] for n in lens], train=False)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("maps", [1, 2], ids=["relative", "differential"])
 def test_attention_gradient_against_differences(maps):
     """dq, dk, dv and the learned weights' gradient along a direction against differences of the 64-bit definition"""
