@@ -293,7 +293,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) voi
 
 // ---- sums of parts, in a fixed order ----------------------------------------------------------------------------------------
 // The queries' kernel leaves sums for each 32 queries (dtable's diagonals, dlam) and, split, dQ in parts.  They are added by the
-// first workgroups of the keys' launch, beside its own work; dtable of many groups by two kernels of its own.
+// first workgroups of the keys' launch, beside its own work; dtable of many groups by kernels of its own.
 
 // four channels of a gradient from the 32-bit parts of a split walk, `n` values apart
 __device__ __forceinline__ f32x4 add_parts(const float* p, int parts, int64_t n) {
@@ -309,28 +309,57 @@ __device__ __forceinline__ void join_dq(const MapAttnArgs& a, int block) {
   const f32x4 t = add_parts(a.part_q + i, a.qsplits, n);
   *(u32x2*)((char*)a.dq + i * 2) = u32x2{Num<T>::pack(t[0], t[1]), Num<T>::pack(t[2], t[3])};
 }
-// a head's bucket sums from `parts` rows of diagonals: the rows added per slot, then a wave per bucket adds the slots that belong to it
+// a head's bucket sums from `parts` rows of diagonals: each lane adds the rows of a slot, then lane c takes the 64 slots of the wave
+// that belong to bucket c, one after the other, from the other lanes' registers.  Bound by the loads' latency in short launches: the
+// rows of 16 parts, and the next slots' first 16, are on their way at once (2 heads, 3 x 19: 12 us of the keys' launch,
+// 43 with a wave for each bucket that walks over the slots in LDS)
 template <typename T>
 __device__ __forceinline__ void sum_table(const MapAttnArgs& a, int head, const float* rows, int parts, float* sums) {
   const int n = a.ND + 2, lane = threadIdx.x & 63;
   const float* p = rows + (int64_t)head * parts * n;
-  for (int x = threadIdx.x; x < n; x += blockDim.x) {
-    float t = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) t += p[(int64_t)i * n + x];
-    sums[x] = t;
-  }
-  __syncthreads();
-  for (int c = threadIdx.x >> 6; c < a.NB; c += blockDim.x >> 6) {
-    float t = 0.f;
-    for (int x = lane; x < a.ND; x += 64) {  // slot x: relative position x - R - DIAG_PAD, beyond +-R as +-R
-      const int r = x < DIAG_PAD ? 0 : (x > 2 * a.R + DIAG_PAD ? 2 * a.R : x - DIAG_PAD);
-      int bx = a.buckets[r];
-      bx = bx < 0 ? 0 : (bx >= a.NB ? a.NB - 1 : bx);
-      if (bx == c) t += sums[x] + (x == DIAG_PAD ? sums[a.ND] : 0.f) + (x == 2 * a.R + DIAG_PAD ? sums[a.ND + 1] : 0.f);
+  auto load = [&](int x, int i0, float (&t)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t[i] = i0 + i < parts && x < n ? p[(int64_t)(i0 + i) * n + x] : 0.f;
+  };
+  // slot x < ND: relative position x - R - DIAG_PAD, beyond +-R as +-R; the last two: all pairs beyond -R, and beyond R
+  auto bucket = [&](int x) {
+    int r = x - DIAG_PAD;
+    r = x == a.ND || r < 0 ? 0 : (r > 2 * a.R ? 2 * a.R : r);
+    const int bx = x < n ? a.buckets[r] : -1;
+    return x >= n ? -1 : (bx < 0 ? 0 : (bx >= a.NB ? a.NB - 1 : bx));
+  };
+  for (int c0 = 0; c0 < a.NB; c0 += 64) {
+    float acc = 0.f, t[16];
+    int x = threadIdx.x, bx = bucket(x);
+    load(x, 0, t);
+    while (x - lane < n) {
+      const int xn = x + blockDim.x, bn = bucket(xn);
+      float tn[16], v = 0.f;
+      load(xn, 0, tn);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v += t[i];
+      for (int i0 = 16; i0 < parts; i0 += 16) {
+        load(x, i0, t);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v += t[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 64; ++i) {
+        const float vi = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), i));
+        acc += __builtin_amdgcn_readlane(bx, i) == c0 + lane ? vi : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) t[i] = tn[i];
+      x = xn, bx = bn;
     }
-    t = wave_sum(t);
-    if (lane == 0) ((T*)a.dtable)[(int64_t)head * a.NB + c] = (T)t;
+    __syncthreads();
+    sums[threadIdx.x] = acc;
+    __syncthreads();
+    if ((int)threadIdx.x < min(64, a.NB - c0)) {
+      float s = 0.f;
+      for (int w = 0; w < (int)blockDim.x; w += 64) s += sums[w + lane];
+      ((T*)a.dtable)[(int64_t)head * a.NB + c0 + lane] = (T)s;
+    }
   }
 }
 __device__ __forceinline__ void sum_lam(const MapAttnArgs& a, int head, float* sums) {
@@ -653,7 +682,7 @@ __global__ __launch_bounds__(256) void mapattn_diag_kernel(const MapAttnArgs a) 
 }
 template <typename T>
 __global__ __launch_bounds__(1024) void mapattn_dtable_kernel(const MapAttnArgs a) {
-  extern __shared__ float sums[];
+  __shared__ float sums[1024];
   sum_table<T>(a, blockIdx.x, a.diag_part, a.parts, sums);
 }
 
@@ -681,12 +710,11 @@ int run_dq(const MapAttnArgs& a, hipStream_t s) {
 }
 template <typename T>
 int table_sums(const MapAttnArgs& a, hipStream_t s) {
-  const int lds = (a.ND + 2) * 4;
   if (a.diag_part != a.diag) {
     hipLaunchKernelGGL(mapattn_diag_kernel, dim3((unsigned)((a.ND + 2 + 255) / 256), (unsigned)a.parts, (unsigned)a.H), dim3(256), 0, s, a);
     ANIP_LAUNCH_CHECK("mapattn_diag_kernel");
   }
-  hipLaunchKernelGGL((mapattn_dtable_kernel<T>), dim3((unsigned)a.H), dim3(1024), lds, s, a);
+  hipLaunchKernelGGL((mapattn_dtable_kernel<T>), dim3((unsigned)a.H), dim3(1024), 0, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dtable_kernel");
   return 0;
 }
@@ -703,9 +731,10 @@ int run_dkv(const MapAttnArgs& a0, hipStream_t s) {
     anip_set_error("mapattn dkv: cannot raise the dynamic LDS limit to %d bytes", lds);
     return -2;
   }
-  // sums beside the keys' work: dlam always, dtable up to 512 loads for a thread (2 x 2048, 16 heads: 11 us of two kernels saved)
+  // sums beside the keys' work: dlam always, dtable where a thread has few batches of loads, less time than the keys' work takes
+  // (16 x 500, 8 heads of 64, 32 batches: 31 us, 26 + 11 in two kernels more; 4 heads of 32, 36 x 20, 24 of a lone wave: 22, 6 + 10)
   const int64_t groups = (int64_t)a.B * a.QW * a.qsplits;
-  a.sum_blocks = MAPS == 2 || groups * ((a.ND + 2 + 64 * NG - 1) / (64 * NG)) <= 512 ? a.H : 0;
+  a.sum_blocks = MAPS == 2 || cdiv64(groups, 16) * ((a.ND + 2 + 64 * NG - 1) / (64 * NG)) <= (NG == 1 ? 12 : 32) ? a.H : 0;
   if (!a.sum_blocks) {
     const int r = table_sums<T>(a, s);
     if (r) return r;
