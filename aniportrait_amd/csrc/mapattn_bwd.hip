@@ -31,7 +31,7 @@ __device__ __forceinline__ f32x16 get16(const float* x) {
 
 // ---- dQ: 32 queries per wave (pair), tiles of KT keys -----------------------------------------------------------------------
 template <typename T, int MAPS, int KS, int NT, int KT, int NG, int NS>
-__global__ __launch_bounds__(64 * NG * MAPS, (MAPS == 1 || NG == 4 ? 2 : 1)) void mapattn_dq_kernel(const MapAttnArgs a) {
+__global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) ? 2 : 1)) void mapattn_dq_kernel(const MapAttnArgs a) {
   constexpr bool BIAS = MAPS == 1;
   constexpr int NW = NG * MAPS, BQ = 32 * NG, DT = (KS + 1) / 2, KSV = MAPS == 1 ? KS : NT;  // KSV: steps over this wave's share of dv
   constexpr int KCH = 4 * DT, VCH = 4 * NT;

@@ -458,6 +458,15 @@ def test_relative_attention_tables(shape, case):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 300, 300, 2, 2, 64), (3, 30, 41, 2, 1, 160), (40, 20, 20, 1, 1, 32)], ids=str)
+@pytest.mark.parametrize("n", [64, 65, 200])
+def test_relative_attention_of_many_buckets(shape, n):
+    table = rnd(shape[3], n, dtype=torch.bfloat16, seed=9)
+    buckets = torch.randint(0, n, (2 * 90 + 1,), generator=torch.Generator().manual_seed(1), dtype=torch.int32)
+    _check(1, shape, "bf16", extra=(table, buckets))
+
+
+@pytest.mark.gpu
 def test_relative_attention_clamps_bucket_numbers():
     ops = _ops()
     q, k, v, do, _ = _inputs(1, 1, 40, 40, 2, 2, 64, torch.float16, None)
