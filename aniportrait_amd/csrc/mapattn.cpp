@@ -122,7 +122,7 @@ int walk_splits(int64_t blocks, int64_t tiles) {
 
 struct BwdLayout {
   int nwq, nwk, Tp, QW, ND, parts, qsplits, ksplits;
-  int64_t rows, diag, dlam, part, dkv, dq, total;  // floats
+  int64_t rows, rows3, diag, dlam, part, dkv, dq, total;  // floats
 };
 BwdLayout layout(const anip_attn_params* p, int maps) {
   BwdLayout l{};
@@ -138,13 +138,14 @@ BwdLayout layout(const anip_attn_params* p, int maps) {
     const int64_t groups = (int64_t)p->B * l.QW * l.qsplits;
     l.parts = (int)(groups < 32 ? groups : 32);  // few query groups: their own sums are the parts
     l.diag = (int64_t)p->H * groups * (l.ND + 2);
+    if (l.qsplits > 1) l.rows3 = (int64_t)p->H * groups * 3 * 32;
     l.part = groups > 32 ? (int64_t)p->H * l.parts * (l.ND + 2) : 0;
   } else {
     l.dlam = (int64_t)p->H * p->B * l.QW * l.qsplits;
   }
   if (l.qsplits > 1) l.dq = (int64_t)l.qsplits * p->B * p->Tq * p->H * maps * p->d;
   if (l.ksplits > 1) l.dkv = (int64_t)l.ksplits * p->B * p->Tk * p->Hkv * 2 * maps * p->d;
-  l.total = l.dq + l.dkv + 2 * l.rows + l.diag + l.part + l.dlam;
+  l.total = l.dq + l.dkv + 2 * l.rows + l.diag + l.part + l.dlam + l.rows3;
   return l;
 }
 
@@ -165,6 +166,7 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   a.diag = a.rows_d + l.rows;
   a.diag_part = l.part ? a.diag + l.diag : a.diag;
   a.dlam_part = a.diag + l.diag + l.part;
+  a.rows3 = a.dlam_part + l.dlam;
   hipStream_t s = (hipStream_t)stream;
   AnipProfScope prof_(kid, stream);
   a.splits = a.qsplits = l.qsplits;

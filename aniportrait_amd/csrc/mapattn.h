@@ -36,6 +36,7 @@ struct MapAttnArgs {
   void *dq, *dk, *dvo, *dtable;
   float* dlam;
   int Tp;             // padded rows of rows_lse / rows_d
+  float* rows3;       // (split) [h][b][split][3][32 QW]: sum of dS, sums of P beyond -R and beyond R, of a row's part
   float *rows_lse, *rows_d;  // [(b H + h) MAPS + m][Tp]: -lse in base 2 (-inf for rows without keys), D
   int QW, ND;         // 32-query groups per head; floats per group in diag
   float* diag;        // [h][b][group][ND + 2]: sums of dS along diagonals (+ below -R, above R)

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
   f32x16 dq[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();
-  float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f, dl_sum = 0.f;
+  float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f, p_lo = 0.f, p_hi = 0.f, sum_near = 0.f, dl_sum = 0.f;
   float dpos = 0.f, dneg = 0.f;  // diagonals rel = base + ql and base - 32 + ql of the current 32 keys, base = k0 - pw
   int next_base = 0;
   bool open = false;
@@ -208,20 +208,44 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
 #pragma unroll
           for (int r = 0; r < 16; ++r) dl_sum = fmaf(s[0][r], w[0][r], dl_sum);
       }
+      auto total = [&] {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) t += s[i][r];
+        return t;
+      };
+      if (BIAS) {
+        if (zone != 0) {
+          const float t = total();
+          if (zone < 0) p_lo += t;
+          else p_hi += t;
+        } else {  // those of the pairs that are beyond reach
+          const int rel = k0 + 4 * h - (pw + ql), lo = -a.R - rel, hi = (a.R > 0 ? a.R : 1) - rel;
+          if (k0 - (pw + 31) <= -a.R)
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) p_lo += 32 * i + acc_row(r) <= lo ? s[i][r] : 0.f;
+          if (k0 + 32 * NS - 1 - pw >= a.R)
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+#pragma unroll
+              for (int r = 0; r < 16; ++r) p_hi += 32 * i + acc_row(r) >= hi ? s[i][r] : 0.f;
+        }
+      }
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[i][r] *= MAPS == 1 ? w[i][r] - D : fmaf(w[i][r], wf, wd);
       if (BIAS) {
+        const float t = total();
         if (zone != 0) {
-          float t16 = 0.f;
-#pragma unroll
-          for (int i = 0; i < NS; ++i)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) t16 += s[i][r];
-          if (zone < 0) sum_lo += t16;
-          else sum_hi += t16;
+          if (zone < 0) sum_lo += t;
+          else sum_hi += t;
         } else {
+          sum_near += t;
           // value of (key k0 + ko, query ql) belongs to diagonal ko - ql: lane x takes it from lane (ko - x) mod 32 of its half
           open = true;
           next_base = k0 + 32 * NS - pw;
@@ -256,6 +280,23 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
   if (BIAS && diag) {
     const float done = xor32_sum(dneg);
     if (open && h == 0) diag[next_base - 32 + ql + a.R + DIAG_PAD] = done;
+    // What D is off by (the rounded outputs, the forward's rounded P) is what a row's dS leave over from their sum of 0.  It meets
+    // a bucket with the row's P in it: with most of it, beyond the bias's reach, where it is taken out; with a few keys' up to
+    // there, where it is small beside the roundings.  dtable in bf16, 2 heads, 2 x 3954: 2e-2 off with it, less than 4e-3 without;
+    // it costs 8 us of 54 at 2 x 2048, 16 heads of 64 (two sums more over P and dS).
+    const float eps = xor32_sum(sum_lo + sum_hi + sum_near);
+    if (a.splits == 1) {
+      sum_lo = fmaf(-eps, p_lo, sum_lo);
+      sum_hi = fmaf(-eps, p_hi, sum_hi);
+    } else {  // (sum_table knows the whole row)
+      const float pl = xor32_sum(p_lo), ph = xor32_sum(p_hi);
+      float* r3 = a.rows3 + (((int64_t)head * a.B + b) * a.splits + split) * 3 * a.QW * 32 + q0 + ql;
+      if (h == 0) {
+        r3[0] = eps;
+        r3[a.QW * 32] = pl;
+        r3[a.QW * 64] = ph;
+      }
+    }
     const float lo = wave_sum(sum_lo), hi = wave_sum(sum_hi);
     if (lane == 0) {
       diag[a.ND] = lo;
@@ -328,6 +369,24 @@ __device__ __forceinline__ void sum_table(const MapAttnArgs& a, int head, const 
     const int bx = x < n ? a.buckets[r] : -1;
     return x >= n ? -1 : (bx < 0 ? 0 : (bx >= a.NB ? a.NB - 1 : bx));
   };
+  // split rows: what the far sums have to lose (see the queries' kernel)
+  float off[2] = {0.f, 0.f};
+  if (a.qsplits > 1) {
+    const int per = a.QW * 32;
+    for (int i = threadIdx.x; i < a.B * per; i += blockDim.x) {
+      const int b = i / per;
+      const float* r3 = a.rows3 + ((int64_t)head * a.B + b) * a.qsplits * 3 * per + (i - b * per);
+      float e = 0.f, lo = 0.f, hi = 0.f;
+#pragma unroll 4
+      for (int s = 0; s < a.qsplits; ++s, r3 += 3 * per) {
+        e += r3[0];
+        lo += r3[per];
+        hi += r3[2 * per];
+      }
+      off[0] = fmaf(e, lo, off[0]);
+      off[1] = fmaf(e, hi, off[1]);
+    }
+  }
   for (int c0 = 0; c0 < a.NB; c0 += 64) {
     float acc = 0.f, t[16];
     int x = threadIdx.x, bx = bucket(x);
@@ -351,6 +410,14 @@ __device__ __forceinline__ void sum_table(const MapAttnArgs& a, int head, const 
 #pragma unroll
       for (int i = 0; i < 16; ++i) t[i] = tn[i];
       x = xn, bx = bn;
+    }
+    if (a.qsplits > 1) {
+      const int ends[2] = {bucket(a.ND), bucket(a.ND + 1)};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float t = wave_sum(off[i]);
+        if (ends[i] == c0 + lane) acc -= t;
+      }
     }
     __syncthreads();
     sums[threadIdx.x] = acc;
@@ -734,7 +801,8 @@ int run_dkv(const MapAttnArgs& a0, hipStream_t s) {
   // sums beside the keys' work: dlam always, dtable where a thread has few batches of loads, less time than the keys' work takes
   // (16 x 500, 8 heads of 64, 32 batches: 31 us, 26 + 11 in two kernels more; 4 heads of 32, 36 x 20, 24 of a lone wave: 22, 6 + 10)
   const int64_t groups = (int64_t)a.B * a.QW * a.qsplits;
-  a.sum_blocks = MAPS == 2 || cdiv64(groups, 16) * ((a.ND + 2 + 64 * NG - 1) / (64 * NG)) <= (NG == 1 ? 12 : 32) ? a.H : 0;
+  a.sum_blocks = MAPS == 2 || (cdiv64(groups, 16) * ((a.ND + 2 + 64 * NG - 1) / (64 * NG)) +
+                                (a.qsplits > 1 ? cdiv64((int64_t)a.B * a.QW, 2 * NG) : 0)) <= (NG == 1 ? 12 : 48) ? a.H : 0;
   if (!a.sum_blocks) {
     const int r = table_sums<T>(a, s);
     if (r) return r;

@@ -467,6 +467,31 @@ def test_relative_attention_of_many_buckets(shape, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("T", [700, 1500])   # rows whole, and split over workgroups
+def test_table_gradient_where_outputs_round_alike(T):
+    """values about 1: all outputs round the same way, and so D is off the same way in all rows.  Beyond the bias's reach that has
+    to cancel: dtable is off by its own rounding and by what is left of the pairs within reach"""
+    ops, H, d, R, u = _ops(), 2, 32, 128, 2.0 ** -8
+    q, k = rnd(1, T, H, d, dtype=torch.bfloat16, seed=1), rnd(1, T, H, d, dtype=torch.bfloat16, seed=2)
+    v, do = rnd(1, T, H, d, dtype=torch.bfloat16, scale=0.05, shift=1.003, seed=3), rnd(1, T, H, d, dtype=torch.bfloat16, scale=0.1, shift=1.0, seed=4)
+    table, buckets = rnd(H, 32, dtype=torch.bfloat16, seed=9), ops.relative_buckets(32, R, device="cpu")
+    a = [t.to(DEV) for t in (q, k, v, table, buckets)]
+    out, lse = ops.relative_attention(*a, for_backward=True)
+    got = ops.relative_attention_backward(do.to(DEV), *a[:3], out, lse, *a[3:])[3].cpu().double()
+    Q, K, V, G = (t[0].double().transpose(0, 1) for t in (q, k, v, do))
+    rel = torch.arange(T)[None] - torch.arange(T)[:, None]
+    b = buckets.long()[rel.clamp(-R, R) + R]
+    P = (Q @ K.transpose(1, 2) * d ** -0.5 + table.double()[:, b]).softmax(-1)
+    W, O_ = G @ V.transpose(1, 2), P @ V
+    D = (G * O_).sum(-1, keepdim=True)
+    off = 2 * u * (G.abs() * O_.abs()).sum(-1, keepdim=True)    # of D: out rounded, P rounded (V > 0)
+    add = lambda x: torch.stack([torch.zeros(32, dtype=torch.float64).index_add(0, b.flatten(), y.flatten()) for y in x])   # noqa: E731
+    want = add(P * (W - D))
+    bound = u * want.abs() + add(P * off * (rel.abs() < R)) + 2.0 ** -18 * add(P * (G.abs() @ V.abs().transpose(1, 2) + D.abs()))
+    assert ((got - want).abs() <= bound).all(), ((got - want).abs() / bound).max()
+
+
+@pytest.mark.gpu
 def test_relative_attention_clamps_bucket_numbers():
     ops = _ops()
     q, k, v, do, _ = _inputs(1, 1, 40, 40, 2, 2, 64, torch.float16, None)
