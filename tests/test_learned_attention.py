@@ -429,6 +429,25 @@ def test_keys_behind_the_last_query_of_a_causal_call_are_never_used(maps, Tq, st
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Tq", [1, 90])
+@pytest.mark.parametrize("maps", [1, 2], ids=["relative", "differential"])
+def test_attention_of_broadcast_keys(maps, Tq):
+    """one sequence's keys and values for all of a batch (stride 0), a broadcast gradient: what copies give"""
+    ops, dt = _ops(), torch.bfloat16
+    q, k, v, do, _ = (x if x is None else x.to(DEV) for x in _inputs(maps, 3, Tq, 120, 4, 2, 64, dt, None))
+    k, v, do = k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1), do[:1, :1].expand(3, Tq, -1, -1)
+    if maps == 1:
+        more = (rnd(4, 32, dtype=dt, seed=9).to(DEV), ops.relative_buckets(32, 128, device=DEV))
+        fwd, bwd = ops.relative_attention, ops.relative_attention_backward
+    else:
+        more, fwd, bwd = (torch.tensor([0.3, 0.6, 0.1, 0.9], device=DEV),), ops.differential_attention, ops.differential_attention_backward
+    got = fwd(q, k, v, *more, causal=True, for_backward=True)
+    want = fwd(q, k.contiguous(), v.contiguous(), *more, causal=True, for_backward=True)
+    for x, y in zip(got + bwd(do, q, k, v, *got, *more, causal=True), want + bwd(do.contiguous(), q, k.contiguous(), v.contiguous(), *want, *more, causal=True)):
+        assert torch.equal(x, y) and x.is_contiguous()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("maps", [1, 2], ids=["relative", "differential"])
 def test_attention_scale(maps):
     _check(maps, (1, 90, 90, 2, 2, 64), "fp16", True, scale=0.4)
