@@ -68,6 +68,10 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
   load_row<KS>(qf, (const char*)a.q + 2 * (b * a.q_sb + (int64_t)qi * a.q_st + (int64_t)(head * MAPS + m) * a.q_sh), valid, h, a.d);
   load_row<KSV, MAPS>(df, drow, valid, h, a.dv, m);
 
+  // the split that has the first keys (the first one where there are none) leaves the rows' statistics for the keys' kernel
+  const bool first = nt_keys > 0 ? nt0 == 0 && nt_all > 0 : split == 0;
+  const int64_t rows_at = ((int64_t)bh * MAPS + m) * a.Tp + qi;
+
   // ---- row statistics: D_m = dO . o_m (o_1 = o + lam o_2), -lse in base 2 -------------------------------------------------
   float nl, D;
   {
@@ -94,10 +98,9 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
     }
     const float l = valid ? a.lse[((int64_t)bh * MAPS + m) * a.Tq + qi] * LOG2E : -INFINITY;
     nl = l == -INFINITY ? -INFINITY : -l;  // rows without keys: P = 2^-inf = 0
-    if (h == 0 && split == 0) {
-      const int64_t at = ((int64_t)bh * MAPS + m) * a.Tp + qi;
-      a.rows_lse[at] = nl + Num<T>::PSH;
-      a.rows_d[at] = D * (1.0f / (1 << Num<T>::PSH));
+    if (h == 0 && first) {
+      a.rows_lse[rows_at] = nl + Num<T>::PSH;
+      a.rows_d[rows_at] = D * (1.0f / (1 << Num<T>::PSH));
     }
   }
 
@@ -144,7 +147,11 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
     far_hi = bias_at<T>(a, head, a.R);
   }
   // dS = wf P W + wd P
-  const float wf = m == 0 ? 1.f : -lam, wd = m == 0 ? -D : lam * D;
+  const float wf = m == 0 ? 1.f : -lam;
+  float wd = -wf * D;
+  // All keys of these rows in one step: D from P and W themselves.  Rounded outputs leave W - D of rows with few keys nothing but
+  // their rounding (one key: dS is 0; a sequence of one key in a padded batch gave its 898 rows a dQ of 5e-3 of the other one's)
+  const int whole = (a.causal ? min(len, start + q0 + 32) : len) <= 32 * NS ? 0 : -1;
 
   if (nt0 < nt_all) issue(nt0);
   for (int t = nt0; t < nt_all; ++t) {
@@ -207,6 +214,20 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
         if (m == 1)
 #pragma unroll
           for (int r = 0; r < 16; ++r) dl_sum = fmaf(s[0][r], w[0][r], dl_sum);
+      }
+      if (k0 == whole) {
+        float pw1 = 0.f, p1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            pw1 = fmaf(s[i][r], w[i][r], pw1);
+            p1 += s[i][r];
+          }
+        pw1 = xor32_sum(pw1), p1 = xor32_sum(p1);
+        D = p1 > 0.f ? pw1 / p1 : 0.f;
+        wd = -wf * D;
+        if (h == 0) a.rows_d[rows_at] = D * (1.0f / (1 << Num<T>::PSH));
       }
       auto total = [&] {
         float t = 0.f;

@@ -448,6 +448,26 @@ def test_attention_of_broadcast_keys(maps, Tq):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Tq,Tk,causal", [(90, 90, False), (20, 40, True), (300, 1100, False)])
+@pytest.mark.parametrize("maps", [1, 2], ids=["relative", "differential"])
+def test_rows_that_see_one_key_have_no_gradient(maps, Tq, Tk, causal):
+    """softmax over one key is 1 whatever its score: dq and dk are 0, up to the 32-bit sums of W (2^-16 of its terms' sizes)"""
+    ops, dt, d = _ops(), torch.bfloat16, 64
+    q, k, v, do, lens = (x.to(DEV) for x in _inputs(maps, 2, Tq, Tk, 2, 2, d, dt, [Tk, 1]))
+    if maps == 1:
+        more = (rnd(2, 32, dtype=dt, seed=9).to(DEV), ops.relative_buckets(32, 128, device=DEV))
+        fwd, bwd = ops.relative_attention, ops.relative_attention_backward
+    else:
+        more, fwd, bwd = (torch.tensor([0.7, 0.9], device=DEV),), ops.differential_attention, ops.differential_attention_backward
+    got = fwd(q, k, v, *more, causal=causal, kv_lens=lens, for_backward=True)
+    dq, dk = bwd(do, q, k, v, *got, *more, causal=causal, kv_lens=lens)[:2]
+    w = torch.einsum("ihc,hc->ih", do[1].double().abs(), v[1, 0].double().abs()).repeat_interleave(maps, 1)   # (Tq, heads): |dO| |V|
+    assert (dq[1].double().abs() <= 2.0 ** -16 * d ** -0.5 * w[..., None] * k[1, 0].double().abs()).all()
+    assert (dk[1, 0].double().abs() <= 2.0 ** -16 * d ** -0.5 * torch.einsum("ih,ihc->hc", w, q[1].double().abs())).all()
+    assert dk[1, 1:].abs().sum() == 0 and dq[0].abs().max() > 0
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("maps", [1, 2], ids=["relative", "differential"])
 def test_attention_scale(maps):
     _check(maps, (1, 90, 90, 2, 2, 64), "fp16", True, scale=0.4)
