@@ -45,9 +45,12 @@ def family(name):
                      ("temporal_attn", "temporal_attn_kernel"), ("gn_stats", "gn_stats_kernel"), ("gn_scale_shift", "gn_apply_kernel"),
                      ("gn_apply", "gn_apply_kernel"), ("gn_slab", "gn_apply_kernel"), ("layernorm_kernel", "layernorm_kernel"), ("softmax_rows", "softmax_rows_kernel"),
                      ("conv_direct", "conv_small_kernel"), ("conv3x3_c4", "conv_small_kernel"), ("conv_small", "conv_small_kernel"), ("linear_small", "linear_small_kernel"),
-                     ("bn_", "batchnorm_kernels"), ("ffn_geglu", "gemm_kernel<false>")):
+                     ("bn_", "batchnorm_kernels"), ("ffn_geglu", "gemm_kernel<false>"), ("head_norm", "head_norm_kernels")):
         if key in name:
             return fam
+    if "mapattn" in name:               # one map or two: the first number of the template (c++filt trips over bf16, hence "int, EL"); the join of split gradients has none
+        m = re.search(r"mapattn_\w+?_kernel(?:IDF16[_b]Li|<[^,]*, )(\d)", name)
+        return "differential_attention_kernels" if (m and m.group(1) == "2") or "int, EL" in name else "relative_attention_kernels"
     if any(k in name for k in ("add_kernel", "window_accumulate", "cfg_ddim", "ncfhw", "nhwc", "u8_to_f16", "f16_to_u8")):
         return "elementwise"
     return None
