@@ -4,7 +4,7 @@
 //   dlam = -sum P_2 W          dtable[bucket] = sum of dS over the pairs of the bucket
 // Two kernels, one that owns queries (dQ, dlam, dtable's partial sums) and one that owns keys (dK, dV): each recomputes P and W
 // (7 products instead of 5 at one map) and needs no atomics, so equal inputs give equal gradients.  P is recomputed from the row
-// statistics of the forward; D from dO and the stored outputs.  dS and P are rounded to the inputs' type as operands of the
+// statistics of the forward; D from dO and the stored outputs, or from P and W where a row's keys all lie in one step.  dS and P are rounded to the inputs' type as operands of the
 // matrix products (2^-9 or 2^-12 relative per term, averaged over a row); all sums are 32-bit.
 #include "mapattn.h"
 
