@@ -29,6 +29,9 @@ __device__ __forceinline__ f32x16 get16(const float* x) {
   return v;
 }
 
+// fragments of a wave's Q rows in LDS instead of registers, so that nothing goes to scratch: one map of 160 channels, and lone waves of 128
+constexpr int dq_held(int maps, int ks, int ng) { return maps == 1 ? (ng == 4 ? (ks == 10 ? 6 : 0) : (ks == 8 ? 4 : 0)) : 0; }
+
 // ---- dQ: 32 queries per wave (pair), tiles of KT keys -----------------------------------------------------------------------
 template <typename T, int MAPS, int KS, int NT, int KT, int NG, int NS>
 __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) ? 2 : 1)) void mapattn_dq_kernel(const MapAttnArgs a) {
@@ -39,7 +42,8 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
   constexpr int E = BQ + KT;
   static_assert(MAPS == 1 || KT == 32, "the pair's exchange has one slot per tile");
   extern __shared__ __attribute__((aligned(1024))) char smem[];
-  float* near = (float*)(smem + 2 * STAGE);  // (one map)
+  constexpr int QL = dq_held(MAPS, KS, NG);
+  float* near = (float*)(smem + 2 * STAGE + NW * QL * 1024);  // (one map)
 
   const int tid = threadIdx.x, lane = tid & 63, ql = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -67,6 +71,9 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
   const char* drow = (const char*)a.dout + 2 * (b * a.do_sb + (int64_t)qi * a.do_st + (int64_t)head * a.do_sh);
   load_row<KS>(qf, (const char*)a.q + 2 * (b * a.q_sb + (int64_t)qi * a.q_st + (int64_t)(head * MAPS + m) * a.q_sh), valid, h, a.d);
   load_row<KSV, MAPS>(df, drow, valid, h, a.dv, m);
+  char* qlds = smem + 2 * STAGE + wave * (QL * 1024) + lane * 16;  // the last QL fragments of the Q rows
+#pragma unroll
+  for (int i = 0; i < QL; ++i) *(u32x4*)(qlds + i * 1024) = qf[KS - QL + i];
 
   // the split that has the first keys (the first one where there are none) leaves the rows' statistics for the keys' kernel
   const bool first = nt_keys > 0 ? nt0 == 0 && nt_all > 0 : split == 0;
@@ -177,7 +184,8 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
 #pragma unroll
         for (int kk = 0; kk < KS; ++kk)
 #pragma unroll
-          for (int i = 0; i < NS; ++i) s[i] = Num<T>::mfma(kr.get(st + m * K_BYTES, sub + i, kk), qf[kk], s[i]);
+          for (int i = 0; i < NS; ++i)
+            s[i] = Num<T>::mfma(kr.get(st + m * K_BYTES, sub + i, kk), kk < KS - QL ? qf[kk] : lds16(qlds + (kk - (KS - QL)) * 1024), s[i]);
       }
       float mul = a.scale_log2, add = 0.f;
       int zone = 0;  // -1, 1: all of these pairs beyond the bias's reach
@@ -769,8 +777,8 @@ __global__ __launch_bounds__(256) void mapattn_diag_kernel(const MapAttnArgs a) 
   a.diag_part[((int64_t)head * a.parts + part) * (a.ND + 2) + slot] = t;
 }
 template <typename T>
-__global__ __launch_bounds__(1024) void mapattn_dtable_kernel(const MapAttnArgs a) {
-  __shared__ float sums[1024];
+__global__ __launch_bounds__(512) void mapattn_dtable_kernel(const MapAttnArgs a) {
+  __shared__ float sums[512];
   sum_table<T>(a, blockIdx.x, a.diag_part, a.parts, sums);
 }
 
@@ -780,11 +788,13 @@ namespace {
 template <typename T, int MAPS, int KS, int NT, int NG>
 int run_dq(const MapAttnArgs& a, hipStream_t s) {
   constexpr int ROW = 16 * (MAPS * 4 * ((KS + 1) / 2) + 4 * NT);
-  constexpr int KT = (MAPS == 2 || NG == 1 || 2 * 64 * ROW > 64 * 1024) ? 32 : 64;
+  // tiles of 32 keys from 128 channels on: with 64 the kernel kept ten registers in scratch, reloaded in every step (16 x 500, 8 heads of
+  // 128, the backward: 126.4 us against 125.3; 4 x 1500: 196 against 193; 160 channels, Q held in LDS for the same: 368 against 367)
+  constexpr int KT = (MAPS == 2 || NG == 1 || KS >= 8) ? 32 : 64;
   // two sub-tiles of 32 at once where the registers allow two waves per SIMD all the same: two chains of products beside each other
   // (2 x 2048, 16 / 4 heads of 64: 54 us against 59, the keys' kernel 63 against 70; heads of 80: no difference)
   constexpr int NS = (KT == 64 && KS <= 4) ? 2 : 1;
-  const int lds = 2 * KT * ROW + (MAPS == 1 ? (2 * (a.R + 32 * NG + KT) + 1) * 4 : 2 * NG * 4096);
+  const int lds = 2 * KT * ROW + MAPS * NG * dq_held(MAPS, KS, NG) * 1024 + (MAPS == 1 ? (2 * (a.R + 32 * NG + KT) + 1) * 4 : 2 * NG * 4096);
   const void* f = (const void*)mapattn_dq_kernel<T, MAPS, KS, NT, KT, NG, NS>;
   if (anip_raise_lds_limit(f, lds) != 0) {
     anip_set_error("mapattn dq: cannot raise the dynamic LDS limit to %d bytes", lds);
@@ -802,7 +812,7 @@ int table_sums(const MapAttnArgs& a, hipStream_t s) {
     hipLaunchKernelGGL(mapattn_diag_kernel, dim3((unsigned)((a.ND + 2 + 255) / 256), (unsigned)a.parts, (unsigned)a.H), dim3(256), 0, s, a);
     ANIP_LAUNCH_CHECK("mapattn_diag_kernel");
   }
-  hipLaunchKernelGGL((mapattn_dtable_kernel<T>), dim3((unsigned)a.H), dim3(1024), 0, s, a);
+  hipLaunchKernelGGL((mapattn_dtable_kernel<T>), dim3((unsigned)a.H), dim3(512), 0, s, a);
   ANIP_LAUNCH_CHECK("mapattn_dtable_kernel");
   return 0;
 }
