@@ -122,7 +122,7 @@ int walk_splits(int64_t blocks, int64_t tiles) {
 
 struct BwdLayout {
   int nwq, nwk, Tp, QW, ND, parts, qsplits, ksplits;
-  int64_t rows, rows3, diag, dlam, part, dkv, dq, total;  // floats
+  int64_t rows, rows3, diag, dlam, part, dkv, dq, sizes, total;  // floats
 };
 BwdLayout layout(const anip_attn_params* p, int maps) {
   BwdLayout l{};
@@ -145,7 +145,8 @@ BwdLayout layout(const anip_attn_params* p, int maps) {
   }
   if (l.qsplits > 1) l.dq = (int64_t)l.qsplits * p->B * p->Tq * p->H * maps * p->d;
   if (l.ksplits > 1) l.dkv = (int64_t)l.ksplits * p->B * p->Tk * p->Hkv * 2 * maps * p->d;
-  l.total = l.dq + l.dkv + 2 * l.rows + l.diag + l.part + l.dlam + l.rows3;
+  if (p->dtype == 0) l.sizes = (int64_t)p->B * p->H * maps * l.QW * 2;
+  l.total = l.dq + l.dkv + 2 * l.rows + l.sizes + l.diag + l.part + l.dlam + l.rows3;
   return l;
 }
 
@@ -163,7 +164,8 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   a.part_o = a.part_q + l.dq;
   a.rows_lse = a.part_o + l.dkv;
   a.rows_d = a.rows_lse + l.rows;
-  a.diag = a.rows_d + l.rows;
+  a.sizes = (f32x2*)(a.rows_d + l.rows);  // (each part before it holds a multiple of 8 floats)
+  a.diag = a.rows_d + l.rows + l.sizes;
   a.diag_part = l.part ? a.diag + l.diag : a.diag;
   a.dlam_part = a.diag + l.diag + l.part;
   a.rows3 = a.dlam_part + l.dlam;

@@ -38,6 +38,7 @@ struct MapAttnArgs {
   int Tp;             // padded rows of rows_lse / rows_d
   float* rows3;       // (split) [h][b][split][3][32 QW]: sum of dS, sums of P beyond -R and beyond R, of a row's part
   float *rows_lse, *rows_d;  // [(b H + h) MAPS + m][Tp]: -lse in base 2 (-inf for rows without keys), D
+  f32x2* sizes;       // (fp16) [m][b H + h][QW]: the largest |dO| and |D| of 32 rows, times the map's weight
   int QW, ND;         // 32-query groups per head; floats per group in diag
   float* diag;        // [h][b][group][ND + 2]: sums of dS along diagonals (+ below -R, above R)
   float* dlam_part;   // [h][b][group]
@@ -68,6 +69,8 @@ struct Num<f16> {
   // P is written 2^PSH times larger where it is summed over queries: fp16 keeps full precision down to 2^-14 only, and the
   // weights of long rows are smaller
   static constexpr int PSH = 8;
+  // dS, which is as large as the gradient that comes in, takes a power of two that follows the data
+  static constexpr bool SCALED = true;
   __device__ static __forceinline__ uint32_t pack(float a, float b) {
     f32x2 t = {a, b};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(t, f16x2v));  // v_cvt_pk_f16_f32: to nearest even
@@ -81,6 +84,7 @@ struct Num<f16> {
 template <>
 struct Num<bf16_t> {
   static constexpr int PSH = 0;
+  static constexpr bool SCALED = false;
   __device__ static __forceinline__ uint32_t pack(float a, float b) {
     f32x2 t = {a, b};
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(t, bf16x2));
@@ -244,6 +248,13 @@ template <typename T>
 __device__ __forceinline__ void fill_near(const MapAttnArgs& a, int h, int E, float* near, int tid, int n) {
   for (int x = tid; x < 2 * (a.R + E) + 1; x += n) near[x] = bias_at<T>(a, h, x - a.R - E);
 }
+
+// the power of two that brings x into [2^(t - 1), 2^t); 0 where there is nothing to scale
+__device__ __forceinline__ int power_to(float x, int t) {
+  const int e = t - __builtin_amdgcn_frexp_expf(x);
+  return x > 0.f && x < INFINITY ? (e < -100 ? -100 : (e > 100 ? 100 : e)) : 0;
+}
+__device__ __forceinline__ float power(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
 
 // block -> (slot among `slots` tiles, (batch, head) among nbh): all tiles of a (batch, head) on one XCD where the heads can be
 // spread evenly over the 8 of them, so that K and V are fetched into one L2 only.  `falling`: the work falls with the slot

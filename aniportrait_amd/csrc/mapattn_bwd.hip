@@ -5,7 +5,8 @@
 // Two kernels, one that owns queries (dQ, dlam, dtable's partial sums) and one that owns keys (dK, dV): each recomputes P and W
 // (7 products instead of 5 at one map) and needs no atomics, so equal inputs give equal gradients.  P is recomputed from the row
 // statistics of the forward; D from dO and the stored outputs, or from P and W where a row's keys all lie in one step.  dS and P are rounded to the inputs' type as operands of the
-// matrix products (2^-9 or 2^-12 relative per term, averaged over a row); all sums are 32-bit.
+// matrix products (off by 2^-8 or 2^-11 of a term at most, averaged over a row); all sums are 32-bit.  In fp16 both are rounded as a
+// power of two times themselves that follows the data, so that gradients of any size keep that precision.
 #include "mapattn.h"
 
 using namespace mapattn;
@@ -32,10 +33,28 @@ __device__ __forceinline__ f32x16 get16(const float* x) {
 // fragments of a wave's Q rows in LDS instead of registers, so that nothing goes to scratch: one map of 160 channels, and lone waves of 128
 constexpr int dq_held(int maps, int ks, int ng) { return maps == 1 ? (ng == 4 ? (ks == 10 ? 6 : 0) : (ks == 8 ? 4 : 0)) : 0; }
 
+// t + the squares of eight values
+template <typename T>
+__device__ __forceinline__ float squares(const u32x4& x, float t) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) t = fmaf(Num<T>::lo(x[i]), Num<T>::lo(x[i]), fmaf(Num<T>::hi(x[i]), Num<T>::hi(x[i]), t));
+  return t;
+}
+// the largest of a wave's values (none below 0) in all lanes, in the vector ALU: quads, mirrored halves and rows of 16, then rows
+template <int CTRL>
+__device__ __forceinline__ float dpp_most(float v) {
+  return fmaxf(v, __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), CTRL, 0xF, 0xF, true)));
+}
+__device__ __forceinline__ float wave_most(float v) {
+  v = dpp_most<0x140>(dpp_most<0x141>(dpp_most<0x4E>(dpp_most<0xB1>(v))));
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return xor32_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
 // ---- dQ: 32 queries per wave (pair), tiles of KT keys -----------------------------------------------------------------------
 template <typename T, int MAPS, int KS, int NT, int KT, int NG, int NS>
 __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) ? 2 : 1)) void mapattn_dq_kernel(const MapAttnArgs a) {
-  constexpr bool BIAS = MAPS == 1;
+  constexpr bool BIAS = MAPS == 1, SCALED = Num<T>::SCALED;
   constexpr int NW = NG * MAPS, BQ = 32 * NG, DT = (KS + 1) / 2, KSV = MAPS == 1 ? KS : NT;  // KSV: steps over this wave's share of dv
   constexpr int KCH = 4 * DT, VCH = 4 * NT;
   constexpr int K_BYTES = KT * KCH * 16, V_BYTES = KT * VCH * 16, STAGE = MAPS * K_BYTES + V_BYTES;
@@ -80,11 +99,12 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
   const int64_t rows_at = ((int64_t)bh * MAPS + m) * a.Tp + qi;
 
   // ---- row statistics: D_m = dO . o_m (o_1 = o + lam o_2), -lse in base 2 -------------------------------------------------
-  float nl, D;
+  float nl, D, n2 = 0.f;  // (n2: |dO|^2)
   {
     const int64_t orow = (((int64_t)b * a.Tq + qi) * a.H + head) * a.dv * 2;
     auto dot = [&](const void* o) {
       float t = 0.f;
+      n2 = 0.f;
 #pragma unroll 4
       for (int c = h; c < a.dv / 8; c += 2) {
         u32x4 x = {0u, 0u, 0u, 0u}, y = x;
@@ -94,6 +114,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) t = fmaf(Num<T>::lo(x[i]), Num<T>::lo(y[i]), fmaf(Num<T>::hi(x[i]), Num<T>::hi(y[i]), t));
+        if (SCALED) n2 = squares<T>(x, n2);
       }
       return xor32_sum(t);
     };
@@ -107,8 +128,21 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
     nl = l == -INFINITY ? -INFINITY : -l;  // rows without keys: P = 2^-inf = 0
     if (h == 0 && first) {
       a.rows_lse[rows_at] = nl + Num<T>::PSH;
-      a.rows_d[rows_at] = D * (1.0f / (1 << Num<T>::PSH));
+      a.rows_d[rows_at] = MAPS == 1 ? -D : D * (1.0f / (1 << Num<T>::PSH));
     }
+  }
+
+  // dS = wf P W + wd P, in fp16 2^fe times that.  dS is as large as P |dO| |V|, and fp16 keeps its precision from 2^-14 to 2^16: 2^fe
+  // brings the largest |dO| of the wave's rows to 2^8.  That is room for weights of 2^-20 beside values of about 1, and for values of up
+  // to about 50.  If larger ones overflow it, the walk is done again with room for any (a maximum of dS in every step instead: dQ at
+  // 2 x 2048, 16 / 4 heads of 64, 70 us against 65).
+  const float w0 = MAPS == 2 && m == 1 ? -lam : 1.f;
+  int fe = 0;
+  bool again = false;
+  if (SCALED) {
+    const float most = sqrtf(wave_most(xor32_sum(n2))) * fabsf(w0), mostD = wave_most(fabsf(D)) * fabsf(w0);
+    fe = __builtin_amdgcn_readfirstlane(power_to(most, 8));
+    if (first && lane == 0 && q0 < a.Tq) a.sizes[((int64_t)m * a.B * a.H + bh) * a.QW + q0 / 32] = f32x2{most, mostD};
   }
 
   float* diag = nullptr;
@@ -153,15 +187,41 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
     far_lo = bias_at<T>(a, head, -a.R);
     far_hi = bias_at<T>(a, head, a.R);
   }
-  // dS = wf P W + wd P
-  const float wf = m == 0 ? 1.f : -lam;
-  float wd = -wf * D;
   // All keys of these rows in one step: D from P and W themselves.  Rounded outputs leave W - D of rows with few keys nothing but
   // their rounding (one key: dS is 0; a sequence of one key in a padded batch gave its 898 rows a dQ of 5e-3 of the other one's)
   const int whole = (a.causal ? min(len, start + q0 + 32) : len) <= 32 * NS ? 0 : -1;
 
+  float wf = power(fe) * w0, wd = -wf * D;
   if (nt0 < nt_all) issue(nt0);
-  for (int t = nt0; t < nt_all; ++t) {
+  for (int t = nt0;; ++t) {
+    if (t >= nt_all) {
+      if (!SCALED || again || nt0 >= nt_all) break;
+      // an infinity among the rounded dS leaves one, or NaN, in dQ
+      float bad[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bad[r & 3] = fmaf(dq[dt][r], 0.f, bad[r & 3]);
+      int* over = (int*)smem;
+      const int mine_over = __any((bad[0] + bad[1]) + (bad[2] + bad[3]) != 0.f);
+      lds_barrier();  // all tiles read
+      if (lane == 0) over[wave] = mine_over;
+      lds_barrier();
+      int any = 0;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) any |= over[i];
+      if (!__builtin_amdgcn_readfirstlane(any)) break;
+      lds_barrier();  // all flags read
+      again = true;
+      fe -= 14;  // |W| and |D| are at most |dO| 2^16 sqrt(256): with |dO| at 2^-6 dS stays below 2^15
+      wf = power(fe) * w0, wd = -wf * D;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();
+      sum_lo = sum_hi = p_lo = p_hi = sum_near = dl_sum = dpos = dneg = 0.f;
+      open = false;
+      t = nt0;
+      issue(t);
+    }
     MAPATTN_WAIT_DMA();
     __syncthreads();
     if (t + 1 < nt_all) issue(t + 1);
@@ -235,7 +295,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
         pw1 = xor32_sum(pw1), p1 = xor32_sum(p1);
         D = p1 > 0.f ? pw1 / p1 : 0.f;
         wd = -wf * D;
-        if (h == 0) a.rows_d[rows_at] = D * (1.0f / (1 << Num<T>::PSH));
+        if (h == 0) a.rows_d[rows_at] = MAPS == 1 ? -D : D * (1.0f / (1 << Num<T>::PSH));
       }
       auto total = [&] {
         float t = 0.f;
@@ -267,7 +327,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
 #pragma unroll
       for (int i = 0; i < NS; ++i)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[i][r] *= MAPS == 1 ? w[i][r] - D : fmaf(w[i][r], wf, wd);
+        for (int r = 0; r < 16; ++r) s[i][r] *= MAPS == 1 && !SCALED ? w[i][r] - D : fmaf(w[i][r], wf, wd);
       if (BIAS) {
         const float t = total();
         if (zone != 0) {
@@ -288,7 +348,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
               dneg += ql <= ko ? 0.f : v;
             }
             const float done = xor32_sum(dneg);  // no later key reaches these 32 diagonals
-            if (diag && h == 0) diag[k0 + 32 * i - pw - 32 + ql + a.R + DIAG_PAD] = done;
+            if (diag && h == 0) diag[k0 + 32 * i - pw - 32 + ql + a.R + DIAG_PAD] = __builtin_amdgcn_ldexpf(done, -fe);
             dneg = dpos;
             dpos = 0.f;
           }
@@ -306,8 +366,10 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
     }
   }
 
+  const float fi = power(-fe);
   if (BIAS && diag) {
-    const float done = xor32_sum(dneg);
+    sum_lo *= fi, sum_hi *= fi, sum_near *= fi;
+    const float done = xor32_sum(dneg) * fi;
     if (open && h == 0) diag[next_base - 32 + ql + a.R + DIAG_PAD] = done;
     // What D is off by (the rounded outputs, the forward's rounded P) is what a row's dS leave over from their sum of 0.  It meets
     // a bucket with the row's P in it: with most of it, beyond the bias's reach, where it is taken out; with a few keys' up to
@@ -337,6 +399,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
     if (lane == 0) a.dlam_part[(((int64_t)head * a.B + b) * a.QW + q0 / 32) * a.splits + split] = -t;
   }
   if (!valid) return;
+  const float scale = a.scale * fi;
   if (a.splits > 1) {
     float* pp = a.part_q + (((int64_t)split * a.B * a.Tq + (int64_t)b * a.Tq + qi) * a.H * MAPS + head * MAPS + m) * a.d;
 #pragma unroll
@@ -345,7 +408,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
       for (int rq = 0; rq < 4; ++rq) {
         const int c0 = dt * 32 + rq * 8 + h * 4;
         const f32x16& x = dq[dt];
-        if (c0 < a.d) *(f32x4*)(pp + c0) = f32x4{x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale, x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale};
+        if (c0 < a.d) *(f32x4*)(pp + c0) = f32x4{x[4 * rq] * scale, x[4 * rq + 1] * scale, x[4 * rq + 2] * scale, x[4 * rq + 3] * scale};
       }
     return;
   }
@@ -357,7 +420,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
       const int c0 = dt * 32 + rq * 8 + h * 4;
       const f32x16& x = dq[dt];
       if (c0 < a.d)
-        *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale), Num<T>::pack(x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale)};
+        *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * scale, x[4 * rq + 1] * scale), Num<T>::pack(x[4 * rq + 2] * scale, x[4 * rq + 3] * scale)};
     }
 }
 
@@ -474,17 +537,17 @@ __device__ __forceinline__ void sum_lam(const MapAttnArgs& a, int head, float* s
 }
 
 // fragments of a wave's K rows in LDS instead of registers.  Two maps, the widest heads: 477 us against 503 at 2 x 4096 causal, 8
-// heads of 128 + 128, where 18 registers went to scratch.  One map of up to 128 channels: with 6 of 8 there (and 32 queries a step)
-// two waves share a SIMD where there was one: 168 -> 139 us at 2 x 2048 causal, 16 heads of 128, 86 -> 46 at 16 x 500 (4 of 8: 12
-// registers in scratch, 170 us; all 8: 147).
-constexpr int dkv_held(int maps, int ks, int ng) { return maps == 2 ? (ks >= 8 ? 3 : 0) : (ks == 8 && ng == 4 ? 6 : 0); }
+// heads of 128 + 128, where 18 registers went to scratch.  One map of up to 128 channels: with 7 of 8 there (and 32 queries a step)
+// two waves share a SIMD where there was one: 168 -> 139 us with 6 at 2 x 2048 causal, 16 heads of 128, 86 -> 46 at 16 x 500 (4 of 8: 12
+// registers in scratch, 170 us; all 8: 147; in fp16 6 leave 36 bytes there, 7 none, at the same time).
+constexpr int dkv_held(int maps, int ks, int ng) { return maps == 2 ? (ks >= 8 ? 3 : 0) : (ks == 8 && ng == 4 ? 7 : 0); }
 // two waves of the kernel on a SIMD
 constexpr bool dkv_two(int maps, int ks, int ng) { return (maps == 1 && ks <= 5) || (ng == 4 && (maps == 2 || ks <= 8)); }
 
 // ---- dK, dV: 32 keys per wave (pair; K and V rows in registers), tiles of QT queries of every head that shares them ------------
 template <typename T, int MAPS, int KS, int NT, int QT, int NG, int NS>
 __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void mapattn_dkv_kernel(const MapAttnArgs a) {
-  constexpr bool BIAS = MAPS == 1;
+  constexpr bool BIAS = MAPS == 1, SCALED = Num<T>::SCALED;
   constexpr int NW = NG * MAPS, BK = 32 * NG, DT = (KS + 1) / 2;
   constexpr int KSV = MAPS == 1 ? KS : NT;               // steps over this wave's share of dv in W
   constexpr int VT = MAPS == 1 ? NT : (NT + 1) / 2;      // 32-channel tiles of this wave's share of dV
@@ -527,6 +590,8 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
   u32x4 kf[KS], vf[KSV];
   load_row<KS>(kf, (const char*)a.k + 2 * (b * a.k_sb + (int64_t)key * a.k_st + (int64_t)(kvh * MAPS + m) * a.k_sh), valid, h, a.d);
   load_row<KSV, MAPS>(vf, (const char*)a.v + 2 * (b * a.v_sb + (int64_t)key * a.v_st + (int64_t)kvh * a.v_sh), valid, h, a.dv, m);
+  u32x4 vo[SCALED && MAPS == 2 ? KSV : 1];  // (fp16, two maps) the other wave's channels, for |V|
+  if (SCALED && MAPS == 2) load_row<SCALED && MAPS == 2 ? KSV : 1, MAPS>(vo, (const char*)a.v + 2 * (b * a.v_sb + (int64_t)key * a.v_st + (int64_t)kvh * a.v_sh), valid, h, a.dv, 1 - m);
 
 #pragma unroll
   for (int i = 0; i < KL; ++i) *(u32x4*)(klds + i * 1024) = kf[KS - KL + i];
@@ -578,8 +643,25 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
   for (int nt = 0; nt < VT; ++nt) dv[nt] = zero16();
   float far_lo = 0.f, far_hi = 0.f, lam = 0.f;
   constexpr float PF = 1.0f / (1 << Num<T>::PSH);
-
+  // (fp16) dS is rounded as 2^fe of itself: below 2^14 for all queries and the wave's keys, since |W| <= |dO| |V|, and as large as that allows
+  f32x2 most = {0.f, 0.f};
+  if (SCALED) {
+    const f32x2* z = a.sizes + ((int64_t)m * a.B * a.H + (int64_t)b * a.H + kvh * a.G) * a.QW;
+    for (int i = lane; i < a.G * a.QW; i += 64) {
+      const f32x2 x = z[i];
+      most[0] = fmaxf(most[0], x[0]), most[1] = fmaxf(most[1], x[1]);
+    }
+  }
   if (it0 < total) issue(it0);
+  int fe = 0;
+  if (SCALED) {
+    float v2 = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KSV; ++kk) v2 = squares<T>(vf[kk], MAPS == 2 ? squares<T>(vo[MAPS == 2 ? kk : 0], v2) : v2);
+    fe = __builtin_amdgcn_readfirstlane(power_to(fmaf(wave_most(most[0]), sqrtf(wave_most(xor32_sum(v2))), wave_most(most[1])), 14));
+  }
+  const float fs = power(fe);
+
   for (int it = it0; it < total; ++it) {
     const int g = it / per, t = tq0 + it - g * per;
     if (it == it0 || it - g * per == 0) {  // the next head: its bias, its lam
@@ -612,7 +694,19 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
       const int pq = pt + 32 * sub;
       f32x16 s[NS], w[NS];
 #pragma unroll
-      for (int i = 0; i < NS; ++i) s[i] = w[i] = zero16();
+      for (int i = 0; i < NS; ++i) {
+        s[i] = zero16();
+        if (MAPS == 2) {
+          w[i] = zero16();
+        } else {  // W - D at once
+#pragma unroll
+          for (int rq = 0; rq < 4; ++rq) {
+            const f32x4 D = *(const f32x4*)(rt + R_BYTES + (32 * (sub + i) + 8 * rq + 4 * h) * 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[i][4 * rq + e] = D[e];
+          }
+        }
+      }
       if (MAPS == 1 || !skip) {
 #pragma unroll
         for (int kk = 0; kk < KSV; ++kk)
@@ -683,18 +777,20 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
 #pragma unroll
         for (int nt = 0; nt < VT; ++nt)
           if (MAPS == 1 || NT % 2 == 0 || m * VT + nt < NT) dv[nt] = Num<T>::mfma(ot.get(st + MAPS * Q_BYTES, 2 * sub + kb2, nt), pv[kb2 >> 1][kb2 & 1], dv[nt]);
-      const float wf = m == 0 ? PF : -lam * PF, wd = m == 0 ? -1.f : lam;
+      const float wf = (m == 0 ? PF : -lam * PF) * fs, wd = (m == 0 ? -1.f : lam) * fs;
+      if (MAPS == 1) {
 #pragma unroll
-      for (int i = 0; i < NS; ++i)
+        for (int i = 0; i < NS; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[i][r] *= SCALED ? w[i][r] * wf : w[i][r];
+      } else {
 #pragma unroll
         for (int rq = 0; rq < 4; ++rq) {
-          const f32x4 D = *(const f32x4*)(rt + (MAPS + m) * R_BYTES + (32 * (sub + i) + 8 * rq + 4 * h) * 4);
+          const f32x4 D = *(const f32x4*)(rt + (MAPS + m) * R_BYTES + (8 * rq + 4 * h) * 4);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int r = 4 * rq + e;
-            s[i][r] *= MAPS == 1 ? fmaf(w[i][r], PF, -D[e]) : fmaf(w[i][r], wf, wd * D[e]);
-          }
+          for (int e = 0; e < 4; ++e) s[0][4 * rq + e] *= fmaf(w[0][4 * rq + e], wf, wd * D[e]);
         }
+      }
 #pragma unroll
       for (int kb2 = 0; kb2 < 2 * NS; ++kb2) {
         const f32x16& x = s[kb2 >> 1];
@@ -708,6 +804,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
   }
 
   if (key >= a.Tk) return;  // keys behind len get zeros
+  const float scale = a.scale * power(-fe);
   const int64_t row = ((int64_t)b * a.Tk + key) * a.Hkv + kvh;
   if (a.splits > 1) {  // 32-bit parts, (dk of each map, dv) of a key together
     float* pp = a.part_o + ((int64_t)split * a.B * a.Tk * a.Hkv + row) * (2 * a.dv);
@@ -717,7 +814,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
       for (int rq = 0; rq < 4; ++rq) {
         const int c0 = dt * 32 + rq * 8 + h * 4;
         const f32x16& x = dk[dt];
-        if (c0 < a.d) *(f32x4*)(pp + m * a.d + c0) = f32x4{x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale, x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale};
+        if (c0 < a.d) *(f32x4*)(pp + m * a.d + c0) = f32x4{x[4 * rq] * scale, x[4 * rq + 1] * scale, x[4 * rq + 2] * scale, x[4 * rq + 3] * scale};
       }
 #pragma unroll
     for (int nt = 0; nt < VT; ++nt)
@@ -737,7 +834,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
       const int c0 = dt * 32 + rq * 8 + h * 4;
       const f32x16& x = dk[dt];
       if (c0 < a.d)
-        *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * a.scale, x[4 * rq + 1] * a.scale), Num<T>::pack(x[4 * rq + 2] * a.scale, x[4 * rq + 3] * a.scale)};
+        *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * scale, x[4 * rq + 1] * scale), Num<T>::pack(x[4 * rq + 2] * scale, x[4 * rq + 3] * scale)};
     }
   op = (char*)a.dvo + row * a.dv * 2;
 #pragma unroll

@@ -1,0 +1,104 @@
+"""Root-mean-square errors of relative_attention, differential_attention and their gradients: what rounding leaves, and no more
+(limits derived in learned_attention_walk.py)."""
+import pytest
+import torch
+
+import learned_attention_walk as W
+
+DEV = "cuda"
+DTYPES = {"fp16": torch.float16, "bf16": torch.bfloat16}
+MAPS = pytest.mark.parametrize("maps", [1, 2], ids=["relative", "differential"])
+
+
+def rnd(*shape, dtype=torch.float32, scale=1.0, seed=0):
+    return (torch.randn(shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype)
+
+
+def inputs(maps, shape, dt, q=1.3, v=1.0, do=1.0, table=1.0, causal=False):
+    B, Tq, Tk, H, Hkv, d = shape
+    from aniportrait_amd import hipops
+    a = dict(q=rnd(B, Tq, maps * H, d, dtype=dt, scale=q, seed=1), k=rnd(B, Tk, maps * Hkv, d, dtype=dt, seed=2),
+             v=rnd(B, Tk, Hkv, maps * d, dtype=dt, scale=v, seed=3), do=rnd(B, Tq, H, maps * d, dtype=dt, scale=do, seed=4))
+    if maps == 1:
+        more = dict(table=rnd(H, 32, dtype=dt, scale=table, seed=5), buckets=hipops.relative_buckets(32, 128, not causal, device="cpu"))
+    else:
+        more = dict(lam=torch.rand(H, generator=torch.Generator().manual_seed(6)) * 0.6 + 0.2)
+    return a, more
+
+
+def step(maps, a, more, **kw):
+    """forward and backward on the GPU -> {name: tensor}"""
+    from aniportrait_amd import hipops as ops
+    a, more = {n: x.to(DEV) for n, x in a.items()}, [x.to(DEV) for x in more.values()]
+    do = a.pop("do")
+    fwd, bwd = (ops.relative_attention, ops.relative_attention_backward) if maps == 1 else (ops.differential_attention, ops.differential_attention_backward)
+    saved = fwd(*a.values(), *more, for_backward=True, **kw)
+    grads = bwd(do, *a.values(), *saved, *more, **kw)
+    return dict(zip(("out", "dq", "dk", "dv", "dtable" if maps == 1 else "dlam"), (saved[0], *grads)))
+
+
+def check(maps, a, more, got=None, exact_d=(), names=("out", "dq", "dk", "dv", "dtable"), causal=False):
+    got = got or step(maps, a, more, causal=causal)
+    want = W.attention(maps, **a, **more, causal=causal, exact_d=exact_d)
+    rel = {n: W.off(got[n], want[n], n) for n in names if n in want}
+    assert all(x <= W.LIMIT for x in rel.values()), rel
+
+
+@MAPS
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_limits_see_small_mistakes(maps, dtype):
+    """on the CPU: rounded values pass; values off by 1 %, one head's gradient lost from a shared key head, D left out of one row in
+    ten and a bucket without its gradient do not"""
+    a, more = inputs(maps, (1, 200, 200, 4, 2, 32), DTYPES[dtype], causal=True)
+    want = W.attention(maps, **a, **more, causal=True)
+    for n, (ref, _) in want.items():
+        good = ref.to(DTYPES[dtype])
+        assert W.off(good, want[n]) <= 1.0, n
+        if n != "dtable":   # (a few elements, which D's roundings reach: 1 % may be theirs)
+            assert W.off(good * 1.01, want[n]) > W.LIMIT, n
+    lost = want["dq"][0].clone()
+    lost[:, ::10] *= 0.9
+    assert W.off(lost, want["dq"]) > W.LIMIT
+    half = {n: x.clone() for n, x in a.items()}
+    half["do"][:, :, 0] *= 0.97
+    other = W.attention(maps, **half, **more, causal=True)
+    assert W.off(other["dk"][0], want["dk"]) > W.LIMIT and W.off(other["dv"][0], want["dv"]) > W.LIMIT
+    if maps == 1:
+        gone = want["dtable"][0].clone()
+        gone[0, 7] = 0
+        assert W.off(gone, want["dtable"]) > W.LIMIT
+
+
+SHAPES = [((2, 300, 300, 4, 2, 64), True), ((1, 900, 900, 2, 1, 80), True), ((1, 260, 400, 2, 2, 128), False), ((5, 40, 40, 2, 2, 40), False),
+          ((1, 20, 1000, 2, 1, 32), False), ((1, 600, 60, 2, 2, 96), False)]
+
+
+@pytest.mark.gpu
+@MAPS
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape,causal", SHAPES, ids=str)
+def test_errors_of_a_training_step(maps, shape, causal, dtype):
+    a, more = inputs(maps, shape, DTYPES[dtype], causal=causal)
+    check(maps, a, more, causal=causal)
+
+
+@pytest.mark.gpu
+@MAPS
+@pytest.mark.parametrize("do,v", [(1e-2, 1.0), (1e-3, 1.0), (1e-4, 1.0), (1e-5, 1.0), (8000.0, 1.0), (1.0, 100.0), (1.0, 1e-3), (1e-3, 300.0), (30.0, 3000.0)])
+@pytest.mark.parametrize("shape,causal", [((1, 1000, 1000, 4, 2, 64), True), ((1, 500, 700, 2, 2, 128), False), ((3, 45, 45, 2, 1, 40), False)], ids=str)
+def test_fp16_gradients_of_any_size(maps, shape, causal, do, v):
+    """small gradients keep their digits, large ones stay finite: dS is rounded as a power of two times itself"""
+    a, more = inputs(maps, shape, torch.float16, do=do, v=v, causal=causal)
+    check(maps, a, more, causal=causal, names=("dq", "dk", "dv"))
+
+
+@pytest.mark.gpu
+@MAPS
+def test_fp16_gradients_of_uneven_size(maps):
+    """rows and heads of very different gradients, and values that grow along the keys, in one call"""
+    a, more = inputs(maps, (2, 700, 700, 4, 2, 64), torch.float16)
+    a["do"] *= torch.logspace(-4, 3, 700)[None, :, None, None].half()
+    a["v"] *= torch.logspace(-3, 2.5, 700)[None, :, None, None].half()
+    check(maps, a, more, names=("dq", "dk", "dv"))
+    a["do"][:, :, 1:] *= 2.0 ** -7
+    check(maps, a, more, names=("dq", "dk", "dv"))
