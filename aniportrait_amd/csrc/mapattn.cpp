@@ -138,11 +138,11 @@ BwdLayout layout(const anip_attn_params* p, int maps) {
     const int64_t groups = (int64_t)p->B * l.QW * l.qsplits;
     l.parts = (int)(groups < 32 ? groups : 32);  // few query groups: their own sums are the parts
     l.diag = (int64_t)p->H * groups * (l.ND + 2);
-    if (l.qsplits > 1) l.rows3 = (int64_t)p->H * groups * 3 * 32;
     l.part = groups > 32 ? (int64_t)p->H * l.parts * (l.ND + 2) : 0;
   } else {
     l.dlam = (int64_t)p->H * p->B * l.QW * l.qsplits;
   }
+  if (l.qsplits > 1) l.rows3 = (int64_t)p->H * p->B * l.QW * l.qsplits * (maps == 1 ? 3 : 2) * 32;
   if (l.qsplits > 1) l.dq = (int64_t)l.qsplits * p->B * p->Tq * p->H * maps * p->d;
   if (l.ksplits > 1) l.dkv = (int64_t)l.ksplits * p->B * p->Tk * p->Hkv * 2 * maps * p->d;
   if (p->dtype == 0) l.sizes = (int64_t)p->B * p->H * maps * l.QW * 2;

@@ -36,8 +36,8 @@ struct MapAttnArgs {
   void *dq, *dk, *dvo, *dtable;
   float* dlam;
   int Tp;             // padded rows of rows_lse / rows_d
-  float* rows3;       // (split) [h][b][split][3][32 QW]: sum of dS, sums of P beyond -R and beyond R, of a row's part
-  float *rows_lse, *rows_d;  // [(b H + h) MAPS + m][Tp]: -lse in base 2 (-inf for rows without keys), D
+  float* rows3;       // (split) [h][b][split][3][32 QW]: sum of dS, sums of P beyond -R and beyond R, of a row's part; two maps: [..][2][32 QW], sums of P W
+  float *rows_lse, *rows_d;  // [(b H + h) MAPS + m][Tp]: -lse in base 2 (-inf for rows without keys), -D (two maps: 2^-PSH D)
   f32x2* sizes;       // (fp16) [m][b H + h][QW]: the largest |dO| and |D| of 32 rows, times the map's weight
   int QW, ND;         // 32-query groups per head; floats per group in diag
   float* diag;        // [h][b][group][ND + 2]: sums of dS along diagonals (+ below -R, above R)

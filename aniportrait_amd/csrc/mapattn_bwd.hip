@@ -4,7 +4,8 @@
 //   dlam = -sum P_2 W          dtable[bucket] = sum of dS over the pairs of the bucket
 // Two kernels, one that owns queries (dQ, dlam, dtable's partial sums) and one that owns keys (dK, dV): each recomputes P and W
 // (7 products instead of 5 at one map) and needs no atomics, so equal inputs give equal gradients.  P is recomputed from the row
-// statistics of the forward; D from dO and the stored outputs, or from P and W where a row's keys all lie in one step.  dS and P are rounded to the inputs' type as operands of the
+// statistics of the forward; D from dO and the stored outputs for dQ, or from P and W where a row's keys all lie in one step, and from P
+// and W of all its keys for dK.  dS and P are rounded to the inputs' type as operands of the
 // matrix products (off by 2^-8 or 2^-11 of a term at most, averaged over a row); all sums are 32-bit.  In fp16 both are rounded as a
 // power of two times themselves that follows the data, so that gradients of any size keep that precision.
 #include "mapattn.h"
@@ -126,10 +127,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
     }
     const float l = valid ? a.lse[((int64_t)bh * MAPS + m) * a.Tq + qi] * LOG2E : -INFINITY;
     nl = l == -INFINITY ? -INFINITY : -l;  // rows without keys: P = 2^-inf = 0
-    if (h == 0 && first) {
-      a.rows_lse[rows_at] = nl + Num<T>::PSH;
-      a.rows_d[rows_at] = MAPS == 1 ? -D : D * (1.0f / (1 << Num<T>::PSH));
-    }
+    if (h == 0 && first) a.rows_lse[rows_at] = nl + Num<T>::PSH;
   }
 
   // dS = wf P W + wd P, in fp16 2^fe times that.  dS is as large as P |dO| |V|, and fp16 keeps its precision from 2^-14 to 2^16: 2^fe
@@ -178,7 +176,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
   f32x16 dq[DT];
 #pragma unroll
   for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();
-  float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f, p_lo = 0.f, p_hi = 0.f, sum_near = 0.f, dl_sum = 0.f;
+  float far_lo = 0.f, far_hi = 0.f, sum_lo = 0.f, sum_hi = 0.f, p_lo = 0.f, p_hi = 0.f, sum_near = 0.f, pw_sum = 0.f;
   float dpos = 0.f, dneg = 0.f;  // diagonals rel = base + ql and base - 32 + ql of the current 32 keys, base = k0 - pw
   int next_base = 0;
   bool open = false;
@@ -217,7 +215,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
       wf = power(fe) * w0, wd = -wf * D;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();
-      sum_lo = sum_hi = p_lo = p_hi = sum_near = dl_sum = dpos = dneg = 0.f;
+      sum_lo = sum_hi = p_lo = p_hi = sum_near = pw_sum = dpos = dneg = 0.f;
       open = false;
       t = nt0;
       issue(t);
@@ -279,9 +277,8 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
         const f32x16 w2 = get16(theirs);
 #pragma unroll
         for (int r = 0; r < 16; ++r) w[0][r] += w2[r];
-        if (m == 1)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) dl_sum = fmaf(s[0][r], w[0][r], dl_sum);
+        for (int r = 0; r < 16; ++r) pw_sum = fmaf(s[0][r], w[0][r], pw_sum);
       }
       if (k0 == whole) {
         float pw1 = 0.f, p1 = 0.f;
@@ -295,7 +292,6 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
         pw1 = xor32_sum(pw1), p1 = xor32_sum(p1);
         D = p1 > 0.f ? pw1 / p1 : 0.f;
         wd = -wf * D;
-        if (h == 0) a.rows_d[rows_at] = MAPS == 1 ? -D : D * (1.0f / (1 << Num<T>::PSH));
       }
       auto total = [&] {
         float t = 0.f;
@@ -366,26 +362,35 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
     }
   }
 
+  // D for the keys' kernel from P and W themselves, in all rows: what D was off by is left over in the row's dS, whose sum is 0; two maps
+  // add P W.  Where few keys hold a row's weight W - D is small, and mostly what the rounding of the outputs made of D (bf16, queries of
+  // 8 times 1: dk 4.5e-3 off with D from the outputs, 2.4e-3 with this, whatever the queries' size; dQ, whose walk it ends, keeps 4.9e-3).
+  // Costs nothing where the walk is whole, and a launch of 3 us where it is split.
   const float fi = power(-fe);
+  sum_lo *= fi, sum_hi *= fi, sum_near *= fi;
+  const float left = xor32_sum(MAPS == 1 ? sum_lo + sum_hi + sum_near : pw_sum);
+  if (h == 0) {
+    if (a.splits == 1) a.rows_d[rows_at] = MAPS == 1 ? -(D + left) : left * (1.0f / (1 << Num<T>::PSH));
+    else if (first) a.rows_d[rows_at] = MAPS == 1 ? -D : 0.f;
+  }
+  // parts of rows: what is left over and the sums of P beyond -R and beyond R; two maps: the sums of P W
+  float* part = a.rows3 + ((((int64_t)head * a.B + b) * a.splits + split) * (MAPS == 1 ? 3 : 2) + m) * a.QW * 32 + q0 + ql;
+  if (a.splits > 1 && h == 0 && q0 < a.Tq) part[0] = left;
   if (BIAS && diag) {
-    sum_lo *= fi, sum_hi *= fi, sum_near *= fi;
     const float done = xor32_sum(dneg) * fi;
     if (open && h == 0) diag[next_base - 32 + ql + a.R + DIAG_PAD] = done;
     // What D is off by (the rounded outputs, the forward's rounded P) is what a row's dS leave over from their sum of 0.  It meets
     // a bucket with the row's P in it: with most of it, beyond the bias's reach, where it is taken out; with a few keys' up to
     // there, where it is small beside the roundings.  dtable in bf16, 2 heads, 2 x 3954: 2e-2 off with it, less than 4e-3 without;
     // it costs 8 us of 54 at 2 x 2048, 16 heads of 64 (two sums more over P and dS).
-    const float eps = xor32_sum(sum_lo + sum_hi + sum_near);
     if (a.splits == 1) {
-      sum_lo = fmaf(-eps, p_lo, sum_lo);
-      sum_hi = fmaf(-eps, p_hi, sum_hi);
+      sum_lo = fmaf(-left, p_lo, sum_lo);
+      sum_hi = fmaf(-left, p_hi, sum_hi);
     } else {  // (sum_table knows the whole row)
       const float pl = xor32_sum(p_lo), ph = xor32_sum(p_hi);
-      float* r3 = a.rows3 + (((int64_t)head * a.B + b) * a.splits + split) * 3 * a.QW * 32 + q0 + ql;
       if (h == 0) {
-        r3[0] = eps;
-        r3[a.QW * 32] = pl;
-        r3[a.QW * 64] = ph;
+        part[a.QW * 32] = pl;
+        part[a.QW * 64] = ph;
       }
     }
     const float lo = wave_sum(sum_lo), hi = wave_sum(sum_hi);
@@ -395,7 +400,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
     }
   }
   if (MAPS == 2 && m == 1 && q0 < a.Tq) {
-    const float t = wave_sum(dl_sum);
+    const float t = wave_sum(pw_sum);
     if (lane == 0) a.dlam_part[(((int64_t)head * a.B + b) * a.QW + q0 / 32) * a.splits + split] = -t;
   }
   if (!valid) return;
@@ -862,6 +867,24 @@ __global__ __launch_bounds__(256) void mapattn_join_kernel(const MapAttnArgs a) 
   *(u32x2*)op = u32x2{Num<T>::pack(t[0], t[1]), Num<T>::pack(t[2], t[3])};
 }
 
+// D of rows whose walk was split, one thread per row: see the queries' kernel
+template <int MAPS>
+__global__ __launch_bounds__(256) void mapattn_rows_kernel(const MapAttnArgs a, float unit) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int m = MAPS == 2 ? blockIdx.y : 0;
+  if (i >= (int64_t)a.B * a.H * a.Tq) return;
+  const int64_t bh = i / a.Tq;
+  const int q = (int)(i - bh * a.Tq), b = (int)(bh / a.H), head = (int)(bh - (int64_t)b * a.H);
+  constexpr int NR = MAPS == 1 ? 3 : 2;
+  const int64_t per = (int64_t)a.QW * 32;
+  const float* p = a.rows3 + (((int64_t)head * a.B + b) * a.qsplits * NR + m) * per + q;
+  float t = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < a.qsplits; ++s) t += p[s * NR * per];
+  float* d = a.rows_d + (bh * MAPS + m) * a.Tp + q;
+  *d = MAPS == 1 ? *d - t : t * unit;
+}
+
 // dtable of many query groups: part sums of the diagonals, block (slots, part, head), one thread per slot; then a workgroup per head
 __global__ __launch_bounds__(256) void mapattn_diag_kernel(const MapAttnArgs a) {
   const int slot = blockIdx.x * 256 + threadIdx.x, part = blockIdx.y, head = blockIdx.z;
@@ -967,6 +990,12 @@ int dkv_t(const MapAttnArgs& a, int maps, int nw, hipStream_t s) {
 
 int mapattn_dq(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) { return bf16 ? dq_t<bf16_t>(a, maps, nw, s) : dq_t<f16>(a, maps, nw, s); }
 int mapattn_dkv(const MapAttnArgs& a, int maps, int bf16, int nw, hipStream_t s) {
+  if (a.qsplits > 1) {
+    const dim3 rows((unsigned)cdiv64((int64_t)a.B * a.H * a.Tq, 256), (unsigned)maps);  // (fewer rows than the queries' kernel had threads)
+    if (maps == 1) hipLaunchKernelGGL(mapattn_rows_kernel<1>, rows, dim3(256), 0, s, a, 1.0f);
+    else hipLaunchKernelGGL(mapattn_rows_kernel<2>, rows, dim3(256), 0, s, a, bf16 ? 1.0f : 1.0f / (1 << Num<f16>::PSH));
+    ANIP_LAUNCH_CHECK("mapattn_rows_kernel");
+  }
   const int r = bf16 ? dkv_t<bf16_t>(a, maps, nw, s) : dkv_t<f16>(a, maps, nw, s);
   if (r || a.splits == 1) return r;
   const unsigned grid = mapattn_grid("mapattn_join_kernel", cdiv64((int64_t)a.B * a.Tk * a.Hkv * (a.dv / 2), 256), 256);

@@ -102,3 +102,19 @@ def test_fp16_gradients_of_uneven_size(maps):
     check(maps, a, more, names=("dq", "dk", "dv"))
     a["do"][:, :, 1:] *= 2.0 ** -7
     check(maps, a, more, names=("dq", "dk", "dv"))
+
+
+PEAKED = [dict(q=8.0), dict(q=16.0), dict(q=4.0, table=8.0)]   # rows whose weight few keys hold
+
+
+@pytest.mark.gpu
+@MAPS
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape,causal", [((1, 1000, 1000, 4, 4, 64), False), ((2, 900, 900, 1, 1, 64), False), ((1, 600, 600, 8, 2, 128), True),
+                                          ((20, 150, 150, 2, 2, 40), False)], ids=str)
+@pytest.mark.parametrize("sharp", PEAKED, ids=str)
+def test_keys_gradients_of_peaked_rows(maps, sharp, shape, causal, dtype):
+    """dk takes D from P and W themselves: what the saved outputs' rounding makes of D stays out of it, with whole and split walks"""
+    a, more = inputs(maps, shape, DTYPES[dtype], causal=causal, **sharp)
+    check(maps, a, more, causal=causal, names=("out", "dk", "dv"), exact_d=("dk",))
+    check(maps, a, more, causal=causal, names=("dq", "dtable"))
