@@ -173,7 +173,7 @@ __global__ __launch_bounds__(64 * QG * MAPS, 2) void mapattn_fwd_kernel(const Ma
 
   // ---- epilogue ---------------------------------------------------------------------------------------------------------
   const float l = xor32_sum(lrun);
-  const bool none = mrun == -INFINITY;  // no key seen: the row is zeros
+  const bool none = l == 0.f;  // no key seen: the row is zeros.  (Not where all scores are NaN: their sum is, while no maximum was set)
   const float inv = none ? 0.f : 1.0f / l;
   const float lse2 = none ? -INFINITY : mrun + __builtin_amdgcn_logf(l);
   if (MAPS == 2 && a.splits == 1) {
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(64 * MAXT * MAPS, (MAPS == 1 ? 2 : 1)) void mapattn
       mrun = all;
     }
   }
-  const bool none = mrun == -INFINITY;
+  const bool none = lrun == 0.f;
   const float inv = none ? 0.f : 1.0f / lrun;
   const float lse2 = none ? -INFINITY : mrun + __builtin_amdgcn_logf(lrun);
 #pragma unroll
@@ -491,7 +491,7 @@ __global__ __launch_bounds__(256) void mapattn_combine_kernel(const MapAttnArgs 
       sum += lw[m][i];
     }
     if (!SHORT) sum = wave_sum(sum);
-    const bool none = mx == -INFINITY;
+    const bool none = sum == 0.f;
     const float inv = none ? 0.f : 1.0f / sum;
     lse2[m] = none ? -INFINITY : base + __builtin_amdgcn_logf(sum);
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};

@@ -118,3 +118,27 @@ def test_keys_gradients_of_peaked_rows(maps, sharp, shape, causal, dtype):
     a, more = inputs(maps, shape, DTYPES[dtype], causal=causal, **sharp)
     check(maps, a, more, causal=causal, names=("out", "dk", "dv"), exact_d=("dk",))
     check(maps, a, more, causal=causal, names=("dq", "dtable"))
+
+
+@pytest.mark.gpu
+@MAPS
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape", [(2, 1, 300, 4, 2, 64), (1, 2, 9000, 2, 1, 64), (1, 3, 40000, 1, 1, 40), (300, 3, 40, 2, 2, 32), (2, 200, 200, 2, 2, 64),
+                                   (1, 70, 3000, 2, 2, 128)], ids=str)
+def test_nan_in_a_query_reaches_its_outputs(maps, shape, dtype):
+    """a row whose scores are all NaN is NaN, not one that sees no key; the other rows are as they were"""
+    from aniportrait_amd import hipops as ops
+    a, more = inputs(maps, shape, DTYPES[dtype], causal=True)
+    q, k, v = (a[n].to(DEV) for n in "qkv")
+    more = [x.to(DEV) for x in more.values()]
+    fwd = ops.relative_attention if maps == 1 else ops.differential_attention
+    want = fwd(q, k, v, *more, causal=True, for_backward=True)
+    bad = q.clone()
+    bad[-1, -1, -1, 3] = float("nan")
+    got = fwd(bad, k, v, *more, causal=True, for_backward=True)
+    assert got[0][-1, -1, -1].isnan().all() and got[-1][-1, -1, -1].isnan()
+    if maps == 2:
+        assert got[1][-1, -1, -1].isnan().all()
+    rest = torch.ones(got[0].shape[:3], dtype=torch.bool, device=DEV)
+    rest[-1, -1, -1] = False
+    assert torch.equal(got[0][rest], want[0][rest])
