@@ -666,6 +666,14 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
     fe = __builtin_amdgcn_readfirstlane(power_to(fmaf(wave_most(most[0]), sqrtf(wave_most(xor32_sum(v2))), wave_most(most[1])), 14));
   }
   const float fs = power(fe);
+  // (fp16, two maps) what meets dO in dV is up to 2^PSH (1 + |lam|) large: from |lam| = 127 on it is rounded as a part of itself
+  int pe = 0;
+  if (SCALED && MAPS == 2) {
+    float l = 0.f;
+    for (int g = 0; g < a.G; ++g) l = fmaxf(l, fabsf(a.lam[kvh * a.G + g]));
+    pe = min(0, __builtin_amdgcn_readfirstlane(power_to(1.0f + l, 15 - Num<T>::PSH)));
+  }
+  const float ps = power(pe);
 
   for (int it = it0; it < total; ++it) {
     const int g = it / per, t = tq0 + it - g * per;
@@ -677,7 +685,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
         far_lo = bias_at<T>(a, head, -a.R);
         far_hi = bias_at<T>(a, head, a.R);
       } else {
-        lam = a.lam[head];
+        lam = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(a.lam[head])));
       }
     }
     MAPATTN_WAIT_DMA();
@@ -763,7 +771,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
         if (!skip) put16(mine + 1024, s[0]);
         lds_barrier();
         if (skip) continue;
-        const float f1 = m == 0 ? 1.f : -lam, f2 = m == 0 ? -lam : 1.f;
+        const float f1 = ps * (m == 0 ? 1.f : -lam), f2 = ps * (m == 0 ? -lam : 1.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const f32x4 w2 = *(const f32x4*)(theirs + i * 256), p2 = *(const f32x4*)(theirs + 1024 + i * 256);
@@ -809,8 +817,10 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
   }
 
   if (key >= a.Tk) return;  // keys behind len get zeros
-  const float scale = a.scale * power(-fe);
-  const int64_t row = ((int64_t)b * a.Tk + key) * a.Hkv + kvh;
+  const float scale = a.scale * power(-fe), pf = PF * power(-pe);
+  int at = key;
+  opaque(at);  // (its 64-bit form of the loads above would wait through the walk)
+  const int64_t row = ((int64_t)b * a.Tk + at) * a.Hkv + kvh;
   if (a.splits > 1) {  // 32-bit parts, (dk of each map, dv) of a key together
     float* pp = a.part_o + ((int64_t)split * a.B * a.Tk * a.Hkv + row) * (2 * a.dv);
 #pragma unroll
@@ -827,7 +837,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
       for (int rq = 0; rq < 4; ++rq) {
         const int c0 = (m * VT + nt) * 32 + rq * 8 + h * 4;
         const f32x16& x = dv[nt];
-        if (c0 < a.dv) *(f32x4*)(pp + a.dv + c0) = f32x4{x[4 * rq] * PF, x[4 * rq + 1] * PF, x[4 * rq + 2] * PF, x[4 * rq + 3] * PF};
+        if (c0 < a.dv) *(f32x4*)(pp + a.dv + c0) = f32x4{x[4 * rq] * pf, x[4 * rq + 1] * pf, x[4 * rq + 2] * pf, x[4 * rq + 3] * pf};
       }
     return;
   }
@@ -849,7 +859,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
       const int c0 = (m * VT + nt) * 32 + rq * 8 + h * 4;
       const f32x16& x = dv[nt];
       if (c0 < a.dv)
-        *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * PF, x[4 * rq + 1] * PF), Num<T>::pack(x[4 * rq + 2] * PF, x[4 * rq + 3] * PF)};
+        *(u32x2*)(op + c0 * 2) = u32x2{Num<T>::pack(x[4 * rq] * pf, x[4 * rq + 1] * pf), Num<T>::pack(x[4 * rq + 2] * pf, x[4 * rq + 3] * pf)};
     }
 }
 

@@ -142,3 +142,12 @@ def test_nan_in_a_query_reaches_its_outputs(maps, shape, dtype):
     rest = torch.ones(got[0].shape[:3], dtype=torch.bool, device=DEV)
     rest[-1, -1, -1] = False
     assert torch.equal(got[0][rest], want[0][rest])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lam", [0.0, -3.0, 126.0, 129.0, 1000.0, -30000.0])
+def test_fp16_differential_attention_of_large_weights(lam):
+    """dv is finite where its values are, for any lam; two query heads of a key head with weights of their own"""
+    a, more = inputs(2, (1, 400, 400, 4, 2, 64), torch.float16, do=1.0 / (1 + abs(lam)), causal=True)
+    more["lam"] = torch.tensor([lam, 0.5, 0.1, lam])
+    check(2, a, more, causal=True)
