@@ -9,6 +9,7 @@ import ctypes as C
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -620,6 +621,7 @@ def temporal_qkv_attention(x, gamma, beta_pe, w_packed, B, F, T, heads, eps=1e-5
 
 
 # ---- heads with learned positions and maps: tensors (batch, token, head, channel), fp16 or bf16 -----------------------
+# Forward and backward are plain functions; inputs that torch tracks gradients of are refused where it is recording.
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 
@@ -676,6 +678,15 @@ def _aux(t, name, dtype, shape, like):
 def _new(t):
     """uninitialised, contiguous, of t's shape and type"""
     return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
+def _untracked(what, *tensors):
+    """these functions write plain buffers: a gradient that torch is to track through them would be lost without a word"""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what}: an input requires a gradient, which this call would not track: call it under torch.no_grad(), or "
+                           f"from an autograd.Function with its backward beside it")
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what}: an input carries a forward-mode tangent, which this call would not track")
 
 
 def _launch(t, call):
@@ -742,6 +753,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, rope=None, positions=None, eps=1e-6, 
     ref_attention(q_log2_scaled=True)).  interleaved: channel pairs (2 i, 2 i + 1) instead of (i, i + rot / 2).  q_out / k_out:
     where the results go, e.g. a slice of a cache, or the input itself.  Returns (q_out, k_out)."""
     lib = L.load()
+    _untracked("qk_norm_rope", q, k, q_weight, k_weight, rope, q_out, k_out)
     head = _qk_norm_fields(q, k, q_weight, k_weight, rope, positions, eps, interleaved, q_alpha)
     if q_out is None:
         q_out = _new(q)
@@ -774,6 +786,7 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, rope=None, p
     """gradients of qk_norm_rope: (dq, dk, dq_weight, dk_weight) from those of its outputs and its inputs; dq, dk contiguous in
     the inputs' type, the weights' in fp32.  k None: dk and dk_weight are None."""
     lib = L.load()
+    _untracked("qk_norm_rope_backward", dq_out, dk_out, q, k, q_weight, k_weight, rope)
     head = _qk_norm_fields(q, k, q_weight, k_weight, rope, positions, eps, interleaved, q_alpha)
     gq, gk, ko = _heads4(dq_out, "dq_out", q, q.shape), _NOWHERE, _NOWHERE
     dq, dk, dwk = _new(q), None, None
@@ -938,6 +951,7 @@ def relative_attention(q, k, v, table, buckets, causal=False, scale=None, kv_len
     key gets zeros.
     Returns out (B, Tq, H, d), or (out, lse) for_backward (lse (B, H, Tq) fp32)."""
     lib, what = L.load(), "relative_attention"
+    _untracked(what, q, k, v, table)
     fields = _attn_fields(what, 1, q, k, v, causal, scale, kv_lens, q_start)
     out, _, lse = _attention(what, 1, K_REL_ATTN, lib.anip_relative_attention, lib.anip_relative_attention_ws_bytes, q, k, v, fields,
                              _bias_fields(what, table, buckets, q, fields[4]), 0, for_backward)
@@ -948,6 +962,7 @@ def relative_attention_backward(dout, q, k, v, out, lse, table, buckets, causal=
     """gradients of relative_attention from that of its output, its inputs and what it returned for_backward:
     (dq, dk, dv, dtable), in the inputs' type; shared key heads' parts are added, keys behind kv_lens get zeros."""
     lib, what = L.load(), "relative_attention"
+    _untracked("relative_attention_backward", dout, q, k, v, out, lse, table)
     fields = _attn_fields(what, 1, q, k, v, causal, scale, kv_lens, q_start)
     bias = _bias_fields(what, table, buckets, q, fields[4])
     dtable = _new(table)
@@ -965,6 +980,7 @@ def differential_attention(q, k, v, lam, causal=False, scale=None, kv_lens=None,
     d <= 128.  The rest as relative_attention.  Returns out (B, Tq, H, 2 d), or (out, out2, lse) for_backward: out2 the second
     map's output, lse (B, 2 H, Tq) fp32."""
     lib, what = L.load(), "differential_attention"
+    _untracked(what, q, k, v, lam)
     fields = _attn_fields(what, 2, q, k, v, causal, scale, kv_lens, q_start)
     out, out2, lse = _attention(what, 2, K_DIFF_ATTN, lib.anip_differential_attention, lib.anip_differential_attention_ws_bytes, q, k, v,
                                 fields, _NO_BIAS, _aux(lam, "lam", F32, (fields[4],), q), for_backward)
@@ -975,6 +991,7 @@ def differential_attention_backward(dout, q, k, v, out, out2, lse, lam, causal=F
     """gradients of differential_attention from that of its output, its inputs and what it returned for_backward:
     (dq, dk, dv) in the inputs' type and dlam (H,) fp32."""
     lib, what = L.load(), "differential_attention"
+    _untracked("differential_attention_backward", dout, q, k, v, out, out2, lse, lam)
     fields = _attn_fields(what, 2, q, k, v, causal, scale, kv_lens, q_start)
     lp = _aux(lam, "lam", F32, (fields[4],), q)
     dlam = _new(lam)
