@@ -121,7 +121,7 @@ int walk_splits(int64_t blocks, int64_t tiles) {
 }
 
 struct BwdLayout {
-  int nwq, nwk, Tp, QW, ND, parts, qsplits, ksplits;
+  int nwq, nwk, Tp, QW, ND, DR, parts, qsplits, ksplits;
   int64_t rows, rows3, diag, dlam, part, dkv, dq, sizes, total;  // floats
 };
 BwdLayout layout(const anip_attn_params* p, int maps) {
@@ -134,7 +134,11 @@ BwdLayout layout(const anip_attn_params* p, int maps) {
   l.qsplits = walk_splits((int64_t)l.Tp / 32 * p->B * p->H / 4, (p->Tk + 63) / 64);
   l.ksplits = walk_splits((int64_t)((p->Tk + 31) / 32) * p->B * p->Hkv / 4, (int64_t)((p->Tq + 63) / 64) * (p->H / p->Hkv));
   if (maps == 1) {
-    l.ND = 2 * p->max_distance + 2 * mapattn::DIAG_PAD;
+    // the diagonals that exist: queries at the keys' end lie max(Tq, Tk) - 1 from any key; those of q_start may lie anywhere (1024 x 24,
+    // 8 heads, reach 4096: 8 MB of sums instead of 275)
+    const int far = p->Tq > p->Tk ? p->Tq : p->Tk;
+    l.DR = p->q_start != nullptr || p->max_distance < far ? p->max_distance : far;
+    l.ND = 2 * l.DR + 2 * mapattn::DIAG_PAD;
     const int64_t groups = (int64_t)p->B * l.QW * l.qsplits;
     l.parts = (int)(groups < 32 ? groups : 32);  // few query groups: their own sums are the parts
     l.diag = (int64_t)p->H * groups * (l.ND + 2);
@@ -159,7 +163,7 @@ int backward(const char* what, const anip_attn_params* p, int maps, int kid, voi
   MapAttnArgs a = args(p, maps);
   a.dout = p->dout, a.do_sb = p->dout_stride[0], a.do_st = token_stride(p->Tq, p->dout_stride), a.do_sh = p->dout_stride[2];
   a.dq = p->dq, a.dk = p->dk, a.dvo = p->dv, a.dtable = p->dtable, a.dlam = p->dlam;
-  a.Tp = l.Tp, a.QW = l.QW, a.ND = l.ND, a.parts = l.parts;
+  a.Tp = l.Tp, a.QW = l.QW, a.ND = l.ND, a.DR = l.DR, a.parts = l.parts;
   a.part_q = (float*)p->workspace;
   a.part_o = a.part_q + l.dq;
   a.rows_lse = a.part_o + l.dkv;

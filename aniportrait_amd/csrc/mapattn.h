@@ -39,7 +39,7 @@ struct MapAttnArgs {
   float* rows3;       // (split) [h][b][split][3][32 QW]: sum of dS, sums of P beyond -R and beyond R, of a row's part; two maps: [..][2][32 QW], sums of P W
   float *rows_lse, *rows_d;  // [(b H + h) MAPS + m][Tp]: -lse in base 2 (-inf for rows without keys), -D (two maps: 2^-PSH D)
   f32x2* sizes;       // (fp16) [m][b H + h][QW]: the largest |dO| and |D| of 32 rows, times the map's weight
-  int QW, ND;         // 32-query groups per head; floats per group in diag
+  int QW, ND, DR;     // 32-query groups per head; floats per group in diag; relative positions -DR .. DR that they hold (and DIAG_PAD beyond)
   float* diag;        // [h][b][group][ND + 2]: sums of dS along diagonals (+ below -R, above R)
   float* dlam_part;   // [h][b][group]
   float* diag_part;   // [h][parts][ND + 2]

@@ -344,7 +344,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
               dneg += ql <= ko ? 0.f : v;
             }
             const float done = xor32_sum(dneg);  // no later key reaches these 32 diagonals
-            if (diag && h == 0) diag[k0 + 32 * i - pw - 32 + ql + a.R + DIAG_PAD] = __builtin_amdgcn_ldexpf(done, -fe);
+            if (diag && h == 0) diag[k0 + 32 * i - pw - 32 + ql + a.DR + DIAG_PAD] = __builtin_amdgcn_ldexpf(done, -fe);
             dneg = dpos;
             dpos = 0.f;
           }
@@ -378,7 +378,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
   if (a.splits > 1 && h == 0 && q0 < a.Tq) part[0] = left;
   if (BIAS && diag) {
     const float done = xor32_sum(dneg) * fi;
-    if (open && h == 0) diag[next_base - 32 + ql + a.R + DIAG_PAD] = done;
+    if (open && h == 0) diag[next_base - 32 + ql + a.DR + DIAG_PAD] = done;
     // What D is off by (the rounded outputs, the forward's rounded P) is what a row's dS leave over from their sum of 0.  It meets
     // a bucket with the row's P in it: with most of it, beyond the bias's reach, where it is taken out; with a few keys' up to
     // there, where it is small beside the roundings.  dtable in bf16, 2 heads, 2 x 3954: 2e-2 off with it, less than 4e-3 without;
@@ -459,10 +459,10 @@ __device__ __forceinline__ void sum_table(const MapAttnArgs& a, int head, const 
 #pragma unroll
     for (int i = 0; i < 16; ++i) t[i] = i0 + i < parts && x < n ? p[(int64_t)(i0 + i) * n + x] : 0.f;
   };
-  // slot x < ND: relative position x - R - DIAG_PAD, beyond +-R as +-R; the last two: all pairs beyond -R, and beyond R
+  // slot x < ND: relative position x - DR - DIAG_PAD, beyond +-R as +-R; the last two: all pairs beyond -R, and beyond R
   auto bucket = [&](int x) {
-    int r = x - DIAG_PAD;
-    r = x == a.ND || r < 0 ? 0 : (r > 2 * a.R ? 2 * a.R : r);
+    int r = x - DIAG_PAD + a.R - a.DR;
+    r = x == a.ND || r < 0 ? 0 : (x > a.ND || r > 2 * a.R ? 2 * a.R : r);
     const int bx = x < n ? a.buckets[r] : -1;
     return x >= n ? -1 : (bx < 0 ? 0 : (bx >= a.NB ? a.NB - 1 : bx));
   };

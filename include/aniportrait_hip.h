@@ -265,7 +265,8 @@ int anip_qk_norm_rope_backward(const anip_qk_norm_params* p, void* stream);
  *   backward follows.
  * Backward: dq, dk, dv, dtable [H][n_buckets] (inputs' type) or dlam fp32 [H] from dout and the forward's out, out2, lse.  Keys
  *   behind kv_lens get zero gradients.  No atomics: equal inputs give equal gradients.
- * workspace: anip_*_ws_bytes(p, backward) bytes (0: none; < 0: error), 16-byte aligned. */
+ * workspace: anip_*_ws_bytes(p, backward) bytes (0: none; < 0: error), 16-byte aligned.  dtable takes 2 r + 194 floats of it for every
+ *   32 queries of a head (and part of a split walk), r = max_distance, at most max(Tq, Tk) where q_start is NULL. */
 typedef struct anip_attn_params {
   int dtype;
   int B, Tq, Tk, H, Hkv, d, causal;

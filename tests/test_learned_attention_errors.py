@@ -1,5 +1,7 @@
 """Root-mean-square errors of relative_attention, differential_attention and their gradients: what rounding leaves, and no more
 (limits derived in learned_attention_walk.py)."""
+import ctypes as C
+
 import pytest
 import torch
 
@@ -151,3 +153,35 @@ def test_fp16_differential_attention_of_large_weights(lam):
     a, more = inputs(2, (1, 400, 400, 4, 2, 64), torch.float16, do=1.0 / (1 + abs(lam)), causal=True)
     more["lam"] = torch.tensor([lam, 0.5, 0.1, lam])
     check(2, a, more, causal=True)
+
+
+def test_workspace_of_short_sequences_with_a_far_reach():
+    """dtable's sums take the diagonals that the sequences have, not those of the reach"""
+    from aniportrait_amd import _lib as L
+    lib = L.load()
+    p = L.AttnParams()
+    p.dtype, p.B, p.Tq, p.Tk, p.H, p.Hkv, p.d, p.scale = 1, 1024, 24, 24, 8, 8, 64, 0.125
+    for n in ("q", "k", "v", "out", "table", "buckets"):
+        setattr(p, n, 256)
+    for n in ("q_stride", "k_stride", "v_stride"):
+        setattr(p, n, (24 * 512, 512, 64))
+    p.n_buckets, p.max_distance = 32, 4096
+    tensor = p.B * p.Tq * p.H * p.d * 2
+    far = lib.anip_relative_attention_ws_bytes(C.byref(p), 1)
+    assert 0 < far <= 2 * tensor
+    p.max_distance = 24
+    assert lib.anip_relative_attention_ws_bytes(C.byref(p), 1) == far
+    p.q_start, p.max_distance = 256, 4096         # (positions of the caller's: any may occur)
+    assert lib.anip_relative_attention_ws_bytes(C.byref(p), 1) > 10 * far
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("reach", [1, 30, 31, 70, 129, 4096])
+@pytest.mark.parametrize("shape,causal", [((40, 20, 20, 2, 1, 32), True), ((3, 70, 30, 2, 2, 64), False), ((2, 30, 300, 2, 2, 128), True),
+                                          ((1, 129, 129, 2, 2, 160), False), ((1, 1, 70, 4, 1, 64), False), ((1, 700, 700, 1, 1, 48), False)], ids=str)
+def test_table_gradient_of_any_reach(shape, causal, reach):
+    """reaches below, at and beyond the distances that the sequences have"""
+    a, more = inputs(1, shape, torch.float16, causal=causal)
+    r = torch.arange(-reach, reach + 1)
+    more["buckets"] = ((r * 7) % 32).int()        # neighbours in different buckets
+    check(1, a, more, causal=causal)
