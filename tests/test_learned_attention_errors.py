@@ -185,3 +185,75 @@ def test_table_gradient_of_any_reach(shape, causal, reach):
     r = torch.arange(-reach, reach + 1)
     more["buckets"] = ((r * 7) % 32).int()        # neighbours in different buckets
     check(1, a, more, causal=causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_gradients_at_the_end_of_a_layer(dtype):
+    """norm and rotation -> both attentions -> norm of the heads' difference, and back to the projection's rows and all weights: against
+    64-bit differentiation of the whole chain.  Each of its up to six roundings in turn (heads, P, output, its norm, the gradients
+    between) leaves u / sqrt(3) of a value at most in the mean, errors in D as much again"""
+    from aniportrait_amd import hipops as ops
+    dt = DTYPES[dtype]
+    B, T = 2, 150
+    x, g = rnd(B, T, 512, dtype=dt, seed=1), rnd(B, T, 512, dtype=dt, seed=2)
+    w = dict(wq=rnd(64, scale=0.2, seed=3) + 1, wk=rnd(64, scale=0.2, seed=4) + 1, wo=rnd(128, scale=0.2, seed=5) + 1, table=rnd(4, 32, dtype=dt, seed=6),
+             lam=torch.tensor([0.2, 0.6]))
+    rope, buckets = ops.rope_table(T, 64, device="cpu"), ops.relative_buckets(32, 128, False, device="cpu")
+
+    # the framework's operators
+    d = {n: t.to(DEV) for n, t in w.items()}
+    xd, gd, rd, bd = x.to(DEV), g.to(DEV), rope.to(DEV), buckets.to(DEV)
+    q, k, v = xd[..., :256].unflatten(-1, (4, 64)), xd[..., 256:384].unflatten(-1, (2, 64)), xd[..., 384:].unflatten(-1, (2, 64))
+    vd = xd[..., 384:].unflatten(-1, (1, 128))
+    qn, kn = ops.qk_norm_rope(q, k, d["wq"], d["wk"], rd)
+    out, lse = ops.relative_attention(qn, kn, v, d["table"], bd, causal=True, for_backward=True)
+    od, od2, lsed = ops.differential_attention(qn, kn, vd, d["lam"], causal=True, for_backward=True)
+    on, _ = ops.qk_norm_rope(od, None, d["wo"], None)
+    g1, g2 = gd[..., :256].unflatten(-1, (4, 64)), gd[..., 256:].unflatten(-1, (2, 128))
+    god, _, dwo, _ = ops.qk_norm_rope_backward(g2, None, od, None, d["wo"], None)
+    r = ops.relative_attention_backward(g1, qn, kn, v, out, lse, d["table"], bd, causal=True)
+    s = ops.differential_attention_backward(god, qn, kn, vd, od, od2, lsed, d["lam"], causal=True)
+    dq, dk, dwq, dwk = ops.qk_norm_rope_backward(r[0] + s[0], r[1] + s[1], q, k, d["wq"], d["wk"], rd)
+    dx = torch.cat([dq.flatten(2), dk.flatten(2), r[2].flatten(2) + s[2].flatten(2)], -1)
+    got = dict(x=dx, wq=dwq, wk=dwk, wo=dwo, table=r[3], lam=s[3], y=torch.cat([out.flatten(2), on.flatten(2)], -1))
+
+    # the definition
+    p = {n: t.double().requires_grad_() for n, t in dict(w, x=x).items()}
+    turn = torch.view_as_complex(rope.double())[:, None]
+
+    def norm(h, weight):
+        return h * (h.pow(2).mean(-1, keepdim=True) + 1e-6).rsqrt() * weight
+
+    def rotate(h):
+        z = torch.complex(*h.chunk(2, -1)) * turn
+        return torch.cat([z.real, z.imag], -1)
+    q, k = p["x"][..., :256].unflatten(-1, (4, 64)), p["x"][..., 256:384].unflatten(-1, (2, 64))
+    v, vd = p["x"][..., 384:].unflatten(-1, (2, 64)), p["x"][..., 384:].unflatten(-1, (1, 128))
+    qn, kn = rotate(norm(q, p["wq"])), rotate(norm(k, p["wk"]))
+    rel = torch.arange(T)[None] - torch.arange(T)[:, None]
+
+    def maps(qh, kh, bias):
+        z = torch.einsum("bihc,bjhc->bhij", qh, kh) / 8 + bias
+        return z.masked_fill(rel > 0, -float("inf")).softmax(-1)
+    P = maps(qn, kn.repeat_interleave(2, 2), p["table"][:, buckets.long()[rel.clamp(-128, 128) + 128]])
+    y1 = torch.einsum("bhij,bjhc->bihc", P, v.repeat_interleave(2, 2))
+    A = [maps(qn[:, :, m::2], kn[:, :, m::2].expand(-1, -1, 2, -1), 0.0) for m in (0, 1)]
+    o2 = torch.einsum("bhij,bjhc->bihc", A[1], vd.expand(-1, -1, 2, -1))
+    o = torch.einsum("bhij,bjhc->bihc", A[0], vd.expand(-1, -1, 2, -1)) - p["lam"][:, None] * o2
+    y2 = norm(o, p["wo"])
+    y = torch.cat([y1.flatten(2), y2.flatten(2)], -1)
+    *grads, go = torch.autograd.grad(y, [*p.values(), o], g.double())
+    want = dict(zip(p, grads), y=y.detach())
+    limit = 2 * (6 / 3) ** 0.5 * torch.finfo(dt).eps / 2
+    # dlam = -sum go o2 over 38400 terms a head, whose roundings add up as the root of their squares while they cancel themselves: the
+    # norm's gradient go is at right angles to o in every row, and o2 lies mostly along o
+    size = {n: ref.norm() for n, ref in want.items()}
+    size["lam"] = (go * o2).norm()
+    assert size["lam"] > 2 * want["lam"].norm()
+    rel_err = {n: ((got[n].cpu().double() - ref).norm() / size[n]).item() for n, ref in want.items()}
+    for part, sl in (("dq", slice(0, 256)), ("dk", slice(256, 384)), ("dv", slice(384, 512))):
+        rel_err[part] = ((got["x"].cpu().double() - want["x"])[..., sl].norm() / want["x"][..., sl].norm()).item()
+    assert all(e <= limit for e in rel_err.values()), (limit, rel_err)
+    # a hand-over that drops one attention's gradient is seen: it is ten times the limit at least
+    assert (r[0].norm() / dq.norm()).item() > 10 * limit and (s[0].norm() / dq.norm()).item() > 10 * limit
