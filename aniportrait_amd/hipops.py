@@ -944,7 +944,7 @@ def relative_attention(q, k, v, table, buckets, causal=False, scale=None, kv_len
 
     q (B, Tq, H, d), k, v (B, Tk, Hkv, d), fp16 / bf16, H a multiple of Hkv (query heads h .. share key head h / (H / Hkv)),
     d <= 160; table (H, n_buckets) in the same type; buckets from relative_buckets, or any int32 (2 R + 1) of the buckets of the
-    relative positions -R .. R (R <= 4096; further ones take the ends').  scale: default d^-1/2.  kv_lens (B,) int32: keys behind
+    relative positions -R .. R (R <= 4096; further ones take the ends').  A bias of -inf (or bf16's lowest) hides its pairs.  scale: default d^-1/2.  kv_lens (B,) int32: keys behind
     it are not seen, whatever they hold (padded batch, cache).  q_start (B,) int32: the position of query 0 (default Tk - Tq: the
     queries are the last tokens); causal: query i sees keys up to q_start + i, and what lies behind the last query's is not read
     either (a later token's inf or NaN may reach the queries before it: it enters their sums times zero).  A query that sees no

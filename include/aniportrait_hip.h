@@ -253,7 +253,7 @@ int anip_qk_norm_rope_backward(const anip_qk_norm_params* p, void* stream);
 /* anip_relative_attention — o_i = softmax_j(scale q_i.k_j + table[h][buckets[clamp(j - p_i, +-max_distance) + max_distance]]) v_j
  *   q (B, Tq, H, d), k, v (B, Tk, Hkv, d), H a multiple of Hkv (query head h reads key head h / (H / Hkv)), d a multiple of 8 up
  *   to 160; table [H][n_buckets] in the inputs' type, buckets int32 [2 max_distance + 1] (max_distance <= 4096; entries outside
- *   [0, n_buckets) are clamped).
+ *   [0, n_buckets) are clamped).  A bias of -inf, or one that log2 e takes there (bf16's lowest), hides its pairs.
  * anip_differential_attention — o_i = (softmax_j(scale q1_i.k1_j) - lam[h] softmax_j(scale q2_i.k2_j)) v_j
  *   q (B, Tq, 2 H, d), k (B, Tk, 2 Hkv, d): heads 2 h and 2 h + 1 are the two maps of head h; v (B, Tk, Hkv, 2 d), lam fp32 [H],
  *   d a multiple of 8 up to 128; out (B, Tq, H, 2 d).

@@ -257,3 +257,19 @@ def test_gradients_at_the_end_of_a_layer(dtype):
     assert all(e <= limit for e in rel_err.values()), (limit, rel_err)
     # a hand-over that drops one attention's gradient is seen: it is ten times the limit at least
     assert (r[0].norm() / dq.norm()).item() > 10 * limit and (s[0].norm() / dq.norm()).item() > 10 * limit
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 200, 230, 2, 2, 64), (2, 3, 230, 4, 2, 40), (1, 900, 900, 1, 1, 64)], ids=str)
+def test_lowest_bias_of_bf16_hides(shape):
+    """bf16's lowest value times log2 e is beyond 32 bits: it hides its pairs as -inf does, and rows without others are zeros"""
+    a, more = inputs(1, shape, torch.bfloat16)
+    res = []
+    for low in (torch.finfo(torch.bfloat16).min, -float("inf")):
+        table = more["table"].clone()
+        table[:, ::3] = low
+        table[0, :] = low
+        res.append(step(1, a, dict(more, table=table), q_start=torch.full((shape[0],), 5, dtype=torch.int32, device=DEV)))
+    for n in res[0]:
+        assert torch.equal(res[0][n], res[1][n]) and res[0][n].isfinite().all(), n
+    assert res[0]["out"][:, :, 0].abs().max() == 0 and res[0]["dq"][:, :, 0].abs().max() == 0 and res[0]["dtable"][0].abs().max() == 0
