@@ -132,13 +132,15 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
 
   // dS = wf P W + wd P, in fp16 2^fe times that.  dS is as large as P |dO| |V|, and fp16 keeps its precision from 2^-14 to 2^16: 2^fe
   // brings the largest |dO| of the wave's rows to 2^8.  That is room for weights of 2^-20 beside values of about 1, and for values of up
-  // to about 50.  If larger ones overflow it, the walk is done again with room for any (a maximum of dS in every step instead: dQ at
-  // 2 x 2048, 16 / 4 heads of 64, 70 us against 65).
+  // to about 50.  If larger ones overflow it, the walk is done again with room for 128 times larger ones, and for any (a maximum of dS in
+  // every step instead: dQ at 2 x 2048, 16 / 4 heads of 64, 70 us against 65).
   const float w0 = MAPS == 2 && m == 1 ? -lam : 1.f;
-  int fe = 0;
-  bool again = false;
+  int fe = 0, again = 0;
+  bool finite = true;  // (rows of NaN or infinities keep them to themselves)
   if (SCALED) {
-    const float most = sqrtf(wave_most(xor32_sum(n2))) * fabsf(w0), mostD = wave_most(fabsf(D)) * fabsf(w0);
+    n2 = xor32_sum(n2);
+    finite = fabsf(n2) < INFINITY && fabsf(D) < INFINITY && nl == nl;
+    const float most = sqrtf(wave_most(finite ? n2 : 0.f)) * fabsf(w0), mostD = wave_most(finite ? fabsf(D) : 0.f) * fabsf(w0);
     fe = __builtin_amdgcn_readfirstlane(power_to(most, 8));
     if (first && lane == 0 && q0 < a.Tq) a.sizes[((int64_t)m * a.B * a.H + bh) * a.QW + q0 / 32] = f32x2{most, mostD};
   }
@@ -193,7 +195,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
   if (nt0 < nt_all) issue(nt0);
   for (int t = nt0;; ++t) {
     if (t >= nt_all) {
-      if (!SCALED || again || nt0 >= nt_all) break;
+      if (!SCALED || again == 2 || nt0 >= nt_all) break;
       // an infinity among the rounded dS leaves one, or NaN, in dQ
       float bad[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -201,7 +203,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
 #pragma unroll
         for (int r = 0; r < 16; ++r) bad[r & 3] = fmaf(dq[dt][r], 0.f, bad[r & 3]);
       int* over = (int*)smem;
-      const int mine_over = __any((bad[0] + bad[1]) + (bad[2] + bad[3]) != 0.f);
+      const int mine_over = __any(finite && (bad[0] + bad[1]) + (bad[2] + bad[3]) != 0.f);
       lds_barrier();  // all tiles read
       if (lane == 0) over[wave] = mine_over;
       lds_barrier();
@@ -210,8 +212,8 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
       for (int i = 0; i < NW; ++i) any |= over[i];
       if (!__builtin_amdgcn_readfirstlane(any)) break;
       lds_barrier();  // all flags read
-      again = true;
-      fe -= 14;  // |W| and |D| are at most |dO| 2^16 sqrt(256): with |dO| at 2^-6 dS stays below 2^15
+      ++again;
+      if (mine_over) fe -= 7;  // |W| and |D| are at most |dO| 2^16 sqrt(256): with |dO| at 2^-6, the second time, dS stays below 2^15
       wf = power(fe) * w0, wd = -wf * D;
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) dq[dt] = zero16();

@@ -273,3 +273,30 @@ def test_lowest_bias_of_bf16_hides(shape):
     for n in res[0]:
         assert torch.equal(res[0][n], res[1][n]) and res[0][n].isfinite().all(), n
     assert res[0]["out"][:, :, 0].abs().max() == 0 and res[0]["dq"][:, :, 0].abs().max() == 0 and res[0]["dtable"][0].abs().max() == 0
+
+
+@pytest.mark.gpu
+@MAPS
+@pytest.mark.parametrize("odd", ["large", "nan", "inf", "nan query"])
+def test_fp16_rows_beside_an_odd_one(maps, odd):
+    """a query whose gradient passes fp16's range, or is none, leaves the other waves' rows of its workgroup their precision; NaN also its own wave's"""
+    a, more = inputs(maps, (1, 400, 400, 2, 2, 64), torch.float16)
+    if odd == "large":       # its dS reaches 1e6
+        a["do"][0, 5] *= 2000
+        a["v"][0, 7] *= 300
+        a["q"][0, 5] = a["k"][0, 7] * 2
+    want = W.attention(maps, **a, **more)
+    bad = {n: x.clone() for n, x in a.items()}
+    if odd in ("nan", "inf"):
+        bad["do"][0, 5, :, 3] = float(odd)
+    elif odd == "nan query":
+        bad["q"][0, 5, :, 3] = float("nan")
+    got = step(maps, bad, more)
+    rest = torch.arange(400) >= 32 if odd == "large" else torch.arange(400) != 5
+    for lo, hi in ((0, 128), (128, 400)):
+        part = rest & (torch.arange(400) >= lo) & (torch.arange(400) < hi)
+        e = W.off(got["dq"][:, part], tuple(x[:, part] for x in want["dq"]))
+        assert e <= W.LIMIT, (lo, e)
+    if odd != "large":
+        assert got["dq"][0, 5].isnan().all()
+        assert got["out"][0, 6:].isfinite().all()
