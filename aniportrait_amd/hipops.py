@@ -682,9 +682,11 @@ def _new(t):
 
 def _untracked(what, *tensors):
     """these functions write plain buffers: a gradient that torch is to track through them would be lost without a word"""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what}: an input requires a gradient, which this call would not track: call it under torch.no_grad(), or "
-                           f"from an autograd.Function with its backward beside it")
+    if torch.is_grad_enabled():
+        for t in tensors:   # (any() takes half as long again)
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what}: an input requires a gradient, which this call would not track: call it under "
+                                   f"torch.no_grad(), or from an autograd.Function with its backward beside it")
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f"{what}: an input carries a forward-mode tangent, which this call would not track")
 

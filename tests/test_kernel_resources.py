@@ -34,3 +34,16 @@ def test_learned_attention_keeps_its_registers(kernels):
     assert len(mine) > 80, sorted(kernels)[:5]
     spilled = {n: k["vgpr_spill_count"] for n, k in mine.items() if k["vgpr_spill_count"]}
     assert not spilled, spilled
+
+
+@pytest.mark.parametrize("name,maps", [("void mapattn_rows_kernel<2>(MapAttnArgs, float)", 2), ("_Z19mapattn_rows_kernelILi2EEv11MapAttnArgsf", 2),
+                                       ("void mapattn_rows_kernel<1>(MapAttnArgs, float)", 1), ("_Z19mapattn_rows_kernelILi1EEv11MapAttnArgsf", 1),
+                                       ("_Z17mapattn_dq_kernelIDF16bLi2ELi8ELi8ELi32ELi4ELi1EEv11MapAttnArgs", 2),
+                                       ("_Z17mapattn_dq_kernelIDF16_Li1ELi4ELi2ELi64ELi4ELi2EEv11MapAttnArgs", 1)])
+def test_counter_summaries_tell_one_map_from_two(name, maps):
+    import importlib.util
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "tools", "pmc_summarize.py")
+    spec = importlib.util.spec_from_file_location("pmc_summarize", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.family(name) == ("relative_attention_kernels", "differential_attention_kernels")[maps - 1]

@@ -49,7 +49,7 @@ def family(name):
         if key in name:
             return fam
     if "mapattn" in name:               # one map or two: the first number of the template (c++filt trips over bf16, hence "int, EL"); the join of split gradients has none
-        m = re.search(r"mapattn_\w+?_kernel(?:IDF16[_b]Li|<[^,]*, )(\d)", name)
+        m = re.search(r"mapattn_\w+?_kernel(?:IDF16[_b]Li|ILi|<(?:[^,>]*, )?)(\d)", name)
         return "differential_attention_kernels" if (m and m.group(1) == "2") or "int, EL" in name else "relative_attention_kernels"
     if any(k in name for k in ("add_kernel", "window_accumulate", "cfg_ddim", "ncfhw", "nhwc", "u8_to_f16", "f16_to_u8")):
         return "elementwise"
