@@ -140,7 +140,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, (NG == 4 || (MAPS == 1 && KS <= 8) 
   if (SCALED) {
     n2 = xor32_sum(n2);
     finite = fabsf(n2) < INFINITY && fabsf(D) < INFINITY && nl == nl;
-    const float most = sqrtf(wave_most(finite ? n2 : 0.f)) * fabsf(w0), mostD = wave_most(finite ? fabsf(D) : 0.f) * fabsf(w0);
+    const float most = __builtin_amdgcn_sqrtf(wave_most(finite ? n2 : 0.f)) * fabsf(w0), mostD = wave_most(finite ? fabsf(D) : 0.f) * fabsf(w0);
     fe = __builtin_amdgcn_readfirstlane(power_to(most, 8));
     if (first && lane == 0 && q0 < a.Tq) a.sizes[((int64_t)m * a.B * a.H + bh) * a.QW + q0 / 32] = f32x2{most, mostD};
   }
@@ -597,8 +597,6 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
   u32x4 kf[KS], vf[KSV];
   load_row<KS>(kf, (const char*)a.k + 2 * (b * a.k_sb + (int64_t)key * a.k_st + (int64_t)(kvh * MAPS + m) * a.k_sh), valid, h, a.d);
   load_row<KSV, MAPS>(vf, (const char*)a.v + 2 * (b * a.v_sb + (int64_t)key * a.v_st + (int64_t)kvh * a.v_sh), valid, h, a.dv, m);
-  u32x4 vo[SCALED && MAPS == 2 ? KSV : 1];  // (fp16, two maps) the other wave's channels, for |V|
-  if (SCALED && MAPS == 2) load_row<SCALED && MAPS == 2 ? KSV : 1, MAPS>(vo, (const char*)a.v + 2 * (b * a.v_sb + (int64_t)key * a.v_st + (int64_t)kvh * a.v_sh), valid, h, a.dv, 1 - m);
 
 #pragma unroll
   for (int i = 0; i < KL; ++i) *(u32x4*)(klds + i * 1024) = kf[KS - KL + i];
@@ -650,6 +648,7 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
   for (int nt = 0; nt < VT; ++nt) dv[nt] = zero16();
   float far_lo = 0.f, far_hi = 0.f, lam = 0.f;
   constexpr float PF = 1.0f / (1 << Num<T>::PSH);
+  if (it0 < total) issue(it0);
   // (fp16) dS is rounded as 2^fe of itself: below 2^14 for all queries and the wave's keys, since |W| <= |dO| |V|, and as large as that allows
   f32x2 most = {0.f, 0.f};
   if (SCALED) {
@@ -659,13 +658,17 @@ __global__ __launch_bounds__(64 * NG * MAPS, dkv_two(MAPS, KS, NG) ? 2 : 1) void
       most[0] = fmaxf(most[0], x[0]), most[1] = fmaxf(most[1], x[1]);
     }
   }
-  if (it0 < total) issue(it0);
   int fe = 0;
   if (SCALED) {
     float v2 = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < KSV; ++kk) v2 = squares<T>(vf[kk], MAPS == 2 ? squares<T>(vo[MAPS == 2 ? kk : 0], v2) : v2);
-    fe = __builtin_amdgcn_readfirstlane(power_to(fmaf(wave_most(most[0]), sqrtf(wave_most(xor32_sum(v2))), wave_most(most[1])), 14));
+    for (int kk = 0; kk < KSV; ++kk) v2 = squares<T>(vf[kk], v2);
+    if (MAPS == 2) {  // the other half of the channels
+      mine[0] = v2;
+      lds_barrier();
+      v2 += theirs[0];
+    }
+    fe = __builtin_amdgcn_readfirstlane(power_to(fmaf(wave_most(most[0]), __builtin_amdgcn_sqrtf(wave_most(xor32_sum(v2))), wave_most(most[1])), 14));
   }
   const float fs = power(fe);
   // (fp16, two maps) what meets dO in dV is up to 2^PSH (1 + |lam|) large: from |lam| = 127 on it is rounded as a part of itself
